@@ -14,7 +14,8 @@ LIB = os.path.join(PKG, "libadmm_hip.so")
 HIP_SOURCES = ["ctx.hip", "csr.hip", "copies.hip", "forward_rows.hip", "forward_panels.hip", "transposed.hip", "solver.hip", "ftrl_batch.hip", "ftrl.hip",
                "auc.hip", "comm.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-HIP_FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-munsafe-fp-atomics", "-ffp-contract=off",
+# packed float operations stay off: some of their forms have given wrong results on this hardware now and then
+HIP_FLAGS = ["-O3", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-munsafe-fp-atomics", "-ffp-contract=off",
              "-Wall", "-Wno-unused-function", "-Wno-unused-value", "-Wno-unused-result",
              "-I", os.path.join(ROOT, "include"), "-I", CSRC]
 
@@ -26,19 +27,20 @@ def _newer(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def _compile(src):
+def _compile(src, force=False):
     obj = os.path.join(OBJ, os.path.splitext(src)[0] + ".o")
-    deps = [os.path.join(CSRC, src), os.path.join(CSRC, "internal.h"), os.path.join(CSRC, "sweep_common.h"),
+    deps = [os.path.join(CSRC, src), os.path.join(CSRC, "internal.h"), os.path.join(CSRC, "sweep_common.h"), os.path.abspath(__file__),
             os.path.join(ROOT, "include", "admm_hip.h")]
-    if _newer(obj, deps):
+    if force or _newer(obj, deps):
         subprocess.check_call([HIPCC] + HIP_FLAGS + ["-c", os.path.join(CSRC, src), "-o", obj])
     return obj
 
 
-def build_lib(verbose=False):
+def build_lib(verbose=False, force=False):
+    """compiles what is older than its sources (force: everything) and links the library"""
     os.makedirs(OBJ, exist_ok=True)
     with ThreadPoolExecutor(max_workers=min(6, os.cpu_count() or 2)) as ex:
-        objs = list(ex.map(_compile, HIP_SOURCES))
+        objs = list(ex.map(lambda src: _compile(src, force), HIP_SOURCES))
     if _newer(LIB, objs):
         subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-shared", "-o", LIB] + objs + ["-ldl"])
     if verbose:
