@@ -12,7 +12,7 @@ OBJ = os.path.join(PKG, "csrc", "_obj")
 LIB = os.path.join(PKG, "libadmm_hip.so")
 
 HIP_SOURCES = ["ctx.hip", "csr.hip", "copies.hip", "forward_rows.hip", "forward_panels.hip", "transposed.hip", "solver.hip", "ftrl_batch.hip", "ftrl.hip",
-               "auc.hip", "comm.hip"]
+               "auc.hip", "comm.hip", "embed.hip", "softmax.hip", "sample.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # packed float operations stay off: some of their forms have given wrong results on this hardware now and then
 HIP_FLAGS = ["-O3", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-munsafe-fp-atomics", "-ffp-contract=off",
@@ -29,7 +29,7 @@ def _newer(target, deps):
 
 def _compile(src, force=False):
     obj = os.path.join(OBJ, os.path.splitext(src)[0] + ".o")
-    deps = [os.path.join(CSRC, src), os.path.join(CSRC, "internal.h"), os.path.join(CSRC, "sweep_common.h"), os.path.abspath(__file__),
+    deps = [os.path.join(CSRC, src), os.path.join(CSRC, "internal.h"), os.path.join(CSRC, "sweep_common.h"), os.path.join(CSRC, "rows_common.h"), os.path.abspath(__file__),
             os.path.join(ROOT, "include", "admm_hip.h")]
     if force or _newer(obj, deps):
         subprocess.check_call([HIPCC] + HIP_FLAGS + ["-c", os.path.join(CSRC, src), "-o", obj])

@@ -24,9 +24,17 @@ SYMBOLS = [
     "admm_predict", "admm_metrics", "admm_auc_scores", "admm_tied_ranks", "admm_csr_copy_labels", "admm_ftrl_pass", "admm_ftrl_predict", "admm_ftrl_update", "admm_ftrl_pass_multi", "admm_logistic_fg", "admm_lbfgs_solve",
     "admm_payload", "admm_global_update", "admm_dual_update", "admm_consensus", "admm_consensus_static",
     "admm_comm_unique_id", "admm_comm_init", "admm_allreduce_sum_f32", "admm_comm_selftest",
+    "admm_csr_bags", "admm_embed", "admm_embed_order_bytes", "admm_embed_order", "admm_embed_grad_workspace", "admm_embed_grad",
+    "admm_softmax_loss_workspace", "admm_softmax_loss", "admm_sample_workspace", "admm_sample",
 ]
 
-K_FORWARD, K_TRANSPOSED, K_FTRL_SEQ, K_ELEMENTWISE, K_FORWARD_EVAL = 0, 1, 2, 3, 4
+K_FORWARD, K_TRANSPOSED, K_FTRL_SEQ, K_ELEMENTWISE, K_FORWARD_EVAL, K_EMBED, K_SOFTMAX, K_SAMPLE = range(8)
+
+# element types of matrices, ids and labels
+F32, BF16, F16, I32, I64 = range(5)
+_BYTES = (4, 2, 2, 4, 8)
+# a context's stream: the device's default stream (None lets the library make one of its own)
+DEFAULT_STREAM = 1
 
 
 class AdmmError(RuntimeError):
@@ -48,6 +56,19 @@ class LbfgsParams(C.Structure):
 class LbfgsResult(C.Structure):
     _fields_ = [("f", C.c_double), ("evals", C.c_int), ("iters", C.c_int),
                 ("forward_sweeps", C.c_int), ("transposed_sweeps", C.c_int)]
+
+
+class MatStruct(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("rows", C.c_uint64), ("cols", C.c_uint64), ("stride", C.c_uint64), ("type", C.c_int)]
+
+
+class BagsStruct(C.Structure):
+    _fields_ = [("ids", C.c_void_p), ("rowptr", C.c_void_p), ("val", C.c_void_p), ("nrows", C.c_uint64),
+                ("nnz", C.c_uint64), ("id_type", C.c_int)]
+
+
+class SampleParamsStruct(C.Structure):
+    _fields_ = [("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p)]
 
 
 _lib = None
@@ -117,6 +138,16 @@ def load():
         "admm_comm_init": [vp, i32, i32, vp],
         "admm_allreduce_sum_f32": [vp, vp, u64],
         "admm_comm_selftest": [vp],
+        "admm_csr_bags": [vp, vp],
+        "admm_embed": [vp, vp, vp, f32, vp],
+        "admm_embed_order_bytes": [vp, u64, C.POINTER(u64)],
+        "admm_embed_order": [vp, vp, u64, vp, u64],
+        "admm_embed_grad_workspace": [vp, u64, C.POINTER(u64)],
+        "admm_embed_grad": [vp, vp, vp, u64, vp, f32, i32, vp, vp, u64],
+        "admm_softmax_loss_workspace": [u64, u64, C.POINTER(u64)],
+        "admm_softmax_loss": [vp, vp, vp, i32, vp, f32, vp, vp, vp, vp, u64],
+        "admm_sample_workspace": [u64, u64, C.POINTER(u64)],
+        "admm_sample": [vp, vp, vp, vp, vp, vp, vp, u64],
     }
     for name, args in sig.items():
         fn = getattr(L, name)
@@ -178,9 +209,85 @@ class DeviceVec:
             self.ptr = None
 
 
+class DeviceBuf:
+    """bytes in HBM (workspaces, orders, integer arrays)"""
+
+    def __init__(self, ctx, nbytes):
+        self.vec = DeviceVec(ctx, max(1, (int(nbytes) + 3) // 4))
+        self.nbytes = int(nbytes)
+        self.ptr = self.vec.ptr
+
+    def free(self):
+        self.vec.free()
+        self.ptr = None
+
+
+_TORCH = {}  # torch's types, once torch is used
+
+
+def _torch_type(dtype):
+    if not _TORCH:
+        import torch
+        _TORCH.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, torch.int32: I32, torch.int64: I64})
+        for name in ("uint32", "uint64"):
+            if hasattr(torch, name):
+                _TORCH[getattr(torch, name)] = I32 if name == "uint32" else I64
+    return _TORCH.get(dtype)
+
+
+class DeviceMat:
+    """A row-major matrix in HBM (admm_mat): from a pointer, or `of` a torch tensor on the context's GPU"""
+
+    def __init__(self, ptr, rows, cols, type=F32, stride=None):
+        self.struct = MatStruct(int(ptr), int(rows), int(cols), int(cols if stride is None else stride), int(type))
+        self.ref = C.byref(self.struct)
+
+    @property
+    def shape(self):
+        return self.struct.rows, self.struct.cols
+
+    @classmethod
+    def of(cls, ctx, m, name):
+        if isinstance(m, DeviceMat):
+            return m
+        if not hasattr(m, "data_ptr"):
+            raise AdmmError("%s: a DeviceMat or a torch tensor is needed, not %s" % (name, m.__class__.__name__))
+        kind = _torch_type(m.dtype)
+        if kind not in (F32, BF16, F16):
+            raise AdmmError("%s: float32, bfloat16 or float16 is needed, not %s" % (name, m.dtype))
+        ctx._here(m, name)
+        if m.dim() != 2:
+            raise AdmmError("%s: a matrix is needed, not %d dimensions" % (name, m.dim()))
+        rows, cols = m.shape
+        step, inner = m.stride()
+        if cols > 1 and inner != 1:
+            raise AdmmError("%s: the elements of a row lie %d apart: they have to be adjacent" % (name, inner))
+        if rows > 1 and step < cols:
+            raise AdmmError("%s: rows of %d elements lie %d apart" % (name, cols, step))
+        return cls(m.data_ptr(), rows, cols, kind, max(step, cols))
+
+
+class Bags:
+    """Rows of ids (admm_bags); keeps the arrays alive"""
+
+    def __init__(self, struct, keep=()):
+        self.struct, self.keep = struct, keep
+        self.ref = C.byref(struct)
+
+    @property
+    def nrows(self):
+        return self.struct.nrows
+
+    @property
+    def nnz(self):
+        return self.struct.nnz
+
+
 class Context:
     def __init__(self, device=0, stream=None):
         self.L = load()
+        self.device = int(device)
+        self._scratch, self._retired = None, []
         h = C.c_void_p()
         _check(self.L.admm_ctx_create(int(device), C.c_void_p(stream) if stream else None,
                                       C.byref(h)))
@@ -190,6 +297,9 @@ class Context:
 
     def close(self):
         if self.h:
+            for b in self._retired + ([self._scratch] if self._scratch is not None else []):
+                b.free()
+            self._scratch, self._retired = None, []
             self.L.admm_ctx_destroy(self.h)
             self.h = None
 
@@ -281,6 +391,131 @@ class Context:
         _check(self.L.admm_ftrl_update(self.h, _ptr(idx), idx.shape[0], float(label), float(predict), w.ptr, z.ptr,
                                        n.ptr, alpha))
 
+    # models with many classes or tokens -----------------------------------------------------
+    # Matrices are torch tensors or DeviceMats, arrays are torch tensors, DeviceVecs or DeviceBufs; what they point to
+    # belongs to this context's GPU, and the work is queued on this context's stream (make the context on the stream that
+    # the tensors are used on: Context(device, stream=torch.cuda.current_stream().cuda_stream or DEFAULT_STREAM)).
+    def _here(self, t, name):
+        if t.device.type != "cuda" or t.device.index != self.device:
+            raise AdmmError("%s is on %s, the context on GPU %d" % (name, t.device, self.device))
+
+    def _array(self, a, name, count, kinds):
+        """(pointer, type) of `count` adjacent elements of one of the types"""
+        if a is None:
+            return None, kinds[0]
+        if isinstance(a, DeviceVec):
+            if F32 not in kinds or a.n < count:
+                raise AdmmError("%s: %d floats do not do for %d elements" % (name, a.n, count))
+            return a.ptr, F32
+        if isinstance(a, DeviceBuf):
+            if a.nbytes < count * _BYTES[kinds[0]]:
+                raise AdmmError("%s: %d bytes do not do for %d elements" % (name, a.nbytes, count))
+            return a.ptr, kinds[0]
+        kind = _torch_type(a.dtype)
+        if kind not in kinds:
+            raise AdmmError("%s: elements of type %s" % (name, a.dtype))
+        self._here(a, name)
+        if a.numel() < count or not a.is_contiguous():
+            raise AdmmError("%s: %d adjacent elements are needed, it has %s with strides %s" %
+                            (name, count, tuple(a.shape), tuple(a.stride())))
+        return a.data_ptr(), kind
+
+    def _bytes(self, buf, name):
+        if isinstance(buf, DeviceBuf):
+            return buf.ptr, buf.nbytes
+        self._here(buf, name)
+        if not buf.is_contiguous():
+            raise AdmmError("%s: not contiguous" % name)
+        return buf.data_ptr(), buf.numel() * buf.element_size()
+
+    def _workspace(self, given, need):
+        """the caller's workspace, or one that the context keeps for calls without: it grows, and what it outgrew stays until
+        close(), for graphs that were captured with it"""
+        if given is not None:
+            return self._bytes(given, "workspace")
+        if need == 0:
+            return None, 0
+        if self._scratch is None or self._scratch.nbytes < need:
+            if self._scratch is not None:
+                self._retired.append(self._scratch)
+            self._scratch = None
+            self._scratch = DeviceBuf(self, (need + (need >> 2) + 4095) // 4096 * 4096)
+        return self._scratch.ptr, self._scratch.nbytes
+
+    def buf(self, nbytes):
+        return DeviceBuf(self, nbytes)
+
+    def bags(self, ids, rowptr=None, val=None):
+        """Rows of ids for embed / embed_grad: one per row, or with row pointers (nrows + 1 int64) and factors"""
+        if not hasattr(ids, "data_ptr"):
+            raise AdmmError("ids: a torch tensor is needed")
+        nnz = ids.numel()
+        p, kind = self._array(ids, "ids", nnz, (I32, I64))
+        nrows, q, f = nnz, None, None
+        if rowptr is not None:
+            nrows = rowptr.numel() - 1
+            if nrows < 0:
+                raise AdmmError("rowptr: no element")
+            q, _ = self._array(rowptr, "rowptr", nrows + 1, (I64,))
+        if val is not None:
+            f, _ = self._array(val, "val", nnz, (F32,))
+        return Bags(BagsStruct(p or None, q, f, nrows, nnz, kind), (ids, rowptr, val))
+
+    def embed(self, bags, table, out, scale=1.0):
+        """admm_embed: out[r] = scale * sum of val_e * table[id_e] over the entries of row r"""
+        _check(self.L.admm_embed(self.h, bags.ref, DeviceMat.of(self, table, "table").ref, scale, DeviceMat.of(self, out, "out").ref))
+
+    def embed_order_bytes(self, bags, table_rows):
+        n = C.c_uint64()
+        _check(self.L.admm_embed_order_bytes(bags.ref, int(table_rows), C.byref(n)))
+        return n.value
+
+    def embed_order(self, bags, table_rows, order=None):
+        """admm_embed_order: the entries sorted by id, into `order` (a DeviceBuf or a torch tensor of bytes; made if None)"""
+        if order is None:
+            order = DeviceBuf(self, self.embed_order_bytes(bags, table_rows))
+        p, n = self._bytes(order, "order")
+        _check(self.L.admm_embed_order(self.h, bags.ref, int(table_rows), p, n))
+        return order
+
+    def embed_grad(self, bags, order, grad_out, grad_table, scale=1.0, accumulate=False, workspace=None):
+        """admm_embed_grad: the gradient with respect to the table, written whole or added to"""
+        src, to = DeviceMat.of(self, grad_out, "grad_out"), DeviceMat.of(self, grad_table, "grad_table")
+        p, n = self._bytes(order, "order")
+        need = C.c_uint64()
+        _check(self.L.admm_embed_grad_workspace(bags.ref, src.struct.cols, C.byref(need)))
+        w, wn = self._workspace(workspace, need.value)
+        _check(self.L.admm_embed_grad(self.h, bags.ref, p, n, src.ref, scale, 1 if accumulate else 0, to.ref, w, wn))
+
+    def softmax_loss(self, logits, labels, loss, grad=None, lse=None, weight=None, grad_scale=1.0, workspace=None):
+        """admm_softmax_loss: loss per row, and with `grad` (may be the logits) grad_scale times its gradient"""
+        x = DeviceMat.of(self, logits, "logits")
+        g = None if grad is None else DeviceMat.of(self, grad, "grad")
+        rows = x.struct.rows
+        t, kind = self._array(labels, "labels", rows, (I32, I64, F32))
+        w, _ = self._array(weight, "weight", rows, (F32,))
+        o, _ = self._array(loss, "loss", rows, (F32,))
+        e, _ = self._array(lse, "lse", rows, (F32,))
+        need = C.c_uint64()
+        _check(self.L.admm_softmax_loss_workspace(rows, x.struct.cols, C.byref(need)))
+        ws, wn = self._workspace(workspace, need.value)
+        _check(self.L.admm_softmax_loss(self.h, x.ref, t, kind, w, grad_scale, o, e, None if g is None else g.ref, ws, wn))
+
+    def sample(self, logits, uniform, token, logprob=None, temperature=None, top_k=None, top_p=None, min_p=None, workspace=None):
+        """admm_sample: a class per row into `token` (int32), the log of its probability into `logprob`"""
+        x = DeviceMat.of(self, logits, "logits")
+        rows = x.struct.rows
+        u, _ = self._array(uniform, "uniform", rows, (F32,))
+        t, _ = self._array(token, "token", rows, (I32,))
+        lp, _ = self._array(logprob, "logprob", rows, (F32,))
+        given = [self._array(a, name, rows, (kind,))[0] for a, name, kind in
+                 ((temperature, "temperature", F32), (top_k, "top_k", I32), (top_p, "top_p", F32), (min_p, "min_p", F32))]
+        params = SampleParamsStruct(*given)
+        need = C.c_uint64()
+        _check(self.L.admm_sample_workspace(rows, x.struct.cols, C.byref(need)))
+        ws, wn = self._workspace(workspace, need.value)
+        _check(self.L.admm_sample(self.h, x.ref, C.byref(params), u, t, lp, ws, wn))
+
     # consensus algebra --------------------------------------------------------------------
     def payload(self, x, ydual, rho, out):
         _check(self.L.admm_payload(self.h, x.ptr, ydual.ptr, rho, out.ptr, x.n))
@@ -365,6 +600,12 @@ class SampleSet:
         _check(self.ctx.L.admm_csr_download(self.h, _ptr(rowptr), _ptr(col), _ptr(val),
                                             _ptr(label)))
         return rowptr, col[:self.nnz], val[:self.nnz], label[:self.nrows]
+
+    def bags(self):
+        """the set's rows as bags for Context.embed / embed_grad (admm_csr_bags)"""
+        b = BagsStruct()
+        _check(self.ctx.L.admm_csr_bags(self.h, C.byref(b)))
+        return Bags(b, (self,))
 
     def build_transposed(self, panel_rows=0, col_block=0):
         _check(self.ctx.L.admm_csr_build_transposed(self.h, int(panel_rows), int(col_block)))

@@ -418,7 +418,9 @@ extern "C" int admm_ctx_create(int device, void *stream, admm_ctx **out) {
   ctx->device = device;
   hipDeviceProp_t prop;
   if (hipGetDeviceProperties(&prop, device) == hipSuccess) ctx->cu_count = prop.multiProcessorCount;
-  if (stream) {
+  if (stream == ADMM_STREAM_DEFAULT) {
+    ctx->stream = nullptr;
+  } else if (stream) {
     ctx->stream = (hipStream_t)stream;
   } else {
     if (hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking) != hipSuccess) {
@@ -454,7 +456,7 @@ extern "C" int admm_ctx_create(int device, void *stream, admm_ctx **out) {
 extern "C" int admm_ctx_destroy(admm_ctx *ctx) {
   if (!ctx) return ADMM_OK;
   hipSetDevice(ctx->device);
-  if (ctx->stream) hipStreamSynchronize(ctx->stream);
+  if (ctx->stream || !ctx->own_stream) hipStreamSynchronize(ctx->stream);
   for (auto &s : ctx->pending) {
     hipEventDestroy(s.start);
     hipEventDestroy(s.stop);

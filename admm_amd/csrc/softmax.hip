@@ -1,0 +1,323 @@
+// Softmax loss with its gradient: the many-class form of the logistic loss and its residuals.
+//
+// With L = log2(e) and m the row's largest logit, the exponentials are 2^(x L - m L) (one fused multiply-add and one
+// hardware exp2 each), s their sum, and
+//   loss = ln 2 (log2 s - (x_t L - m L)),  grad = exp2(x L - (m L + log2 s)) w - [j = t] w.
+// Both read x L - m L through the same rounded m L, so its rounding cancels.  Where m L would overflow (a mask of the type's
+// lowest value over a whole row), 1 takes the place of L: logits of that size are equal or more than 2^100 apart.
+#include "rows_common.h"
+
+namespace admm_impl {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct SoftmaxArgs {
+  const void *logits;
+  void *grad;  // or NULL; may be the logits
+  uint64_t stride, gstride, rows, cols;
+  const void *labels;
+  int label_type;
+  const float *weight;  // or NULL
+  float grad_scale;
+  float *loss, *lse;  // lse or NULL
+  int lanes_log2;
+  int apart;  // the gradient's rows are aligned otherwise than the logits': written element by element
+};
+
+// the row's label, -1 where it is not trained on; w: its weight
+__device__ inline int64_t label_of(const SoftmaxArgs &a, uint64_t r, float &w) {
+  w = a.weight ? a.weight[r] : 1.0f;
+  int64_t t;
+  if (a.label_type == ADMM_I64) {
+    t = static_cast<const int64_t *>(a.labels)[r];
+  } else if (a.label_type == ADMM_I32) {
+    t = static_cast<const int32_t *>(a.labels)[r];
+  } else {
+    const float f = static_cast<const float *>(a.labels)[r];
+    t = f > -1.0f && f < 9.0e18f ? (int64_t)f : -1;
+  }
+  return t >= 0 && (uint64_t)t < a.cols && w != 0.0f ? t : -1;
+}
+
+__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// largest element of a chunk, NaN aside
+template <class T>
+__device__ inline float chunk_max(const vec_t<T, 16 / sizeof(T)> &x, float m) {
+#pragma unroll
+  for (int k = 0; k < (int)(16 / sizeof(T)); ++k) m = fmaxf(m, (float)x[k]);
+  return m;
+}
+
+// what is taken off a row's exponents: x l - m2
+struct Shift {
+  float l, m2;
+  explicit __device__ Shift(float m) {
+    l = fabsf(m) < 0x1p126f || m == -INFINITY ? kLog2e : 1.0f;
+    m2 = m == -INFINITY ? 0.0f : m * l;  // without a class every power is 2^(-inf - 0) = 0
+  }
+};
+
+template <class T>
+__device__ inline float chunk_sum(const vec_t<T, 16 / sizeof(T)> &x, Shift b) {
+  float s = 0.0f;
+#pragma unroll
+  for (int k = 0; k < (int)(16 / sizeof(T)); ++k) s += exp2_fast(__fmaf_rn((float)x[k], b.l, -b.m2));
+  return s;
+}
+
+// Keeps a chunk in its 16 bytes between two uses: without it the compiler holds the unpacked floats instead, twice the
+// registers, and spills.
+template <class V>
+__device__ inline void stay_packed(V &x) {
+  u32x4 u = __builtin_bit_cast(u32x4, x);
+  asm volatile("" : "+v"(u));
+  x = __builtin_bit_cast(V, u);
+}
+
+// the gradient of a chunk; `at`: which of its elements the label is, or anything else
+template <class T>
+__device__ inline vec_t<T, 16 / sizeof(T)> chunk_grad(const vec_t<T, 16 / sizeof(T)> &x, float l, float lse2, float g, int64_t at) {
+  constexpr int K = 16 / sizeof(T);
+  float v[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = g * exp2_fast(__fmaf_rn((float)x[k], l, -lse2));
+  if (at >= 0 && at < K) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] -= at == k ? g : 0.0f;
+  }
+  vec_t<T, K> y;
+#pragma unroll
+  for (int k = 0; k < K; ++k) y[k] = (T)v[k];
+  return y;
+}
+
+// loss and lse of a row with the label t, and what its gradient takes: lse2 (so that p = 2^(x l - lse2))
+__device__ inline void finish_row(const SoftmaxArgs &a, uint64_t r, Shift b, float s, int64_t t, float w, float xt, bool writes, float &lse2) {
+  const float log2s = __log2f(s);  // -inf where no class is left
+  lse2 = b.m2 + log2s;
+  if (!writes) return;
+  const float nats = b.l == 1.0f ? 1.0f : kLn2;
+  if (a.lse) a.lse[r] = s == 0.0f ? -INFINITY : b.m2 * nats + log2s * kLn2;
+  a.loss[r] = t < 0 ? 0.0f : s == 0.0f ? INFINITY * w : w * (kLn2 * log2s - nats * __fmaf_rn(xt, b.l, -b.m2));
+}
+
+// Rows of up to 64 CH chunks: 2^lanes_log2 lanes hold a row, CH chunks each, and reduce it among themselves.
+template <class T, int CH>
+__global__ void __launch_bounds__(256) k_softmax_lanes(SoftmaxArgs a) {
+  constexpr int K = 16 / sizeof(T);
+  const unsigned lanes = 1u << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
+  const uint64_t per = 256u >> a.lanes_log2;
+  const T none = (T)-INFINITY;
+  for (uint64_t r = (uint64_t)blockIdx.x * per + (threadIdx.x >> a.lanes_log2); r < a.rows; r += (uint64_t)gridDim.x * per) {
+    float w;
+    const int64_t t = label_of(a, r, w);
+    const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, a.cols);
+    T *to = a.grad ? static_cast<T *>(a.grad) + r * a.gstride : nullptr;
+    vec_t<T, K> x[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+      if (c * lanes + lane < row.count) x[c] = row.load(c * lanes + lane, none);
+      else x[c] = none;
+    const float xt = t >= 0 ? (float)row.base[row.lead + t] : 0.0f;
+    float m = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) m = chunk_max<T>(x[c], m);
+    for (unsigned off = 1; off < lanes; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    const Shift b(m);
+    float s = 0.0f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) stay_packed(x[c]);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) s += chunk_sum<T>(x[c], b);
+    for (unsigned off = 1; off < lanes; off <<= 1) s += __shfl_xor(s, off, 64);
+    float lse2;
+    finish_row(a, r, b, s, t, w, xt, lane == 0, lse2);
+    if (!to) continue;
+    const float g = t < 0 ? 0.0f : w * a.grad_scale;
+    const int64_t tc = t < 0 ? -1 : t + row.lead;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) stay_packed(x[c]);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int64_t at = c * lanes + lane;
+      if (at >= row.count) continue;
+      const vec_t<T, K> zero = (T)0.0f;
+      row.store(to, a.apart, at, t < 0 || s == 0.0f ? zero : chunk_grad<T>(x[c], b.l, lse2, g, tc - at * K));
+    }
+  }
+}
+
+template <int NT>
+__device__ inline float block_max(float v, float *sh) {
+  for (int off = 1; off < 64; off <<= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = sh[0];
+#pragma unroll
+  for (int i = 1; i < NT / 64; ++i) v = fmaxf(v, sh[i]);
+  return v;
+}
+
+template <int NT>
+__device__ inline float block_sum(float v, float *sh) {
+  for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = sh[0];
+#pragma unroll
+  for (int i = 1; i < NT / 64; ++i) v += sh[i];
+  return v;
+}
+
+// Rows of any length, one workgroup each, CH chunks a thread kept in registers (CH > 0) or read again (CH == 0).
+template <class T, int NT, int CH>
+__global__ void __launch_bounds__(NT) k_softmax_block(SoftmaxArgs a) {
+  constexpr int K = 16 / sizeof(T);
+  __shared__ float sh[2][NT / 64];
+  const T none = (T)-INFINITY;
+  for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    float w;
+    const int64_t t = label_of(a, r, w);
+    const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, a.cols);
+    T *to = a.grad ? static_cast<T *>(a.grad) + r * a.gstride : nullptr;
+    const vec_t<T, K> zero = (T)0.0f;
+    if (t < 0 && !a.lse) {  // nothing of the row is needed
+      if (to)
+        for (int64_t c = threadIdx.x; c < row.count; c += NT) row.store(to, a.apart, c, zero);
+      if (threadIdx.x == 0) a.loss[r] = 0.0f;
+      continue;
+    }
+    const float xt = t >= 0 ? (float)row.base[row.lead + t] : 0.0f;  // before anyone writes over it
+    vec_t<T, K> x[CH ? CH : 1];
+    float m = -INFINITY, s = 0.0f;
+    Shift b(m);
+    if (CH) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        if (c * NT + threadIdx.x < row.count) x[c] = row.load(c * NT + threadIdx.x, none);
+        else x[c] = none;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) m = chunk_max<T>(x[c], m);
+      m = block_max<NT>(m, sh[0]);
+      b = Shift(m);
+#pragma unroll
+      for (int c = 0; c < CH; ++c) stay_packed(x[c]);
+#pragma unroll
+      for (int c = 0; c < CH; ++c) s += chunk_sum<T>(x[c], b);
+    } else {
+      // one pass: the sum is kept relative to the running maximum
+      for (int64_t c = threadIdx.x; c < row.count; c += NT) {
+        const vec_t<T, K> y = row.load(c, none);
+        const float mc = chunk_max<T>(y, m);
+        if (mc > m) {
+          const Shift next(mc);
+          s *= m == -INFINITY ? 1.0f : exp2_fast(b.m2 - next.m2);  // s is 0 (or NaN) while no class was seen
+          m = mc;
+          b = next;
+        }
+        s += chunk_sum<T>(y, b);
+      }
+      const float mine = m, was = b.m2;
+      m = block_max<NT>(m, sh[0]);
+      b = Shift(m);
+      if (mine != -INFINITY) s *= exp2_fast(was - b.m2);
+    }
+    s = block_sum<NT>(s, sh[1]);
+    float lse2;
+    finish_row(a, r, b, s, t, w, xt, threadIdx.x == 0, lse2);
+    if (to) {
+      const float g = t < 0 ? 0.0f : w * a.grad_scale;
+      const int64_t tc = t < 0 ? -1 : t + row.lead;
+      const bool no = t < 0 || s == 0.0f;
+      if (CH) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) stay_packed(x[c]);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const int64_t at = c * NT + threadIdx.x;
+          if (at < row.count) row.store(to, a.apart, at, no ? zero : chunk_grad<T>(x[c], b.l, lse2, g, tc - at * K));
+        }
+      } else {
+        for (int64_t c = threadIdx.x; c < row.count; c += NT)
+          row.store(to, a.apart, c, no ? zero : chunk_grad<T>(row.load(c, none), b.l, lse2, g, tc - c * K));
+      }
+    }
+    __syncthreads();  // sh is free again
+  }
+}
+
+template <class T>
+static int softmax_loss(admm_ctx *ctx, SoftmaxArgs a) {
+  constexpr uint64_t K = 16 / sizeof(T);
+  auto offset = [](const void *p) { return reinterpret_cast<uintptr_t>(p) & 15; };
+  a.apart = a.grad && (offset(a.grad) != offset(a.logits) || (a.rows > 1 && (a.gstride - a.stride) * sizeof(T) % 16 != 0));
+  const bool even = offset(a.logits) == 0 && (a.rows == 1 || a.stride * sizeof(T) % 16 == 0);
+  const uint64_t chunks = (a.cols + K - 1) / K + (even ? 0 : 1);  // a row between granules touches one more
+  if (chunks <= 256) {
+    a.lanes_log2 = 0;
+    while (a.lanes_log2 < 6 && (1ull << a.lanes_log2) < chunks) ++a.lanes_log2;
+    const dim3 grid(blocks_for(a.rows, 256u >> a.lanes_log2));
+    if (chunks <= 64) hipLaunchKernelGGL((k_softmax_lanes<T, 1>), grid, dim3(256), 0, ctx->stream, a);
+    else if (chunks <= 128) hipLaunchKernelGGL((k_softmax_lanes<T, 2>), grid, dim3(256), 0, ctx->stream, a);
+    else hipLaunchKernelGGL((k_softmax_lanes<T, 4>), grid, dim3(256), 0, ctx->stream, a);
+  } else {
+    const dim3 grid(blocks_for(a.rows, 1));
+    if (chunks <= 1024) hipLaunchKernelGGL((k_softmax_block<T, 256, 4>), grid, dim3(256), 0, ctx->stream, a);
+    else if (chunks <= 4096) hipLaunchKernelGGL((k_softmax_block<T, 512, 8>), grid, dim3(512), 0, ctx->stream, a);
+    else hipLaunchKernelGGL((k_softmax_block<T, 1024, 0>), grid, dim3(1024), 0, ctx->stream, a);
+  }
+  ADMM_HIP_CHECK(hipGetLastError());
+  return ADMM_OK;
+}
+
+}  // namespace admm_impl
+
+using namespace admm_impl;
+
+extern "C" int admm_softmax_loss_workspace(uint64_t rows, uint64_t cols, uint64_t *bytes) {
+  ADMM_REQUIRE(bytes, "admm_softmax_loss_workspace: bytes is NULL");
+  ADMM_REQUIRE(rows < (1ull << 40) && cols < (1ull << 40), "admm_softmax_loss_workspace: %llu x %llu logits", (unsigned long long)rows,
+               (unsigned long long)cols);
+  *bytes = 0;
+  return ADMM_OK;
+}
+
+extern "C" int admm_softmax_loss(admm_ctx *ctx, const admm_mat *logits, const void *labels, int label_type, const float *weight,
+                                 float grad_scale, float *loss, float *lse, const admm_mat *grad, void *workspace,
+                                 uint64_t workspace_bytes) {
+  ADMM_REQUIRE(ctx, "admm_softmax_loss: ctx is NULL");
+  ADMM_TRY(check_mat(logits, "admm_softmax_loss", "logits"));
+  ADMM_REQUIRE(label_type == ADMM_I32 || label_type == ADMM_I64 || label_type == ADMM_F32, "admm_softmax_loss: labels of type %d", label_type);
+  if (grad) {
+    ADMM_TRY(check_mat(grad, "admm_softmax_loss", "grad"));
+    ADMM_REQUIRE(grad->rows == logits->rows && grad->cols == logits->cols && grad->type == logits->type,
+                 "admm_softmax_loss: grad has another shape or type than the logits");
+    const bool same = grad->data == logits->data && (grad->stride == logits->stride || grad->rows <= 1);
+    ADMM_REQUIRE(same || !mats_overlap(grad, logits), "admm_softmax_loss: grad overlaps the logits and is not their own memory");
+  }
+  if (logits->rows == 0) return ADMM_OK;
+  ADMM_REQUIRE(logits->cols > 0, "admm_softmax_loss: no classes");
+  ADMM_REQUIRE(labels && loss, "admm_softmax_loss: labels or loss is NULL");
+  uint64_t need = 0;
+  ADMM_TRY(admm_softmax_loss_workspace(logits->rows, logits->cols, &need));
+  ADMM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+               "admm_softmax_loss: the workspace is NULL, not on 16 bytes or smaller than %llu bytes", (unsigned long long)need);
+  OnDevice on(ctx->device);
+  ADMM_HIP_CHECK(on.error);
+  KernelTimer t(ctx, ADMM_K_SOFTMAX);
+  SoftmaxArgs a = {};
+  a.logits = logits->data;
+  a.stride = logits->stride;
+  a.grad = grad ? grad->data : nullptr;
+  a.gstride = grad ? grad->stride : 0;
+  a.rows = logits->rows;
+  a.cols = logits->cols;
+  a.labels = labels;
+  a.label_type = label_type;
+  a.weight = weight;
+  a.grad_scale = grad_scale;
+  a.loss = loss;
+  a.lse = lse;
+  return logits->type == ADMM_F32 ? softmax_loss<float>(ctx, a) : logits->type == ADMM_BF16 ? softmax_loss<bf16_t>(ctx, a) : softmax_loss<f16_t>(ctx, a);
+}

@@ -44,6 +44,8 @@ int admm_abi_version(void);
  * library create its own. */
 int admm_device_count(int *count);
 int admm_ctx_create(int device, void *stream, admm_ctx **out);
+/* the value of `stream` that names the device's default (legacy) stream */
+#define ADMM_STREAM_DEFAULT ((void *)1)
 int admm_ctx_destroy(admm_ctx *ctx);
 int admm_sync(admm_ctx *ctx);
 
@@ -54,7 +56,10 @@ int admm_sync(admm_ctx *ctx);
 #define ADMM_K_FTRL_SEQ 2   /* exact sequential FTRL pass */
 #define ADMM_K_ELEMENTWISE 3
 #define ADMM_K_FORWARD_EVAL 4 /* the same sweep in its prediction / logloss form */
-#define ADMM_K_COUNT 5
+#define ADMM_K_EMBED 5        /* row lookup of a weight matrix and its gradient */
+#define ADMM_K_SOFTMAX 6      /* softmax loss with its gradient */
+#define ADMM_K_SAMPLE 7       /* drawing classes */
+#define ADMM_K_COUNT 8
 int admm_timing_enable(admm_ctx *ctx, int on);
 /* restricts the timing to the classes whose bit (1u << ADMM_K_*) is set; all classes by default.  Every
  * timed launch costs two event records on the stream, which a step of many small kernels feels. */
@@ -291,6 +296,108 @@ int admm_consensus(admm_ctx *ctx, const float *sum, int num_worker, float rho, f
 int admm_consensus_static(void *stream, const float *sum, int num_worker, float rho,
                           float global_var, float l1, const float *x, float *ydual, float *z,
                           uint64_t dim, double *residuals_out);
+
+/* ---- models with many classes or tokens (no counterpart in the reference, whose model has one weight per feature) ----
+ *
+ * The same four steps as the two-class path above, with a matrix of weights (a row per feature or token, a column per
+ * class or embedding dimension) in the place of the vector: admm_embed is X W (the margins), admm_softmax_loss the loss
+ * and the residuals, admm_embed_grad X^T R (the gradient), admm_sample the answer.
+ *
+ *   - Nothing here allocates, waits for the GPU or keeps anything between calls: the work is queued on the context's
+ *     stream and scratch memory is the caller's (`workspace`, sized by the *_workspace functions, which need no GPU;
+ *     the contents before and after a call mean nothing).  So every call may be captured into a HIP graph (with
+ *     admm_timing_enable off); calls, and replays of graphs, that can run at the same time need workspaces of their
+ *     own.  The calling thread's current device is left as it was.
+ *   - Floating sums are held in 32 bits or more and in an order that depends on the shapes and the ids alone: the same
+ *     call gives the same bits.  A result is rounded once to the type of its matrix.
+ *   - Where a shape has no elements, nothing is launched and the call succeeds. */
+
+#define ADMM_F32 0
+#define ADMM_BF16 1
+#define ADMM_F16 2
+#define ADMM_I32 3 /* also reads unsigned ids, the type of a sample set's columns */
+#define ADMM_I64 4
+
+/* A row-major matrix in DEVICE memory: row r begins at element r * stride, stride >= cols.  Any alignment of the rows to
+ * the element's size works; 16 bytes is the fastest. */
+typedef struct admm_mat {
+  void *data;
+  uint64_t rows, cols, stride;
+  int type; /* ADMM_F32, ADMM_BF16 or ADMM_F16 */
+} admm_mat;
+
+/* Rows of ids in DEVICE memory.  rowptr == NULL: one id per row (tokens), nnz == nrows.  Else row r holds the entries
+ * [rowptr[r], rowptr[r+1]) (a sample set's rows; a row may be empty; what lies beyond nnz is not read).  An id outside
+ * the table (-1 in a padded batch) stands for nothing: it adds zero and receives no gradient.
+ * Limits: nrows, nnz and the table's rows below 2^32 - 1. */
+typedef struct admm_bags {
+  const void *ids;
+  const uint64_t *rowptr;
+  const float *val; /* a factor per entry; NULL: all 1 */
+  uint64_t nrows, nnz;
+  int id_type; /* ADMM_I32 or ADMM_I64 */
+} admm_bags;
+
+/* The rows of a resident sample set as bags: pointers into the set, valid until admm_csr_destroy or a call that renumbers
+ * or frees its rows.  A relabelled set (its stored ids are frequency ranks) and a lean one whose rows are gone give
+ * ADMM_ERR_STATE. */
+int admm_csr_bags(const admm_csr *csr, admm_bags *out);
+
+/* out[r, :] = scale * sum over the entries e of row r of val_e * table[id_e, :].  `out` has the table's type or ADMM_F32,
+ * its columns, and at least nrows rows; rows from nrows on are left as they were.  The two may not overlap. */
+int admm_embed(admm_ctx *ctx, const admm_bags *bags, const admm_mat *table, float scale, const admm_mat *out);
+
+/* What admm_embed_grad needs of the bags: their entries sorted by id (stably), with each one's row and factor, written to
+ * `order`, a DEVICE buffer of at least admm_embed_order_bytes bytes, 256-byte aligned.  For a sample set this is done
+ * once; for tokens once per batch.  It holds copies: after a change of the ids, row pointers or factors it is built
+ * again. */
+int admm_embed_order_bytes(const admm_bags *bags, uint64_t table_rows, uint64_t *bytes);
+int admm_embed_order(admm_ctx *ctx, const admm_bags *bags, uint64_t table_rows, void *order, uint64_t order_bytes);
+
+/* The gradient of admm_embed with respect to its table: for every table row v the sum over the entries with id v of
+ * scale * val_e * grad_out[row_e, :].  accumulate == 0 writes every row of grad_table (zeros where no entry is),
+ * accumulate != 0 adds to it and touches no row without an entry.  grad_table has grad_out's type or ADMM_F32.  `bags` and
+ * `order` are those of admm_embed_order with table_rows == grad_table->rows (only the counts in `bags` are used). */
+int admm_embed_grad_workspace(const admm_bags *bags, uint64_t cols, uint64_t *bytes);
+int admm_embed_grad(admm_ctx *ctx, const admm_bags *bags, const void *order, uint64_t order_bytes,
+                    const admm_mat *grad_out, float scale, int accumulate, const admm_mat *grad_table, void *workspace,
+                    uint64_t workspace_bytes);
+
+/* Per row r with label t and weight w (weight == NULL: 1):
+ *   lse[r] = log sum_j exp(x_j),  loss[r] = w (lse[r] - x_t),  grad[r, j] = grad_scale * w * (exp(x_j - lse[r]) - [j == t]).
+ * labels: DEVICE array of label_type ADMM_I32, ADMM_I64 or ADMM_F32 (a sample set's labels, truncated).  A row whose label
+ * is outside [0, cols) or whose weight is 0 is not trained on: loss 0, gradient 0.  Logits of -inf are classes that are
+ * masked out: probability 0, gradient 0.  A row whose label is masked has loss +inf; one with no class left has loss +inf
+ * and gradient 0 (lse -inf).  A NaN, or a logit of +inf, makes its row NaN.
+ * lse and grad may be NULL (not wanted); grad has the logits' shape and type and may be the logits' own memory (same data
+ * and stride), else it may not overlap them. */
+int admm_softmax_loss_workspace(uint64_t rows, uint64_t cols, uint64_t *bytes);
+int admm_softmax_loss(admm_ctx *ctx, const admm_mat *logits, const void *labels, int label_type, const float *weight,
+                      float grad_scale, float *loss, float *lse, const admm_mat *grad, void *workspace,
+                      uint64_t workspace_bytes);
+
+/* Draws a class per row from softmax(logits / temperature) after its filters, with the given uniform numbers.
+ * Classes are ordered by logit, ties by index, and
+ *   1. top_k[r] > 0 keeps the first top_k[r];
+ *   2. top_p[r] < 1 keeps those whose predecessors' mass is below top_p[r] times the mass that step 1 left (the first
+ *      one always);
+ *   3. min_p[r] > 0 keeps those of at least min_p[r] times the first one's probability (the first one always).
+ * The token is the first class, in the order of the indexes, at which the cumulative mass of the kept classes exceeds
+ * uniform[r] times their total; logprob (may be NULL) is the log of its share of that total.  temperature[r] <= 0 (or
+ * NaN) takes the first class, logprob 0.  temperature, top_k, top_p and min_p are DEVICE arrays of one number per row;
+ * NULL: 1, and no filter.  uniform is in [0, 1); what is outside counts as the nearest end.  NaN logits count as -inf; a
+ * row without any logit above -inf gives token -1 and logprob -inf; logits of +inf share all the mass.
+ * Masses are 64-bit integers (a weight below 2^-(62 - ceil(log2 cols)) of the row's largest may count as none), so a draw
+ * does not depend on the batch it is in.  cols < 2^31. */
+typedef struct admm_sample_params {
+  const float *temperature;
+  const int32_t *top_k;
+  const float *top_p;
+  const float *min_p;
+} admm_sample_params;
+int admm_sample_workspace(uint64_t rows, uint64_t cols, uint64_t *bytes);
+int admm_sample(admm_ctx *ctx, const admm_mat *logits, const admm_sample_params *params, const float *uniform,
+                int32_t *token, float *logprob, void *workspace, uint64_t workspace_bytes);
 
 /* ---- collective (rabit::Allreduce<op::Sum>, src/admm_allreduce.cpp:69) -------------------- */
 
