@@ -1,8 +1,8 @@
 // Draws a class per row from softmax(logits / temperature) after top-k, top-p and min-p, with given uniform numbers.
 //
 // The weight of a class is w = 2^((x - max) L / T), L = log2(e), computed in double and held as the integer
-// rint(w 2^S): sums of integers do not depend on their order, so a row's token does not depend on how it is summed.  S is
-// such that a row of ones still fits 63 bits.
+// rint(w 2^S): sums of integers do not depend on their order, so a row's token does not depend on how it is summed.  S is 51,
+// or less where a row of ones would not fit 63 bits.
 //
 // Every filter keeps a prefix of the classes in the order (logit descending, index ascending), and the draw is the first
 // class in index order at which the cumulative weight passes a bound.  Both are one question -- the first class, by some
@@ -23,6 +23,8 @@ struct SampleArgs {
   int32_t *token;
   float *logprob;
   int index_bits, shift;  // 2^index_bits >= cols; S
+  float *tops;            // [rows][groups] largest logits of kGroup granules each
+  int64_t groups;
 };
 
 // larger logits have smaller keys; -0 counts as 0 and NaN as -inf
@@ -35,33 +37,33 @@ __device__ inline float logit_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key : ~key & 0x7FFFFFFFu);
 }
 
-// 2^y for y <= 0: 2^rint(y) times a polynomial of the rest (|f ln 2| <= 0.35: the series' term of degree 12 is 1e-16)
-__device__ inline double exp2_double(double y) {
-  y = y > -1100.0 ? y : -1100.0;
-  const double n = rint(y), f = (y - n) * 0.69314718055994530942;
-  double p = 1.0 / 479001600.0;
-  p = fma(p, f, 1.0 / 39916800.0);
-  p = fma(p, f, 1.0 / 3628800.0);
-  p = fma(p, f, 1.0 / 362880.0);
-  p = fma(p, f, 1.0 / 40320.0);
-  p = fma(p, f, 1.0 / 5040.0);
-  p = fma(p, f, 1.0 / 720.0);
-  p = fma(p, f, 1.0 / 120.0);
-  p = fma(p, f, 1.0 / 24.0);
-  p = fma(p, f, 1.0 / 6.0);
-  p = fma(p, f, 0.5);
-  p = fma(p, f, 1.0);
-  p = fma(p, f, 1.0);
-  return ldexp(p, (int)n);
-}
-
 struct Weights {
   float top;
   double per;  // L / T
-  int shift;
-  // the weight as a double; the class with the largest logit has 1 (also where that is +inf)
-  __device__ double of(float x) const { return x == top ? 1.0 : x > -INFINITY ? exp2_double(((double)x - (double)top) * per) : 0.0; }
-  __device__ unsigned long long units(double w) const { return (unsigned long long)rint(ldexp(w, shift)); }
+  int shift;   // S <= 51
+  // 2^S times the weight: 2^(n + S) times a polynomial of the rest of the exponent (|f ln 2| <= 0.35: the series' term of
+  // degree 11 is 2e-13, where the draw of a flat row of 2^17 classes sees 8e-6 a class)
+  __device__ double scaled(float x) const {
+    double y = ((double)x - (double)top) * per;
+    y = y > -1100.0 ? y : -1100.0;  // also -inf - top, and (-inf) 0 at an infinite temperature
+    const double n = rint(y), f = (y - n) * 0.69314718055994530942;
+    double p = 1.0 / 3628800.0;
+    p = fma(p, f, 1.0 / 362880.0);
+    p = fma(p, f, 1.0 / 40320.0);
+    p = fma(p, f, 1.0 / 5040.0);
+    p = fma(p, f, 1.0 / 720.0);
+    p = fma(p, f, 1.0 / 120.0);
+    p = fma(p, f, 1.0 / 24.0);
+    p = fma(p, f, 1.0 / 6.0);
+    p = fma(p, f, 0.5);
+    p = fma(p, f, 1.0);
+    p = fma(p, f, 1.0);
+    return x == top ? ldexp(1.0, shift) : x > -INFINITY ? ldexp(p, (int)n + shift) : 0.0;
+  }
+  // rounded to an integer below 2^52: what is left in the mantissa after 2^52 is added
+  __device__ unsigned long long units(double v) const { return __double_as_longlong(v + 0x1p52) & 0xFFFFFFFFFFFFFull; }
+  // does a class of that weight pass min-p?
+  __device__ bool passes(double v, float m) const { return !(m > 0.0f) || v >= ldexp((double)m, shift); }
 };
 
 // the classes of a row, each of them to one thread
@@ -190,7 +192,7 @@ __device__ inline void draw_row(const SampleArgs &a, uint64_t r, const Source &s
     last = select_key(bits, (unsigned long long)k, sh, [&](auto f) { source.each([&](float x, uint32_t j) { f(order(x, j), 1ull); }); });
   if (p < 1.0f) {
     unsigned long long mass = 0;
-    source.each([&](float x, uint32_t j) { mass += order(x, j) <= last ? weight.units(weight.of(x)) : 0; });
+    source.each([&](float x, uint32_t j) { mass += order(x, j) <= last ? weight.units(weight.scaled(x)) : 0; });
     mass = block_sum(mass, sh);
     // kept while the mass before is below p times it: up to the first class at which the sum reaches that
     const double bound = p > 0.0f ? ceil((double)p * (double)mass) : 0.0;
@@ -198,7 +200,7 @@ __device__ inline void draw_row(const SampleArgs &a, uint64_t r, const Source &s
     const unsigned long long end = select_key(bits, target, sh, [&](auto f) {
       source.each([&](float x, uint32_t j) {
         const unsigned long long o = order(x, j);
-        f(o, o <= last ? weight.units(weight.of(x)) : 0ull);
+        f(o, o <= last ? weight.units(weight.scaled(x)) : 0ull);
       });
     });
     last = end < last ? end : last;
@@ -206,9 +208,8 @@ __device__ inline void draw_row(const SampleArgs &a, uint64_t r, const Source &s
   auto kept = [&](float x, uint32_t j) -> unsigned long long {
     const unsigned long long o = order(x, j);
     if (o > last) return 0;
-    const double w = weight.of(x);
-    if (m > 0.0f && !(w >= (double)m) && o != first) return 0;
-    return weight.units(w);
+    const double w = weight.scaled(x);
+    return weight.passes(w, m) || o == first ? weight.units(w) : 0;
   };
   unsigned long long total = 0;
   source.each([&](float x, uint32_t j) { total += kept(x, j); });
@@ -224,8 +225,8 @@ __device__ inline void draw_row(const SampleArgs &a, uint64_t r, const Source &s
     token = ~0ull;
     source.each([&](float x, uint32_t j) {
       const unsigned long long o = order(x, j);
-      const double w = weight.of(x);
-      if (o <= last && w > 0.0 && (!(m > 0.0f) || w >= (double)m || o == first) && j < token) token = j;
+      const double w = weight.scaled(x);
+      if (o <= last && w > 0.0 && (weight.passes(w, m) || o == first) && j < token) token = j;
     });
     token = block_min(token, sh);
   }
@@ -238,14 +239,472 @@ __device__ inline void draw_row(const SampleArgs &a, uint64_t r, const Source &s
   });
 }
 
+// ---- rows in two launches ----------------------------------------------------------------------------
+//
+// k_sample_tops reads the logits once, with as many workgroups as there are, and leaves the largest logit of every kGroup
+// granules.  k_sample_rows, a workgroup per row, knows from those the row's largest logit and a bound that the k-th largest
+// is not below (the k-th largest of the groups'), reads the row again (from the caches) and goes on with few classes:
+//  * top-k: the classes from that bound on are few; everything else happens among them in LDS.
+//  * top-p: the weights are summed by kBuckets buckets of the logit and by kParts parts of the row.  The target falls into one
+//    bucket, whose classes are put in order; what is kept of each part is known then, and only the part where the draw falls
+//    is read again.  Weights below (1 - p) / cols of the largest take no part in the buckets: together they are less
+//    than 1 - p of the whole.
+//  * neither: the same parts, without buckets; min-p is a bound on the weight.
+// Rows that do not fit this (too many classes between a bound and a border, a k larger than the number of groups, u <= 0) are
+// drawn by draw_row from the whole row, to the same result: all sums are the same integers.
+
+constexpr int kGroup = 32;       // granules
+constexpr int kTopsPer = 512;    // granules per workgroup of k_sample_tops
+constexpr int kMaxGroups = 4096; // groups whose largest logits fit LDS beside the rest
+constexpr int kList = 2048;      // classes kept in LDS
+constexpr int kPairs = 512;      // of which all pairs are compared, not sorted digit by digit
+constexpr int kBuckets = 512, kParts = 8;
+
+struct RowShared {
+  union {
+    unsigned long long hist[kParts][kBuckets];
+    float tops[kMaxGroups];
+  };
+  unsigned long long list[kList];    // keys of draw_row's order
+  unsigned long long units[kPairs];  // their weights
+  Shared sh;
+  unsigned int count;
+  float bound;
+};
+
 template <class T>
-__global__ void __launch_bounds__(kThreads) k_sample_rows(SampleArgs a) {
-  __shared__ Shared sh;
-  for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    const RowSource<T> source{Chunks<T>(static_cast<const T *>(a.logits) + r * a.stride, (int64_t)a.cols)};
-    draw_row(a, r, source, sh);
-    __syncthreads();
+__global__ void __launch_bounds__(256) k_sample_tops(SampleArgs a) {
+  constexpr int K = 16 / sizeof(T);
+  const Chunks<T> row(static_cast<const T *>(a.logits) + (uint64_t)blockIdx.y * a.stride, (int64_t)a.cols);
+  const int64_t c0 = (int64_t)blockIdx.x * kTopsPer + threadIdx.x;
+  vec_t<T, K> x[kTopsPer / 256];
+#pragma unroll
+  for (int i = 0; i < kTopsPer / 256; ++i) {
+    x[i] = (T)-INFINITY;
+    if (c0 + i * 256 < row.count) x[i] = row.load(c0 + i * 256, (T)-INFINITY);
   }
+#pragma unroll
+  for (int i = 0; i < kTopsPer / 256; ++i) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < K; ++k) m = fmaxf(m, (float)x[i][k]);
+    for (int off = 1; off < kGroup; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    const int64_t g = (c0 + i * 256) / kGroup;
+    if (threadIdx.x % kGroup == 0 && g < a.groups) a.tops[(uint64_t)blockIdx.y * a.groups + g] = m;
+  }
+}
+
+// the classes in the list, each of them to one thread
+struct ListSource {
+  const unsigned long long *list;
+  int count, index_bits;
+  template <class F>
+  __device__ void each(F f) const {
+    for (int i = threadIdx.x; i < count; i += kThreads) f(logit_of((uint32_t)(list[i] >> index_bits)), (uint32_t)(list[i] & ((1ull << index_bits) - 1)));
+  }
+};
+
+struct Params {
+  float t, p, m, u;
+  int32_t k;
+};
+
+__device__ inline unsigned long long mass_target(float p, unsigned long long mass) {
+  const double bound = p > 0.0f ? ceil((double)p * (double)mass) : 0.0;
+  return bound < 1.0 ? 1ull : (unsigned long long)bound;
+}
+
+__device__ inline unsigned long long draw_target(float u, unsigned long long total) {
+  const double at = floor((double)u * (double)total);
+  const unsigned long long target = at < (double)total ? (unsigned long long)at + 1 : total;
+  return target < total ? target : total;
+}
+
+__device__ inline void write_token(const SampleArgs &a, uint64_t r, unsigned long long token, float x, const Weights &w, float t, unsigned long long total) {
+  a.token[r] = (int32_t)token;
+  if (!a.logprob) return;
+  const double y = x == w.top ? 0.0 : ((double)x - (double)w.top) / (double)t;
+  a.logprob[r] = (float)(y - log(ldexp((double)total, -a.shift)));
+}
+
+// sum of `v` over the `each` threads that share a class
+template <class V>
+__device__ inline V among(V v, int each) {
+  for (int off = 1; off < each; off <<= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+// All filters and the draw among up to kPairs classes: every class against every other, `each` threads a class.
+__device__ inline void draw_pairs(const SampleArgs &a, uint64_t r, const Params &q, const Weights &weight, unsigned long long first, RowShared &s, int count) {
+  int log_each = 0;
+  while (log_each < 6 && (count << (log_each + 1)) <= kThreads) ++log_each;
+  const int each = 1 << log_each, mine = threadIdx.x >> log_each, part = threadIdx.x & (each - 1);
+  const unsigned long long mask = (1ull << a.index_bits) - 1;
+  const bool in = mine < count;
+  const unsigned long long o = in ? s.list[mine] : ~0ull;
+  const float x = logit_of((uint32_t)(o >> a.index_bits));
+  const double w = in ? weight.scaled(x) : 0.0;
+  const unsigned long long units = in ? weight.units(w) : 0;
+  int rank = 0;
+  for (int i = part; i < count; i += each) rank += s.list[i] < o;
+  rank = among(rank, each);
+  const bool top = in && (q.k <= 0 || rank < q.k);
+  if (in && part == 0) s.units[mine] = top ? units : 0;
+  const unsigned long long mass = block_sum(top && part == 0 ? units : 0, s.sh);
+  bool kept = top;
+  if (q.p < 1.0f) {
+    unsigned long long before = 0;
+    for (int i = part; i < count; i += each) before += s.list[i] < o ? s.units[i] : 0;
+    before = among(before, each);
+    kept = kept && before < mass_target(q.p, mass);
+  }
+  if (q.m > 0.0f) kept = kept && (weight.passes(w, q.m) || o == first);
+  __syncthreads();
+  if (in && part == 0) s.units[mine] = kept ? units : 0;
+  const unsigned long long total = block_sum(kept && part == 0 ? units : 0, s.sh);
+  const unsigned long long target = draw_target(q.u, total);
+  unsigned long long upto = 0;
+  for (int i = part; i < count; i += each) upto += (s.list[i] & mask) <= (o & mask) ? s.units[i] : 0;
+  upto = among(upto, each);
+  const unsigned long long token = block_min(kept && upto >= target ? o & mask : ~0ull, s.sh);
+  if (kept && part == 0 && (o & mask) == token) write_token(a, r, token, x, weight, q.t, total);
+}
+
+// The first class, in the order of the indexes, at which the amounts of the granules [c0, c1) reach `target`; visit(x, j) is
+// a class's amount, hit(x, j) gets the class.
+template <class T, class Amount, class Hit>
+__device__ inline void find_class(const Chunks<T> &row, int64_t c0, int64_t c1, unsigned long long target, Shared &sh, Amount amount, Hit hit) {
+  constexpr int K = 16 / sizeof(T);
+  for (int64_t b = c0; b < c1; b += kThreads) {
+    const int64_t c = b + threadIdx.x;
+    vec_t<T, K> x = (T)-INFINITY;
+    if (c < c1) x = row.load(c, (T)-INFINITY);
+    unsigned long long mine = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (k % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+      mine += amount((float)x[k], c * K + k - row.lead);
+    }
+    unsigned long long up = mine;
+    for (int off = 1; off < 64; off <<= 1) {
+      const unsigned long long y = __shfl_up(up, off, 64);
+      if ((int)(threadIdx.x & 63) >= off) up += y;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) sh.sums[threadIdx.x >> 6] = up;
+    __syncthreads();
+    unsigned long long all = 0;
+    for (int i = 0; i < kThreads / 64; ++i) {
+      if (i == (int)(threadIdx.x >> 6)) up += all;
+      all += sh.sums[i];
+    }
+    if (all >= target) {  // uniform
+      unsigned long long sum = up - mine;
+      if (sum < target && target <= up) {
+        bool done = false;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (k % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+          sum += amount((float)x[k], c * K + k - row.lead);
+          if (!done && sum >= target) {
+            hit((float)x[k], c * K + k - row.lead);
+            done = true;
+          }
+        }
+      }
+      return;
+    }
+    target -= all;
+  }
+}
+
+// top-p, min-p or neither, by buckets and parts; false where the row does not fit this
+template <class T>
+__device__ inline bool draw_parts(const SampleArgs &a, uint64_t r, const Params &q, const Chunks<T> &row, const Weights &weight, RowShared &s) {
+  constexpr int K = 16 / sizeof(T);
+  const T none = (T)-INFINITY;
+  const int64_t span = (row.count + kParts - 1) / kParts;
+  const float top = weight.top;
+  auto start = [&](int part) { return part * span < row.count ? part * span : row.count; };
+  auto in_row = [&](int64_t j) { return j >= 0 && j < row.cols; };
+  __syncthreads();  // tops and list are free
+  if (q.p < 1.0f) {
+    // buckets of equal width in the logit, down to weights of (1 - p) / cols, and one power of two more for the roundings
+    const double depth = log2((double)row.cols / (1.0 - (double)q.p)) + 1.0;
+    const float scale = (float)(weight.per * kBuckets / (depth > 1.0 ? depth : 1.0));
+    auto bucket = [&](float x) { return x == top ? 0 : (int)fminf((top - x) * scale, (float)kBuckets); };
+    for (int i = threadIdx.x; i < kParts * kBuckets; i += kThreads) (&s.hist[0][0])[i] = 0;
+    if (threadIdx.x == 0) {
+      s.count = 0;
+      s.sh.found = ~0ull;
+    }
+    __syncthreads();
+    unsigned long long rest = 0, above = 0;  // below the buckets; passing min-p
+    for (int part = 0; part < kParts; ++part) {
+      for (int64_t c = start(part) + threadIdx.x; c < start(part + 1); c += kThreads) {
+        const vec_t<T, K> x = row.load(c, none);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (k % 2 == 0) __builtin_amdgcn_sched_barrier(0);  // two at a time: eight would take all registers
+          const double w = weight.scaled((float)x[k]);
+          const unsigned long long u = weight.units(w);
+          const int b = bucket((float)x[k]);
+          if (b < kBuckets) atomicAdd(&s.hist[part][b], u);
+          else rest += u;
+          if (q.m > 0.0f && weight.passes(w, q.m)) above += u;
+        }
+      }
+    }
+    __syncthreads();
+    unsigned long long mine = rest;
+    if (threadIdx.x < kBuckets) {
+      unsigned long long col = 0;
+#pragma unroll
+      for (int part = 0; part < kParts; ++part) col += s.hist[part][threadIdx.x];
+      s.list[threadIdx.x] = col;
+      mine += col;
+    }
+    const unsigned long long total = block_sum(mine, s.sh), target = mass_target(q.p, total);
+    if (q.m > 0.0f) above = block_sum(above, s.sh);
+    if (!(q.m > 0.0f && target > above)) {  // else every class that passes min-p is among those that top-p keeps
+      if (threadIdx.x < 64) {
+        constexpr int kEach = kBuckets / 64;
+        unsigned long long x[kEach], sum = 0;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+          x[k] = s.list[threadIdx.x * kEach + k];
+          sum += x[k];
+        }
+        unsigned long long up = sum;
+        for (int off = 1; off < 64; off <<= 1) {
+          const unsigned long long y = __shfl_up(up, off, 64);
+          if ((int)threadIdx.x >= off) up += y;
+        }
+        up -= sum;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+          if (up < target && target <= up + x[k]) {
+            s.sh.found = threadIdx.x * kEach + k;
+            s.sh.before = up;
+          }
+          up += x[k];
+        }
+      }
+      __syncthreads();
+      if (s.sh.found == ~0ull) return false;
+      const int border = (int)s.sh.found;
+      const unsigned long long within = target - s.sh.before;
+      // the classes of the bucket that the target falls into
+      for (int64_t c = threadIdx.x; c < row.count; c += kThreads) {
+        const vec_t<T, K> x = row.load(c, none);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const int64_t j = c * K + k - row.lead;
+          if (bucket((float)x[k]) == border && in_row(j)) {
+            const unsigned at = atomicAdd(&s.count, 1u);
+            if (at < (unsigned)kList) s.list[at] = (unsigned long long)key_of((float)x[k]) << a.index_bits | (unsigned long long)j;
+          }
+        }
+      }
+      __syncthreads();
+      const unsigned count = s.count;
+      if (count > (unsigned)kList) return false;
+      const ListSource list{s.list, (int)count, a.index_bits};
+      unsigned long long last;
+      if (count <= (unsigned)kPairs) {
+        const unsigned long long o = threadIdx.x < count ? s.list[threadIdx.x] : ~0ull;
+        if (threadIdx.x < count) s.units[threadIdx.x] = weight.units(weight.scaled(logit_of((uint32_t)(o >> a.index_bits))));
+        __syncthreads();
+        unsigned long long upto = 0;
+        if (threadIdx.x < count)
+          for (unsigned i = 0; i < count; ++i) upto += s.list[i] <= o ? s.units[i] : 0;
+        last = block_min(threadIdx.x < count && upto >= within ? o : ~0ull, s.sh);
+      } else {
+        last = select_key(32 + a.index_bits, within, s.sh, [&](auto f) {
+          list.each([&](float x, uint32_t j) { f((unsigned long long)key_of(x) << a.index_bits | j, weight.units(weight.scaled(x))); });
+        });
+      }
+      // what is kept of every part
+      if (threadIdx.x < kParts) s.hist[threadIdx.x][border] = 0;
+      __syncthreads();
+      list.each([&](float x, uint32_t j) {
+        if (((unsigned long long)key_of(x) << a.index_bits | j) > last) return;
+        atomicAdd(&s.hist[((int64_t)j + row.lead) / K / span][border], weight.units(weight.scaled(x)));
+      });
+      __syncthreads();
+      unsigned long long part_mass = 0;
+      if (threadIdx.x / 64 < kParts) {
+        for (int b = threadIdx.x & 63; b <= border; b += 64) part_mass += s.hist[threadIdx.x / 64][b];
+        for (int off = 1; off < 64; off <<= 1) part_mass += __shfl_xor(part_mass, off, 64);
+        if ((threadIdx.x & 63) == 0) s.units[threadIdx.x / 64] = part_mass;
+      }
+      __syncthreads();
+      unsigned long long kept = 0;
+      for (int part = 0; part < kParts; ++part) kept += s.units[part];
+      unsigned long long at = draw_target(q.u, kept);
+      int part = 0;
+      while (part < kParts - 1 && at > s.units[part]) at -= s.units[part++];
+      find_class(row, start(part), start(part + 1), at, s.sh,
+                 [&](float x, int64_t j) -> unsigned long long {
+                   const int b = bucket(x);
+                   if (b > border || (b == border && ((unsigned long long)key_of(x) << a.index_bits | (unsigned long long)j) > last)) return 0;
+                   return weight.units(weight.scaled(x));
+                 },
+                 [&](float x, int64_t j) { write_token(a, r, (unsigned long long)j, x, weight, q.t, kept); });
+      return true;
+    }
+  }
+  unsigned long long total = 0;
+  auto amount = [&](float x, int64_t) -> unsigned long long {
+    const double w = weight.scaled(x);
+    return weight.passes(w, q.m) ? weight.units(w) : 0;
+  };
+  for (int part = 0; part < kParts; ++part) {
+    unsigned long long mine = 0;
+    for (int64_t c = start(part) + threadIdx.x; c < start(part + 1); c += kThreads) {
+      const vec_t<T, K> x = row.load(c, none);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (k % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+        mine += amount((float)x[k], 0);
+      }
+    }
+    mine = block_sum(mine, s.sh);
+    if (threadIdx.x == 0) s.units[part] = mine;
+    total += mine;
+  }
+  __syncthreads();
+  unsigned long long at = draw_target(q.u, total);
+  int part = 0;
+  while (part < kParts - 1 && at > s.units[part]) at -= s.units[part++];
+  find_class(row, start(part), start(part + 1), at, s.sh, amount,
+             [&](float x, int64_t j) { write_token(a, r, (unsigned long long)j, x, weight, q.t, total); });
+  return true;
+}
+
+template <class T, bool TOPS>
+__global__ void __launch_bounds__(kThreads) k_sample_rows(SampleArgs a) {
+  constexpr int K = 16 / sizeof(T);
+  __shared__ RowShared s;
+  const T none = (T)-INFINITY;
+  for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    __syncthreads();
+    const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int64_t)a.cols);
+    const RowSource<T> whole{row};
+    const Params q{a.temperature ? a.temperature[r] : 1.0f, a.top_p ? a.top_p[r] : 1.0f, a.min_p ? a.min_p[r] : 0.0f, a.uniform[r],
+                   a.top_k && (uint64_t)a.top_k[r] < a.cols ? a.top_k[r] : 0};
+    const int64_t small = (row.count + kGroup - 1) / kGroup, size = (small + kMaxGroups - 1) / kMaxGroups;
+    const int groups = (int)((small + size - 1) / size);  // of `size` times kGroup granules
+    // the groups' largest logits
+    if (TOPS) {
+      for (int g = threadIdx.x; g < groups; g += kThreads) {
+        float m = -INFINITY;
+        for (int64_t i = g * size; i < (g + 1) * size && i < small; ++i) m = fmaxf(m, a.tops[r * a.groups + i]);
+        s.tops[g] = m;
+      }
+    } else {
+      for (int64_t c = threadIdx.x; c < (int64_t)groups * kGroup; c += kThreads) {
+        float m = -INFINITY;
+        if (c < row.count) {
+          const vec_t<T, K> x = row.load(c, none);
+#pragma unroll
+          for (int k = 0; k < K; ++k) m = fmaxf(m, (float)x[k]);
+        }
+        for (int off = 1; off < kGroup; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+        if (c % kGroup == 0) s.tops[c / kGroup] = m;
+      }
+    }
+    if (threadIdx.x == 0) {
+      s.count = 0;
+      s.bound = -INFINITY;
+    }
+    __syncthreads();
+    float top = -INFINITY;
+    for (int g = threadIdx.x; g < groups; g += kThreads) top = fmaxf(top, s.tops[g]);
+    for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    top = logit_of((uint32_t)block_min(key_of(top), s.sh));
+    const bool greedy = !(q.t > 0.0f) || q.m > 1.0f;  // no class but the first has a weight above 1
+    auto put = [&](float v, int64_t j) {
+      const unsigned at = atomicAdd(&s.count, 1u);
+      if (at < (unsigned)kList) s.list[at] = (unsigned long long)key_of(v) << a.index_bits | (unsigned long long)j;
+    };
+    const int want = greedy ? 1 : q.k;
+    if (top > -INFINITY && want > 0 && want <= groups) {
+      // the want-th largest of the groups': rank by comparison
+      for (int g = threadIdx.x; g < groups; g += kThreads) {
+        const float v = s.tops[g];
+        int above = 0, same = 0;
+        for (int i = 0; i < groups; ++i) {
+          above += s.tops[i] > v;
+          same += s.tops[i] == v;
+        }
+        if (above < want && want <= above + same) s.bound = v;  // all that write, write the same
+      }
+      __syncthreads();
+      const float bound = s.bound;
+      // the classes from it on
+      const int lane = threadIdx.x & (kGroup - 1);
+      for (int g = threadIdx.x / kGroup; g < groups; g += kThreads / kGroup) {
+        if (s.tops[g] < bound) continue;
+        for (int64_t c = (int64_t)g * size * kGroup + lane; c < (int64_t)(g + 1) * size * kGroup && c < row.count; c += kGroup) {
+          const vec_t<T, K> x = row.load(c, none);
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            const float v = (float)x[k];
+            const int64_t j = c * K + k - row.lead;
+            if (v >= bound && j >= 0 && j < row.cols) put(v, j);
+          }
+        }
+      }
+      __syncthreads();
+      const unsigned count = s.count;
+      if (count <= (unsigned)kList && (greedy || q.u > 0.0f)) {
+        unsigned long long first = ~0ull;
+        for (unsigned i = threadIdx.x; i < count; i += kThreads) first = s.list[i] < first ? s.list[i] : first;
+        first = block_min(first, s.sh);
+        if (greedy) {
+          if (threadIdx.x == 0) {
+            a.token[r] = (int32_t)(first & ((1ull << a.index_bits) - 1));
+            if (a.logprob) a.logprob[r] = 0.0f;
+          }
+        } else if (count <= (unsigned)kPairs) {
+          draw_pairs(a, r, q, Weights{top, 1.44269504088896340736 / (double)q.t, a.shift}, first, s, (int)count);
+        } else {
+          draw_row(a, r, ListSource{s.list, (int)count, a.index_bits}, s.sh);
+        }
+        continue;
+      }
+    }
+    if (top > -INFINITY && !greedy && q.k == 0 && q.u > 0.0f && draw_parts(a, r, q, row, Weights{top, 1.44269504088896340736 / (double)q.t, a.shift}, s)) continue;
+    draw_row(a, r, whole, s.sh);
+  }
+}
+
+// From this many columns on the largest logits of the groups come from a launch of their own; below, the row's workgroup has
+// read the row before a second launch could begin.
+constexpr uint64_t kTopsFrom = 16384;
+
+static uint64_t tops_groups(uint64_t cols, uint64_t per) { return ((cols + per - 1) / per + 1 + kGroup - 1) / kGroup; }
+
+template <class T>
+static int sample(admm_ctx *ctx, SampleArgs a) {
+  a.groups = (int64_t)tops_groups(a.cols, 16 / sizeof(T));
+  const dim3 grid(blocks_for(a.rows, 1));
+  if (a.cols <= kTopsFrom) {
+    hipLaunchKernelGGL((k_sample_rows<T, false>), grid, dim3(kThreads), 0, ctx->stream, a);
+  } else {
+    const unsigned per_row = (unsigned)((a.groups * kGroup + kTopsPer - 1) / kTopsPer);
+    for (uint64_t r = 0; r < a.rows; r += 65535) {  // rows are the second dimension of the grid
+      SampleArgs b = a;
+      b.logits = static_cast<const T *>(a.logits) + r * a.stride;
+      b.tops = a.tops + r * a.groups;
+      const unsigned rows = (unsigned)(a.rows - r < 65535 ? a.rows - r : 65535);
+      hipLaunchKernelGGL(k_sample_tops<T>, dim3(per_row, rows), dim3(256), 0, ctx->stream, b);
+    }
+    hipLaunchKernelGGL((k_sample_rows<T, true>), grid, dim3(kThreads), 0, ctx->stream, a);
+  }
+  ADMM_HIP_CHECK(hipGetLastError());
+  return ADMM_OK;
 }
 
 }  // namespace admm_impl
@@ -256,7 +715,7 @@ extern "C" int admm_sample_workspace(uint64_t rows, uint64_t cols, uint64_t *byt
   ADMM_REQUIRE(bytes, "admm_sample_workspace: bytes is NULL");
   ADMM_REQUIRE(rows < (1ull << 40) && cols < (1ull << 31), "admm_sample_workspace: %llu x %llu logits", (unsigned long long)rows,
                (unsigned long long)cols);
-  *bytes = 0;
+  *bytes = cols > kTopsFrom ? round_up(rows * tops_groups(cols, 4), 64) * 4 : 0;  // of the narrowest granules
   return ADMM_OK;
 }
 
@@ -290,11 +749,7 @@ extern "C" int admm_sample(admm_ctx *ctx, const admm_mat *logits, const admm_sam
   a.logprob = logprob;
   a.index_bits = 1;
   while ((1ull << a.index_bits) < a.cols) ++a.index_bits;
-  a.shift = 62 - a.index_bits;
-  const dim3 grid(blocks_for(a.rows, 1));
-  if (logits->type == ADMM_F32) hipLaunchKernelGGL(k_sample_rows<float>, grid, dim3(kThreads), 0, ctx->stream, a);
-  else if (logits->type == ADMM_BF16) hipLaunchKernelGGL(k_sample_rows<bf16_t>, grid, dim3(kThreads), 0, ctx->stream, a);
-  else hipLaunchKernelGGL(k_sample_rows<f16_t>, grid, dim3(kThreads), 0, ctx->stream, a);
-  ADMM_HIP_CHECK(hipGetLastError());
-  return ADMM_OK;
+  a.shift = 62 - a.index_bits < 51 ? 62 - a.index_bits : 51;
+  a.tops = static_cast<float *>(workspace);
+  return logits->type == ADMM_F32 ? sample<float>(ctx, a) : logits->type == ADMM_BF16 ? sample<bf16_t>(ctx, a) : sample<f16_t>(ctx, a);
 }

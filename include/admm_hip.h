@@ -387,8 +387,8 @@ int admm_softmax_loss(admm_ctx *ctx, const admm_mat *logits, const void *labels,
  * NaN) takes the first class, logprob 0.  temperature, top_k, top_p and min_p are DEVICE arrays of one number per row;
  * NULL: 1, and no filter.  uniform is in [0, 1); what is outside counts as the nearest end.  NaN logits count as -inf; a
  * row without any logit above -inf gives token -1 and logprob -inf; logits of +inf share all the mass.
- * Masses are 64-bit integers (a weight below 2^-(62 - ceil(log2 cols)) of the row's largest may count as none), so a draw
- * does not depend on the batch it is in.  cols < 2^31. */
+ * Weights are rounded to multiples of 2^-51 of the row's largest (for more than 2^11 classes of 2^-(62 - ceil(log2 cols)))
+ * and summed as integers, so a draw does not depend on the batch it is in.  cols < 2^31. */
 typedef struct admm_sample_params {
   const float *temperature;
   const int32_t *top_k;
