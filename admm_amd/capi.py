@@ -6,6 +6,7 @@ creation fails.
 """
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -158,7 +159,7 @@ def load():
 
 
 def _check(rc):
-    if rc != 0:
+    if rc:
         raise AdmmError("libadmm_hip error %d: %s" % (rc, load().admm_last_error().decode()))
 
 
@@ -222,65 +223,75 @@ class DeviceBuf:
         self.ptr = None
 
 
-_TORCH = {}  # torch's types, once torch is used
+class _Types(dict):
+    """torch's element types to the library's; filled at the first look, so that this module does not need torch"""
 
+    def __init__(self, *kinds):
+        super().__init__()
+        self.kinds = kinds
 
-def _torch_type(dtype):
-    if not _TORCH:
+    def __missing__(self, dtype):
         import torch
-        _TORCH.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, torch.int32: I32, torch.int64: I64})
-        for name in ("uint32", "uint64"):
-            if hasattr(torch, name):
-                _TORCH[getattr(torch, name)] = I32 if name == "uint32" else I64
-    return _TORCH.get(dtype)
+        names = {"float32": F32, "bfloat16": BF16, "float16": F16, "int32": I32, "uint32": I32, "int64": I64, "uint64": I64}
+        self.update({getattr(torch, n): k for n, k in names.items() if k in self.kinds and hasattr(torch, n)})
+        if dtype not in self:
+            raise KeyError(dtype)
+        return self[dtype]
+
+
+_FLOATS, _ARRAYS = _Types(F32, BF16, F16), _Types(F32, I32, I64)
+
+
+# admm_mat and admm_bags as bytes, which a void pointer argument takes as they are: making a ctypes structure costs as much
+# as the call itself
+_MAT = struct.Struct("PQQQi4x").pack
+_BAGS = struct.Struct("PPPQQi4x").pack
 
 
 class DeviceMat:
     """A row-major matrix in HBM (admm_mat): from a pointer, or `of` a torch tensor on the context's GPU"""
 
-    def __init__(self, ptr, rows, cols, type=F32, stride=None):
-        self.struct = MatStruct(int(ptr), int(rows), int(cols), int(cols if stride is None else stride), int(type))
-        self.ref = C.byref(self.struct)
+    __slots__ = ("rows", "cols", "packed")
 
-    @property
-    def shape(self):
-        return self.struct.rows, self.struct.cols
+    def __init__(self, ptr, rows, cols, type=F32, stride=None):
+        self.rows, self.cols = rows, cols
+        self.packed = _MAT(ptr, rows, cols, cols if stride is None else stride, type)
 
     @classmethod
     def of(cls, ctx, m, name):
         if isinstance(m, DeviceMat):
             return m
-        if not hasattr(m, "data_ptr"):
-            raise AdmmError("%s: a DeviceMat or a torch tensor is needed, not %s" % (name, m.__class__.__name__))
-        kind = _torch_type(m.dtype)
-        if kind not in (F32, BF16, F16):
-            raise AdmmError("%s: float32, bfloat16 or float16 is needed, not %s" % (name, m.dtype))
-        ctx._here(m, name)
-        if m.dim() != 2:
-            raise AdmmError("%s: a matrix is needed, not %d dimensions" % (name, m.dim()))
-        rows, cols = m.shape
-        step, inner = m.stride()
-        if cols > 1 and inner != 1:
+        try:
+            (rows, cols), (step, inner), kind = m.shape, m.stride(), _FLOATS[m.dtype]
+        except Exception:
+            raise _not_a_matrix(m, name) from None
+        if m.get_device() != ctx.device:
+            raise ctx._elsewhere(m, name)
+        if inner != 1 and cols > 1:
             raise AdmmError("%s: the elements of a row lie %d apart: they have to be adjacent" % (name, inner))
-        if rows > 1 and step < cols:
-            raise AdmmError("%s: rows of %d elements lie %d apart" % (name, cols, step))
-        return cls(m.data_ptr(), rows, cols, kind, max(step, cols))
+        if step < cols:
+            if rows > 1:
+                raise AdmmError("%s: rows of %d elements lie %d apart" % (name, cols, step))
+            step = cols
+        return cls(m.data_ptr(), rows, cols, kind, step)
+
+
+def _not_a_matrix(m, name):
+    if not hasattr(m, "data_ptr"):
+        return AdmmError("%s: a DeviceMat or a torch tensor is needed, not %s" % (name, m.__class__.__name__))
+    if m.dim() != 2:
+        return AdmmError("%s: a matrix is needed, not %d dimensions" % (name, m.dim()))
+    return AdmmError("%s: float32, bfloat16 or float16 is needed, not %s" % (name, m.dtype))
 
 
 class Bags:
     """Rows of ids (admm_bags); keeps the arrays alive"""
 
-    def __init__(self, struct, keep=()):
-        self.struct, self.keep = struct, keep
-        self.ref = C.byref(struct)
+    __slots__ = ("nrows", "nnz", "keep", "packed")
 
-    @property
-    def nrows(self):
-        return self.struct.nrows
-
-    @property
-    def nnz(self):
-        return self.struct.nnz
+    def __init__(self, ids, rowptr, val, nrows, nnz, id_type, keep=()):
+        self.nrows, self.nnz, self.keep = nrows, nnz, keep
+        self.packed = _BAGS(ids or 0, rowptr or 0, val or 0, nrows, nnz, id_type)
 
 
 class Context:
@@ -288,6 +299,8 @@ class Context:
         self.L = load()
         self.device = int(device)
         self._scratch, self._retired = None, []
+        self._size = C.c_uint64()
+        self._size_ref = C.byref(self._size)
         h = C.c_void_p()
         _check(self.L.admm_ctx_create(int(device), C.c_void_p(stream) if stream else None,
                                       C.byref(h)))
@@ -395,14 +408,28 @@ class Context:
     # Matrices are torch tensors or DeviceMats, arrays are torch tensors, DeviceVecs or DeviceBufs; what they point to
     # belongs to this context's GPU, and the work is queued on this context's stream (make the context on the stream that
     # the tensors are used on: Context(device, stream=torch.cuda.current_stream().cuda_stream or DEFAULT_STREAM)).
-    def _here(self, t, name):
-        if t.device.type != "cuda" or t.device.index != self.device:
-            raise AdmmError("%s is on %s, the context on GPU %d" % (name, t.device, self.device))
+    def _elsewhere(self, t, name):
+        return AdmmError("%s is on %s, the context on GPU %d" % (name, t.device, self.device))
 
     def _array(self, a, name, count, kinds):
         """(pointer, type) of `count` adjacent elements of one of the types"""
         if a is None:
             return None, kinds[0]
+        if hasattr(a, "data_ptr"):
+            kind = _ARRAYS.get(a.dtype)
+            if kind is None:
+                try:
+                    kind = _ARRAYS[a.dtype]
+                except KeyError:
+                    pass
+            if kind not in kinds:
+                raise AdmmError("%s: elements of type %s" % (name, a.dtype))
+            if a.get_device() != self.device:
+                raise self._elsewhere(a, name)
+            if a.numel() < count or not a.is_contiguous():
+                raise AdmmError("%s: %d adjacent elements are needed, it has %s with strides %s" %
+                                (name, count, tuple(a.shape), tuple(a.stride())))
+            return a.data_ptr(), kind
         if isinstance(a, DeviceVec):
             if F32 not in kinds or a.n < count:
                 raise AdmmError("%s: %d floats do not do for %d elements" % (name, a.n, count))
@@ -411,28 +438,24 @@ class Context:
             if a.nbytes < count * _BYTES[kinds[0]]:
                 raise AdmmError("%s: %d bytes do not do for %d elements" % (name, a.nbytes, count))
             return a.ptr, kinds[0]
-        kind = _torch_type(a.dtype)
-        if kind not in kinds:
-            raise AdmmError("%s: elements of type %s" % (name, a.dtype))
-        self._here(a, name)
-        if a.numel() < count or not a.is_contiguous():
-            raise AdmmError("%s: %d adjacent elements are needed, it has %s with strides %s" %
-                            (name, count, tuple(a.shape), tuple(a.stride())))
-        return a.data_ptr(), kind
+        raise AdmmError("%s: a torch tensor, a DeviceVec or a DeviceBuf is needed, not %s" % (name, a.__class__.__name__))
 
     def _bytes(self, buf, name):
         if isinstance(buf, DeviceBuf):
             return buf.ptr, buf.nbytes
-        self._here(buf, name)
+        if buf.get_device() != self.device:
+            raise self._elsewhere(buf, name)
         if not buf.is_contiguous():
             raise AdmmError("%s: not contiguous" % name)
-        return buf.data_ptr(), buf.numel() * buf.element_size()
+        return buf.data_ptr(), buf.nbytes
 
-    def _workspace(self, given, need):
+    def _workspace(self, given, size, *shape):
         """the caller's workspace, or one that the context keeps for calls without: it grows, and what it outgrew stays until
         close(), for graphs that were captured with it"""
         if given is not None:
             return self._bytes(given, "workspace")
+        _check(size(*shape, self._size_ref))
+        need = self._size.value
         if need == 0:
             return None, 0
         if self._scratch is None or self._scratch.nbytes < need:
@@ -459,62 +482,57 @@ class Context:
             q, _ = self._array(rowptr, "rowptr", nrows + 1, (I64,))
         if val is not None:
             f, _ = self._array(val, "val", nnz, (F32,))
-        return Bags(BagsStruct(p or None, q, f, nrows, nnz, kind), (ids, rowptr, val))
+        return Bags(p, q, f, nrows, nnz, kind, (ids, rowptr, val))
 
     def embed(self, bags, table, out, scale=1.0):
         """admm_embed: out[r] = scale * sum of val_e * table[id_e] over the entries of row r"""
-        _check(self.L.admm_embed(self.h, bags.ref, DeviceMat.of(self, table, "table").ref, scale, DeviceMat.of(self, out, "out").ref))
+        _check(self.L.admm_embed(self.h, bags.packed, DeviceMat.of(self, table, "table").packed, scale, DeviceMat.of(self, out, "out").packed))
 
     def embed_order_bytes(self, bags, table_rows):
-        n = C.c_uint64()
-        _check(self.L.admm_embed_order_bytes(bags.ref, int(table_rows), C.byref(n)))
-        return n.value
+        _check(self.L.admm_embed_order_bytes(bags.packed, int(table_rows), self._size_ref))
+        return self._size.value
 
     def embed_order(self, bags, table_rows, order=None):
         """admm_embed_order: the entries sorted by id, into `order` (a DeviceBuf or a torch tensor of bytes; made if None)"""
         if order is None:
             order = DeviceBuf(self, self.embed_order_bytes(bags, table_rows))
         p, n = self._bytes(order, "order")
-        _check(self.L.admm_embed_order(self.h, bags.ref, int(table_rows), p, n))
+        _check(self.L.admm_embed_order(self.h, bags.packed, int(table_rows), p, n))
         return order
 
     def embed_grad(self, bags, order, grad_out, grad_table, scale=1.0, accumulate=False, workspace=None):
         """admm_embed_grad: the gradient with respect to the table, written whole or added to"""
         src, to = DeviceMat.of(self, grad_out, "grad_out"), DeviceMat.of(self, grad_table, "grad_table")
         p, n = self._bytes(order, "order")
-        need = C.c_uint64()
-        _check(self.L.admm_embed_grad_workspace(bags.ref, src.struct.cols, C.byref(need)))
-        w, wn = self._workspace(workspace, need.value)
-        _check(self.L.admm_embed_grad(self.h, bags.ref, p, n, src.ref, scale, 1 if accumulate else 0, to.ref, w, wn))
+        w, wn = self._workspace(workspace, self.L.admm_embed_grad_workspace, bags.packed, src.cols)
+        _check(self.L.admm_embed_grad(self.h, bags.packed, p, n, src.packed, scale, 1 if accumulate else 0, to.packed, w, wn))
 
     def softmax_loss(self, logits, labels, loss, grad=None, lse=None, weight=None, grad_scale=1.0, workspace=None):
         """admm_softmax_loss: loss per row, and with `grad` (may be the logits) grad_scale times its gradient"""
         x = DeviceMat.of(self, logits, "logits")
         g = None if grad is None else DeviceMat.of(self, grad, "grad")
-        rows = x.struct.rows
+        rows = x.rows
         t, kind = self._array(labels, "labels", rows, (I32, I64, F32))
         w, _ = self._array(weight, "weight", rows, (F32,))
         o, _ = self._array(loss, "loss", rows, (F32,))
         e, _ = self._array(lse, "lse", rows, (F32,))
-        need = C.c_uint64()
-        _check(self.L.admm_softmax_loss_workspace(rows, x.struct.cols, C.byref(need)))
-        ws, wn = self._workspace(workspace, need.value)
-        _check(self.L.admm_softmax_loss(self.h, x.ref, t, kind, w, grad_scale, o, e, None if g is None else g.ref, ws, wn))
+        ws, wn = self._workspace(workspace, self.L.admm_softmax_loss_workspace, rows, x.cols)
+        _check(self.L.admm_softmax_loss(self.h, x.packed, t, kind, w, grad_scale, o, e, None if g is None else g.packed, ws, wn))
 
     def sample(self, logits, uniform, token, logprob=None, temperature=None, top_k=None, top_p=None, min_p=None, workspace=None):
         """admm_sample: a class per row into `token` (int32), the log of its probability into `logprob`"""
         x = DeviceMat.of(self, logits, "logits")
-        rows = x.struct.rows
+        rows = x.rows
         u, _ = self._array(uniform, "uniform", rows, (F32,))
         t, _ = self._array(token, "token", rows, (I32,))
         lp, _ = self._array(logprob, "logprob", rows, (F32,))
-        given = [self._array(a, name, rows, (kind,))[0] for a, name, kind in
-                 ((temperature, "temperature", F32), (top_k, "top_k", I32), (top_p, "top_p", F32), (min_p, "min_p", F32))]
-        params = SampleParamsStruct(*given)
-        need = C.c_uint64()
-        _check(self.L.admm_sample_workspace(rows, x.struct.cols, C.byref(need)))
-        ws, wn = self._workspace(workspace, need.value)
-        _check(self.L.admm_sample(self.h, x.ref, C.byref(params), u, t, lp, ws, wn))
+        f, _ = self._array(temperature, "temperature", rows, (F32,))
+        k, _ = self._array(top_k, "top_k", rows, (I32,))
+        p, _ = self._array(top_p, "top_p", rows, (F32,))
+        m, _ = self._array(min_p, "min_p", rows, (F32,))
+        params = SampleParamsStruct(f, k, p, m)
+        ws, wn = self._workspace(workspace, self.L.admm_sample_workspace, rows, x.cols)
+        _check(self.L.admm_sample(self.h, x.packed, C.byref(params), u, t, lp, ws, wn))
 
     # consensus algebra --------------------------------------------------------------------
     def payload(self, x, ydual, rho, out):
@@ -605,7 +623,7 @@ class SampleSet:
         """the set's rows as bags for Context.embed / embed_grad (admm_csr_bags)"""
         b = BagsStruct()
         _check(self.ctx.L.admm_csr_bags(self.h, C.byref(b)))
-        return Bags(b, (self,))
+        return Bags(b.ids, b.rowptr, b.val, b.nrows, b.nnz, b.id_type, (self,))
 
     def build_transposed(self, panel_rows=0, col_block=0):
         _check(self.ctx.L.admm_csr_build_transposed(self.h, int(panel_rows), int(col_block)))

@@ -41,16 +41,16 @@ __device__ inline void store_n(T *p, const float (&v)[N]) {
   }
 }
 
-// A row of `cols` elements at any address, seen as the 16-byte granules of memory that it touches: all but the first and
-// the last are whole and are read and written at once, those two element by element, so nothing outside the row is
-// touched.  Element k of chunk c is column c * kPer + k - lead.
-template <class T>
+// A row of `cols` elements at any address, seen as the granules of 16 (or BYTES) bytes of memory that it touches: all but the
+// first and the last are whole and are read and written at once, those two element by element, so nothing outside the row
+// is touched.  Element k of chunk c is column c * kPer + k - lead.
+template <class T, int BYTES = 16>
 struct Chunks {
-  static constexpr int kPer = 16 / sizeof(T);
-  const T *base;  // on 16 bytes; the row begins `lead` elements after it
+  static constexpr int kPer = BYTES / sizeof(T);
+  const T *base;  // on BYTES bytes; the row begins `lead` elements after it
   int64_t lead, cols, count;
   __device__ Chunks(const T *row, int64_t n) {
-    lead = (int64_t)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    lead = (int64_t)((reinterpret_cast<uintptr_t>(row) & (BYTES - 1)) / sizeof(T));
     base = row - lead;
     cols = n;
     count = (lead + n + kPer - 1) / kPer;

@@ -12,7 +12,7 @@
 
 namespace admm_impl {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kDigit = 8;
 
 struct SampleArgs {
@@ -38,49 +38,46 @@ __device__ inline float logit_of(uint32_t key) {
 }
 
 struct Weights {
-  float top;
-  double per;  // L / T
-  int shift;   // S <= 51
-  // 2^S times the weight: 2^(n + S) times a polynomial of the rest of the exponent (|f ln 2| <= 0.35: the series' term of
-  // degree 11 is 2e-13, where the draw of a flat row of 2^17 classes sees 8e-6 a class)
+  float top;      // the row's largest logit
+  double per;     // L / T
+  double least;   // 2^S min-p, or 0
+  int shift;      // S <= 51
+  __device__ Weights(float top_, float t, float min_p, int shift_) : top(top_), shift(shift_) {
+    per = fmax(1.44269504088896340736 / (double)t, 1e-300);  // not 0 at an infinite temperature: -inf stays -inf
+    least = min_p > 0.0f ? ldexp((double)min_p, shift) : 0.0;
+  }
+  // 2^S times the weight of a class: 2^(n + S) times a polynomial of the rest of the exponent (|f ln 2| <= 0.35: the series'
+  // term of degree 11 is 2e-13, where the draw of a flat row of 2^17 classes sees 8e-6 a class).  0 for -inf and NaN; a top of
+  // +inf is not meant here.
   __device__ double scaled(float x) const {
-    double y = ((double)x - (double)top) * per;
-    y = y > -1100.0 ? y : -1100.0;  // also -inf - top, and (-inf) 0 at an infinite temperature
-    const double n = rint(y), f = (y - n) * 0.69314718055994530942;
-    double p = 1.0 / 3628800.0;
-    p = fma(p, f, 1.0 / 362880.0);
-    p = fma(p, f, 1.0 / 40320.0);
-    p = fma(p, f, 1.0 / 5040.0);
-    p = fma(p, f, 1.0 / 720.0);
-    p = fma(p, f, 1.0 / 120.0);
-    p = fma(p, f, 1.0 / 24.0);
-    p = fma(p, f, 1.0 / 6.0);
-    p = fma(p, f, 0.5);
+    const double y = fmax(((double)x - (double)top) * per, -1100.0);
+    const double n = rint(y), f = y - n;
+    double p = 7.054911620801121e-09;  // ln(2)^k / k!
+    p = fma(p, f, 1.0178086009239699e-07);
+    p = fma(p, f, 1.3215486790144307e-06);
+    p = fma(p, f, 1.525273380405984e-05);
+    p = fma(p, f, 0.0001540353039338161);
+    p = fma(p, f, 0.0013333558146428443);
+    p = fma(p, f, 0.009618129107628477);
+    p = fma(p, f, 0.05550410866482158);
+    p = fma(p, f, 0.2402265069591007);
+    p = fma(p, f, 0.6931471805599453);
     p = fma(p, f, 1.0);
-    p = fma(p, f, 1.0);
-    return x == top ? ldexp(1.0, shift) : x > -INFINITY ? ldexp(p, (int)n + shift) : 0.0;
+    return ldexp(p, (int)n + shift);
   }
   // rounded to an integer below 2^52: what is left in the mantissa after 2^52 is added
-  __device__ unsigned long long units(double v) const { return __double_as_longlong(v + 0x1p52) & 0xFFFFFFFFFFFFFull; }
-  // does a class of that weight pass min-p?
-  __device__ bool passes(double v, float m) const { return !(m > 0.0f) || v >= ldexp((double)m, shift); }
+  __device__ static unsigned long long units(double v) { return __double_as_longlong(v + 0x1p52) & 0xFFFFFFFFFFFFFull; }
 };
 
 // the classes of a row, each of them to one thread
 template <class T>
 struct RowSource {
-  Chunks<T> row;
+  const T *row;
+  int64_t cols;
   template <class F>
   __device__ void each(F f) const {
-    constexpr int K = 16 / sizeof(T);
-    for (int64_t c = threadIdx.x; c < row.count; c += kThreads) {
-      const vec_t<T, K> x = row.load(c, (T)-INFINITY);
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int64_t j = c * K + k - row.lead;
-        if (j >= 0 && j < row.cols) f((float)x[k], (uint32_t)j);
-      }
-    }
+#pragma unroll 1
+    for (int64_t j = threadIdx.x; j < cols; j += kThreads) f((float)row[j], (uint32_t)j);
   }
 };
 
@@ -162,45 +159,47 @@ __device__ inline unsigned long long select_key(int bits, unsigned long long tar
   return prefix;
 }
 
-// the token of one row from the classes that `source` gives out
+struct Params {
+  float t, p, m, u;
+  int32_t k;  // 0: no top-k
+};
+
+// the target of top-p: kept while the mass before is below p times all, up to the first class at which the sum reaches that
+__device__ inline unsigned long long mass_target(float p, unsigned long long mass) {
+  const double bound = p > 0.0f ? ceil((double)p * (double)mass) : 0.0;
+  return bound < 1.0 ? 1ull : (unsigned long long)bound;
+}
+
+// the draw's: the first class at which the sum exceeds u times all
+__device__ inline unsigned long long draw_target(float u, unsigned long long total) {
+  const double at = floor((double)u * (double)total);
+  const unsigned long long target = at < (double)total ? (unsigned long long)at + 1 : total;
+  return target < total ? target : total;
+}
+
+__device__ inline void write_token(const SampleArgs &a, uint64_t r, uint32_t token, float x, const Weights &w, float t, unsigned long long total) {
+  a.token[r] = (int32_t)token;
+  if (!a.logprob) return;
+  const double y = x == w.top ? 0.0 : ((double)x - (double)w.top) / (double)t;
+  a.logprob[r] = (float)(y - log(ldexp((double)total, -w.shift)));
+}
+
+// The token of one row from the classes that `source` gives out; any row, any parameters.  `first`: the key of the first class.
 template <class Source>
-__device__ inline void draw_row(const SampleArgs &a, uint64_t r, const Source &source, Shared &sh) {
+__device__ inline void draw_row(const SampleArgs &a, uint64_t r, const Params &q, const Weights &weight, unsigned long long first, const Source &source, Shared &sh) {
   const int bits = 32 + a.index_bits;
   auto order = [&](float x, uint32_t j) { return (unsigned long long)key_of(x) << a.index_bits | j; };
-  unsigned long long first = ~0ull;
-  source.each([&](float x, uint32_t j) {
-    const unsigned long long k = order(x, j);
-    first = k < first ? k : first;
-  });
-  first = block_min(first, sh);
-  const float top = logit_of((uint32_t)(first >> a.index_bits));
-  const float t = a.temperature ? a.temperature[r] : 1.0f;
-  const bool none = top == -INFINITY;
-  if (none || !(t > 0.0f)) {
-    if (threadIdx.x == 0) {
-      a.token[r] = none ? -1 : (int32_t)(first & ((1ull << a.index_bits) - 1));
-      if (a.logprob) a.logprob[r] = none ? -INFINITY : 0.0f;
-    }
-    return;
-  }
-  const Weights weight{top, 1.44269504088896340736 / (double)t, a.shift};
-  const float m = a.min_p ? a.min_p[r] : 0.0f;
-  const int32_t k = a.top_k ? a.top_k[r] : 0;
-  const float p = a.top_p ? a.top_p[r] : 1.0f;
+  auto scaled = [&](float x) { return x == weight.top ? ldexp(1.0, weight.shift) : weight.scaled(x); };  // also where top is +inf
   unsigned long long last = ~0ull;  // the last class that is kept
-  if (k > 0 && (uint64_t)k < a.cols)
-    last = select_key(bits, (unsigned long long)k, sh, [&](auto f) { source.each([&](float x, uint32_t j) { f(order(x, j), 1ull); }); });
-  if (p < 1.0f) {
+  if (q.k > 0) last = select_key(bits, (unsigned long long)q.k, sh, [&](auto f) { source.each([&](float x, uint32_t j) { f(order(x, j), 1ull); }); });
+  if (q.p < 1.0f) {
     unsigned long long mass = 0;
-    source.each([&](float x, uint32_t j) { mass += order(x, j) <= last ? weight.units(weight.scaled(x)) : 0; });
+    source.each([&](float x, uint32_t j) { mass += order(x, j) <= last ? weight.units(scaled(x)) : 0; });
     mass = block_sum(mass, sh);
-    // kept while the mass before is below p times it: up to the first class at which the sum reaches that
-    const double bound = p > 0.0f ? ceil((double)p * (double)mass) : 0.0;
-    const unsigned long long target = bound < 1.0 ? 1ull : (unsigned long long)bound;
-    const unsigned long long end = select_key(bits, target, sh, [&](auto f) {
+    const unsigned long long end = select_key(bits, mass_target(q.p, mass), sh, [&](auto f) {
       source.each([&](float x, uint32_t j) {
         const unsigned long long o = order(x, j);
-        f(o, o <= last ? weight.units(weight.scaled(x)) : 0ull);
+        f(o, o <= last ? weight.units(scaled(x)) : 0ull);
       });
     });
     last = end < last ? end : last;
@@ -208,50 +207,45 @@ __device__ inline void draw_row(const SampleArgs &a, uint64_t r, const Source &s
   auto kept = [&](float x, uint32_t j) -> unsigned long long {
     const unsigned long long o = order(x, j);
     if (o > last) return 0;
-    const double w = weight.scaled(x);
-    return weight.passes(w, m) || o == first ? weight.units(w) : 0;
+    const double w = scaled(x);
+    return w >= weight.least || o == first ? weight.units(w) : 0;
   };
   unsigned long long total = 0;
   source.each([&](float x, uint32_t j) { total += kept(x, j); });
   total = block_sum(total, sh);
-  const float u = a.uniform[r];
   unsigned long long token;
-  if (u > 0.0f) {
-    const double at = floor((double)u * (double)total);
-    unsigned long long target = at < (double)total ? (unsigned long long)at + 1 : total;
-    target = target < total ? target : total;
-    token = select_key(a.index_bits, target, sh, [&](auto f) { source.each([&](float x, uint32_t j) { f(j, kept(x, j)); }); });
+  if (q.u > 0.0f) {
+    token = select_key(a.index_bits, draw_target(q.u, total), sh, [&](auto f) { source.each([&](float x, uint32_t j) { f(j, kept(x, j)); }); });
   } else {  // the first class of any weight, however small
     token = ~0ull;
     source.each([&](float x, uint32_t j) {
       const unsigned long long o = order(x, j);
-      const double w = weight.scaled(x);
-      if (o <= last && w > 0.0 && (weight.passes(w, m) || o == first) && j < token) token = j;
+      const double w = scaled(x);
+      if (o <= last && w > 0.0 && (w >= weight.least || o == first) && j < token) token = j;
     });
     token = block_min(token, sh);
   }
   source.each([&](float x, uint32_t j) {
-    if (j != token) return;
-    a.token[r] = (int32_t)j;
-    if (!a.logprob) return;
-    const double y = x == top ? 0.0 : ((double)x - (double)top) / (double)t;
-    a.logprob[r] = (float)(y - log(ldexp((double)total, -a.shift)));
+    if (j == token) write_token(a, r, j, x, weight, q.t, total);
   });
 }
 
-// ---- rows in two launches ----------------------------------------------------------------------------
+// ---- rows in a few launches ----------------------------------------------------------------------------
 //
 // k_sample_tops reads the logits once, with as many workgroups as there are, and leaves the largest logit of every kGroup
-// granules.  k_sample_rows, a workgroup per row, knows from those the row's largest logit and a bound that the k-th largest
-// is not below (the k-th largest of the groups'), reads the row again (from the caches) and goes on with few classes:
-//  * top-k: the classes from that bound on are few; everything else happens among them in LDS.
-//  * top-p: the weights are summed by kBuckets buckets of the logit and by kParts parts of the row.  The target falls into one
-//    bucket, whose classes are put in order; what is kept of each part is known then, and only the part where the draw falls
-//    is read again.  Weights below (1 - p) / cols of the largest take no part in the buckets: together they are less
-//    than 1 - p of the whole.
-//  * neither: the same parts, without buckets; min-p is a bound on the weight.
-// Rows that do not fit this (too many classes between a bound and a border, a k larger than the number of groups, u <= 0) are
-// drawn by draw_row from the whole row, to the same result: all sums are the same integers.
+// granules.  The other kernels have a workgroup per row, know from those the row's largest logit, and read the row again
+// (from the caches), or little of it:
+//  * k_sample_list (where top-k is given): the k-th largest logit is not below the k-th largest of the groups'.  The classes from
+//    that bound on are few; everything else happens among them in LDS.
+//  * k_sample_parts (the rows without top-k).  For top-p the weights are summed by kBuckets buckets of the logit and by kParts
+//    parts of the row.  The target falls into one bucket, whose classes are put in order; what is kept of each part is known
+//    then, and only the part where the draw falls is read again.  Weights below (1 - p) / cols of the largest take no part in
+//    the buckets: together they are less than 1 - p of the whole.  Without top-p the same parts, without buckets; min-p is a
+//    bound on the weight.
+//  * k_sample_any: rows that do not fit this (too many classes between a bound and a border, a k larger than the number of
+//    groups, u <= 0, logits of +inf) are drawn by draw_row from the whole row, to the same result: all sums are the same integers.
+// A row that is left to a later kernel has the token kLeft.  One kernel for all of it is slower: it takes so many registers
+// that it spills, and a single row of 128000 classes with top-k took 43 us in it.
 
 constexpr int kGroup = 32;       // granules
 constexpr int kTopsPer = 512;    // granules per workgroup of k_sample_tops
@@ -259,18 +253,53 @@ constexpr int kMaxGroups = 4096; // groups whose largest logits fit LDS beside t
 constexpr int kList = 2048;      // classes kept in LDS
 constexpr int kPairs = 512;      // of which all pairs are compared, not sorted digit by digit
 constexpr int kBuckets = 512, kParts = 8;
+constexpr int32_t kLeft = -2;
 
-struct RowShared {
-  union {
-    unsigned long long hist[kParts][kBuckets];
-    float tops[kMaxGroups];
-  };
-  unsigned long long list[kList];    // keys of draw_row's order
+struct ListShared {
+  float tops[kMaxGroups];
+  unsigned int hits[kMaxGroups];
+  unsigned long long list[kPairs];   // keys of draw_row's order
   unsigned long long units[kPairs];  // their weights
   Shared sh;
-  unsigned int count;
-  float bound;
+  unsigned int count, nhits, bound;
 };
+
+struct PartsShared {
+  unsigned long long hist[kParts][kBuckets];
+  unsigned long long list[kList], units[kPairs];
+  Shared sh;
+  unsigned int count;
+};
+
+__device__ inline Params params_of(const SampleArgs &a, uint64_t r) {
+  return Params{a.temperature ? a.temperature[r] : 1.0f, a.top_p ? a.top_p[r] : 1.0f, a.min_p ? a.min_p[r] : 0.0f, a.uniform[r],
+                a.top_k && (uint64_t)a.top_k[r] < a.cols ? a.top_k[r] : 0};
+}
+
+__device__ inline bool is_greedy(const Params &q) { return !(q.t > 0.0f) || q.m > 1.0f; }  // no class but the first has a weight above 1
+
+__device__ inline void write_none(const SampleArgs &a, uint64_t r) {
+  if (threadIdx.x != 0) return;
+  a.token[r] = -1;
+  if (a.logprob) a.logprob[r] = -INFINITY;
+}
+
+// the row's largest logit, from the groups' or (rows so short that k_sample_tops has not run) the row itself
+template <class T, bool TOPS>
+__device__ inline float row_top(const SampleArgs &a, uint64_t r, const Chunks<T> &row, Shared &sh) {
+  constexpr int K = 16 / sizeof(T);
+  float top = -INFINITY;
+  if (TOPS) {
+    for (int64_t g = threadIdx.x; g < (row.count + kGroup - 1) / kGroup; g += kThreads) top = fmaxf(top, a.tops[r * a.groups + g]);
+  } else {
+    for (int64_t c = threadIdx.x; c < row.count; c += kThreads) {
+      const vec_t<T, K> x = row.load(c, (T)-INFINITY);
+#pragma unroll
+      for (int k = 0; k < K; ++k) top = fmaxf(top, (float)x[k]);
+    }
+  }
+  return logit_of((uint32_t)block_min(key_of(top), sh));
+}
 
 template <class T>
 __global__ void __launch_bounds__(256) k_sample_tops(SampleArgs a) {
@@ -304,29 +333,6 @@ struct ListSource {
   }
 };
 
-struct Params {
-  float t, p, m, u;
-  int32_t k;
-};
-
-__device__ inline unsigned long long mass_target(float p, unsigned long long mass) {
-  const double bound = p > 0.0f ? ceil((double)p * (double)mass) : 0.0;
-  return bound < 1.0 ? 1ull : (unsigned long long)bound;
-}
-
-__device__ inline unsigned long long draw_target(float u, unsigned long long total) {
-  const double at = floor((double)u * (double)total);
-  const unsigned long long target = at < (double)total ? (unsigned long long)at + 1 : total;
-  return target < total ? target : total;
-}
-
-__device__ inline void write_token(const SampleArgs &a, uint64_t r, unsigned long long token, float x, const Weights &w, float t, unsigned long long total) {
-  a.token[r] = (int32_t)token;
-  if (!a.logprob) return;
-  const double y = x == w.top ? 0.0 : ((double)x - (double)w.top) / (double)t;
-  a.logprob[r] = (float)(y - log(ldexp((double)total, -a.shift)));
-}
-
 // sum of `v` over the `each` threads that share a class
 template <class V>
 __device__ inline V among(V v, int each) {
@@ -335,7 +341,7 @@ __device__ inline V among(V v, int each) {
 }
 
 // All filters and the draw among up to kPairs classes: every class against every other, `each` threads a class.
-__device__ inline void draw_pairs(const SampleArgs &a, uint64_t r, const Params &q, const Weights &weight, unsigned long long first, RowShared &s, int count) {
+__device__ inline void draw_pairs(const SampleArgs &a, uint64_t r, const Params &q, const Weights &weight, unsigned long long first, ListShared &s, int count) {
   int log_each = 0;
   while (log_each < 6 && (count << (log_each + 1)) <= kThreads) ++log_each;
   const int each = 1 << log_each, mine = threadIdx.x >> log_each, part = threadIdx.x & (each - 1);
@@ -358,7 +364,7 @@ __device__ inline void draw_pairs(const SampleArgs &a, uint64_t r, const Params 
     before = among(before, each);
     kept = kept && before < mass_target(q.p, mass);
   }
-  if (q.m > 0.0f) kept = kept && (weight.passes(w, q.m) || o == first);
+  kept = kept && (w >= weight.least || o == first);
   __syncthreads();
   if (in && part == 0) s.units[mine] = kept ? units : 0;
   const unsigned long long total = block_sum(kept && part == 0 ? units : 0, s.sh);
@@ -367,23 +373,24 @@ __device__ inline void draw_pairs(const SampleArgs &a, uint64_t r, const Params 
   for (int i = part; i < count; i += each) upto += (s.list[i] & mask) <= (o & mask) ? s.units[i] : 0;
   upto = among(upto, each);
   const unsigned long long token = block_min(kept && upto >= target ? o & mask : ~0ull, s.sh);
-  if (kept && part == 0 && (o & mask) == token) write_token(a, r, token, x, weight, q.t, total);
+  if (kept && part == 0 && (o & mask) == token) write_token(a, r, (uint32_t)token, x, weight, q.t, total);
 }
 
 // The first class, in the order of the indexes, at which the amounts of the granules [c0, c1) reach `target`; visit(x, j) is
 // a class's amount, hit(x, j) gets the class.
 template <class T, class Amount, class Hit>
-__device__ inline void find_class(const Chunks<T> &row, int64_t c0, int64_t c1, unsigned long long target, Shared &sh, Amount amount, Hit hit) {
-  constexpr int K = 16 / sizeof(T);
+__device__ inline void find_class(const Chunks<T, 8> &row, int64_t c0, int64_t c1, unsigned long long target, Shared &sh, Amount amount, Hit hit) {
+  constexpr int K = 8 / sizeof(T);
+#pragma unroll 1
   for (int64_t b = c0; b < c1; b += kThreads) {
     const int64_t c = b + threadIdx.x;
     vec_t<T, K> x = (T)-INFINITY;
     if (c < c1) x = row.load(c, (T)-INFINITY);
-    unsigned long long mine = 0;
+    unsigned long long u[K], mine = 0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (k % 2 == 0) __builtin_amdgcn_sched_barrier(0);
-      mine += amount((float)x[k], c * K + k - row.lead);
+      u[k] = amount((float)x[k], c * K + k - row.lead);
+      mine += u[k];
     }
     unsigned long long up = mine;
     for (int off = 1; off < 64; off <<= 1) {
@@ -400,17 +407,10 @@ __device__ inline void find_class(const Chunks<T> &row, int64_t c0, int64_t c1, 
     }
     if (all >= target) {  // uniform
       unsigned long long sum = up - mine;
-      if (sum < target && target <= up) {
-        bool done = false;
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          if (k % 2 == 0) __builtin_amdgcn_sched_barrier(0);
-          sum += amount((float)x[k], c * K + k - row.lead);
-          if (!done && sum >= target) {
-            hit((float)x[k], c * K + k - row.lead);
-            done = true;
-          }
-        }
+      for (int k = 0; k < K; ++k) {
+        if (sum < target && target <= sum + u[k]) hit((float)x[k], c * K + k - row.lead);
+        sum += u[k];
       }
       return;
     }
@@ -420,8 +420,8 @@ __device__ inline void find_class(const Chunks<T> &row, int64_t c0, int64_t c1, 
 
 // top-p, min-p or neither, by buckets and parts; false where the row does not fit this
 template <class T>
-__device__ inline bool draw_parts(const SampleArgs &a, uint64_t r, const Params &q, const Chunks<T> &row, const Weights &weight, RowShared &s) {
-  constexpr int K = 16 / sizeof(T);
+__device__ inline bool draw_parts(const SampleArgs &a, uint64_t r, const Params &q, const Chunks<T, 8> &row, const Weights &weight, PartsShared &s) {
+  constexpr int K = 8 / sizeof(T);  // narrow granules: the arithmetic is the bound, and eight classes at once take too many registers
   const T none = (T)-INFINITY;
   const int64_t span = (row.count + kParts - 1) / kParts;
   const float top = weight.top;
@@ -431,8 +431,8 @@ __device__ inline bool draw_parts(const SampleArgs &a, uint64_t r, const Params 
   if (q.p < 1.0f) {
     // buckets of equal width in the logit, down to weights of (1 - p) / cols, and one power of two more for the roundings
     const double depth = log2((double)row.cols / (1.0 - (double)q.p)) + 1.0;
-    const float scale = (float)(weight.per * kBuckets / (depth > 1.0 ? depth : 1.0));
-    auto bucket = [&](float x) { return x == top ? 0 : (int)fminf((top - x) * scale, (float)kBuckets); };
+    const float scale = fminf((float)(weight.per * kBuckets / (depth > 1.0 ? depth : 1.0)), 0x1p100f);  // (0 times infinity is no bucket)
+    auto bucket = [&](float x) { return (int)fminf((top - x) * scale, (float)kBuckets); };
     for (int i = threadIdx.x; i < kParts * kBuckets; i += kThreads) (&s.hist[0][0])[i] = 0;
     if (threadIdx.x == 0) {
       s.count = 0;
@@ -440,18 +440,19 @@ __device__ inline bool draw_parts(const SampleArgs &a, uint64_t r, const Params 
     }
     __syncthreads();
     unsigned long long rest = 0, above = 0;  // below the buckets; passing min-p
+#pragma unroll 1
     for (int part = 0; part < kParts; ++part) {
+#pragma unroll 1
       for (int64_t c = start(part) + threadIdx.x; c < start(part + 1); c += kThreads) {
         const vec_t<T, K> x = row.load(c, none);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-          if (k % 2 == 0) __builtin_amdgcn_sched_barrier(0);  // two at a time: eight would take all registers
           const double w = weight.scaled((float)x[k]);
           const unsigned long long u = weight.units(w);
           const int b = bucket((float)x[k]);
           if (b < kBuckets) atomicAdd(&s.hist[part][b], u);
           else rest += u;
-          if (q.m > 0.0f && weight.passes(w, q.m)) above += u;
+          if (q.m > 0.0f) above += w >= weight.least ? u : 0;
         }
       }
     }
@@ -495,6 +496,7 @@ __device__ inline bool draw_parts(const SampleArgs &a, uint64_t r, const Params 
       const int border = (int)s.sh.found;
       const unsigned long long within = target - s.sh.before;
       // the classes of the bucket that the target falls into
+#pragma unroll 1
       for (int64_t c = threadIdx.x; c < row.count; c += kThreads) {
         const vec_t<T, K> x = row.load(c, none);
 #pragma unroll
@@ -534,12 +536,14 @@ __device__ inline bool draw_parts(const SampleArgs &a, uint64_t r, const Params 
       __syncthreads();
       unsigned long long part_mass = 0;
       if (threadIdx.x / 64 < kParts) {
+#pragma unroll 1
         for (int b = threadIdx.x & 63; b <= border; b += 64) part_mass += s.hist[threadIdx.x / 64][b];
         for (int off = 1; off < 64; off <<= 1) part_mass += __shfl_xor(part_mass, off, 64);
         if ((threadIdx.x & 63) == 0) s.units[threadIdx.x / 64] = part_mass;
       }
       __syncthreads();
       unsigned long long kept = 0;
+#pragma unroll 1
       for (int part = 0; part < kParts; ++part) kept += s.units[part];
       unsigned long long at = draw_target(q.u, kept);
       int part = 0;
@@ -550,24 +554,23 @@ __device__ inline bool draw_parts(const SampleArgs &a, uint64_t r, const Params 
                    if (b > border || (b == border && ((unsigned long long)key_of(x) << a.index_bits | (unsigned long long)j) > last)) return 0;
                    return weight.units(weight.scaled(x));
                  },
-                 [&](float x, int64_t j) { write_token(a, r, (unsigned long long)j, x, weight, q.t, kept); });
+                 [&](float x, int64_t j) { write_token(a, r, (uint32_t)j, x, weight, q.t, kept); });
       return true;
     }
   }
   unsigned long long total = 0;
   auto amount = [&](float x, int64_t) -> unsigned long long {
     const double w = weight.scaled(x);
-    return weight.passes(w, q.m) ? weight.units(w) : 0;
+    return w >= weight.least ? weight.units(w) : 0;
   };
+#pragma unroll 1
   for (int part = 0; part < kParts; ++part) {
     unsigned long long mine = 0;
+#pragma unroll 1
     for (int64_t c = start(part) + threadIdx.x; c < start(part + 1); c += kThreads) {
       const vec_t<T, K> x = row.load(c, none);
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (k % 2 == 0) __builtin_amdgcn_sched_barrier(0);
-        mine += amount((float)x[k], 0);
-      }
+      for (int k = 0; k < K; ++k) mine += amount((float)x[k], 0);
     }
     mine = block_sum(mine, s.sh);
     if (threadIdx.x == 0) s.units[part] = mine;
@@ -578,29 +581,29 @@ __device__ inline bool draw_parts(const SampleArgs &a, uint64_t r, const Params 
   int part = 0;
   while (part < kParts - 1 && at > s.units[part]) at -= s.units[part++];
   find_class(row, start(part), start(part + 1), at, s.sh, amount,
-             [&](float x, int64_t j) { write_token(a, r, (unsigned long long)j, x, weight, q.t, total); });
+             [&](float x, int64_t j) { write_token(a, r, (uint32_t)j, x, weight, q.t, total); });
   return true;
 }
 
 template <class T, bool TOPS>
-__global__ void __launch_bounds__(kThreads) k_sample_rows(SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) k_sample_list(SampleArgs a) {
   constexpr int K = 16 / sizeof(T);
-  __shared__ RowShared s;
+  __shared__ ListShared s;
   const T none = (T)-INFINITY;
   for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     __syncthreads();
     const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int64_t)a.cols);
-    const RowSource<T> whole{row};
-    const Params q{a.temperature ? a.temperature[r] : 1.0f, a.top_p ? a.top_p[r] : 1.0f, a.min_p ? a.min_p[r] : 0.0f, a.uniform[r],
-                   a.top_k && (uint64_t)a.top_k[r] < a.cols ? a.top_k[r] : 0};
+    const Params q = params_of(a, r);
     const int64_t small = (row.count + kGroup - 1) / kGroup, size = (small + kMaxGroups - 1) / kMaxGroups;
     const int groups = (int)((small + size - 1) / size);  // of `size` times kGroup granules
-    // the groups' largest logits
+    // the groups' largest logits, and the row's
+    float top = -INFINITY;
     if (TOPS) {
       for (int g = threadIdx.x; g < groups; g += kThreads) {
         float m = -INFINITY;
         for (int64_t i = g * size; i < (g + 1) * size && i < small; ++i) m = fmaxf(m, a.tops[r * a.groups + i]);
         s.tops[g] = m;
+        top = fmaxf(top, m);
       }
     } else {
       for (int64_t c = threadIdx.x; c < (int64_t)groups * kGroup; c += kThreads) {
@@ -612,71 +615,149 @@ __global__ void __launch_bounds__(kThreads) k_sample_rows(SampleArgs a) {
         }
         for (int off = 1; off < kGroup; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
         if (c % kGroup == 0) s.tops[c / kGroup] = m;
+        top = fmaxf(top, m);
       }
     }
-    if (threadIdx.x == 0) {
-      s.count = 0;
-      s.bound = -INFINITY;
+    if (threadIdx.x == 0) s.count = s.nhits = 0;
+    top = logit_of((uint32_t)block_min(key_of(top), s.sh));
+    if (top == -INFINITY) {  // uniform, as everything that skips a barrier here
+      write_none(a, r);
+      continue;
+    }
+    const bool greedy = is_greedy(q);
+    const int want = greedy ? 1 : q.k;
+    if (!greedy && (want == 0 || want > groups || !(q.u > 0.0f) || top == INFINITY)) {
+      if (threadIdx.x == 0) a.token[r] = kLeft;
+      continue;
+    }
+    // the want-th largest of the groups' largest logits: by one wave, bisecting their keys; a bound that a few more reach does
+    // as well
+    if (threadIdx.x < 64) {
+      uint32_t lo = key_of(top), hi = key_of(-INFINITY);  // the bound's key is between them
+      uint32_t mine[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine[i] = (int)threadIdx.x + 64 * i < groups ? key_of(s.tops[threadIdx.x + 64 * i]) : 0xFFFFFFFFu;
+      while (lo < hi) {
+        const uint32_t mid = lo + ((hi - lo) >> 1);
+        int have = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) have += __popcll(__ballot(mine[i] <= mid));
+        for (int g = 512 + threadIdx.x; g < (groups + 63) / 64 * 64; g += 64) have += __popcll(__ballot(g < groups && key_of(s.tops[g]) <= mid));
+        if (have >= want) hi = mid;
+        else lo = mid + 1;
+        if (have >= want && have <= want + want / 8) break;
+      }
+      if (threadIdx.x == 0) s.bound = hi;
     }
     __syncthreads();
-    float top = -INFINITY;
-    for (int g = threadIdx.x; g < groups; g += kThreads) top = fmaxf(top, s.tops[g]);
-    for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-    top = logit_of((uint32_t)block_min(key_of(top), s.sh));
-    const bool greedy = !(q.t > 0.0f) || q.m > 1.0f;  // no class but the first has a weight above 1
-    auto put = [&](float v, int64_t j) {
-      const unsigned at = atomicAdd(&s.count, 1u);
-      if (at < (unsigned)kList) s.list[at] = (unsigned long long)key_of(v) << a.index_bits | (unsigned long long)j;
-    };
-    const int want = greedy ? 1 : q.k;
-    if (top > -INFINITY && want > 0 && want <= groups) {
-      // the want-th largest of the groups': rank by comparison
-      for (int g = threadIdx.x; g < groups; g += kThreads) {
-        const float v = s.tops[g];
-        int above = 0, same = 0;
-        for (int i = 0; i < groups; ++i) {
-          above += s.tops[i] > v;
-          same += s.tops[i] == v;
-        }
-        if (above < want && want <= above + same) s.bound = v;  // all that write, write the same
-      }
-      __syncthreads();
-      const float bound = s.bound;
-      // the classes from it on
-      const int lane = threadIdx.x & (kGroup - 1);
-      for (int g = threadIdx.x / kGroup; g < groups; g += kThreads / kGroup) {
-        if (s.tops[g] < bound) continue;
-        for (int64_t c = (int64_t)g * size * kGroup + lane; c < (int64_t)(g + 1) * size * kGroup && c < row.count; c += kGroup) {
-          const vec_t<T, K> x = row.load(c, none);
+    const float bound = logit_of(s.bound);
+    for (int g = threadIdx.x; g < groups; g += kThreads)
+      if (s.tops[g] >= bound) s.hits[atomicAdd(&s.nhits, 1u)] = g;
+    __syncthreads();
+    // the classes from the bound on
+    unsigned long long first = ~0ull;
+    const unsigned per = (unsigned)(size * kGroup), granules = s.nhits * per;  // at most the row's 2^31 / K and kMaxGroups' rounding
+    for (unsigned i = threadIdx.x; i < granules; i += 4 * kThreads) {
+      vec_t<T, K> x[4];
+      int64_t c[4];
 #pragma unroll
-          for (int k = 0; k < K; ++k) {
-            const float v = (float)x[k];
-            const int64_t j = c * K + k - row.lead;
-            if (v >= bound && j >= 0 && j < row.cols) put(v, j);
-          }
-        }
+      for (int u = 0; u < 4; ++u) {
+        const unsigned at = i + u * kThreads;
+        c[u] = at < granules ? (int64_t)s.hits[at / per] * per + at % per : row.count;
+        if (c[u] < row.count) x[u] = row.load(c[u], none);
       }
-      __syncthreads();
-      const unsigned count = s.count;
-      if (count <= (unsigned)kList && (greedy || q.u > 0.0f)) {
-        unsigned long long first = ~0ull;
-        for (unsigned i = threadIdx.x; i < count; i += kThreads) first = s.list[i] < first ? s.list[i] : first;
-        first = block_min(first, s.sh);
-        if (greedy) {
-          if (threadIdx.x == 0) {
-            a.token[r] = (int32_t)(first & ((1ull << a.index_bits) - 1));
-            if (a.logprob) a.logprob[r] = 0.0f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (c[u] >= row.count) continue;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const float v = (float)x[u][k];
+          const int64_t j = c[u] * K + k - row.lead;
+          if (v >= bound && j >= 0 && j < row.cols) {
+            const unsigned at = atomicAdd(&s.count, 1u);
+            const unsigned long long o = (unsigned long long)key_of(v) << a.index_bits | (unsigned long long)j;
+            if (at < (unsigned)kPairs) s.list[at] = o;
+            first = o < first ? o : first;
           }
-        } else if (count <= (unsigned)kPairs) {
-          draw_pairs(a, r, q, Weights{top, 1.44269504088896340736 / (double)q.t, a.shift}, first, s, (int)count);
-        } else {
-          draw_row(a, r, ListSource{s.list, (int)count, a.index_bits}, s.sh);
         }
-        continue;
       }
     }
-    if (top > -INFINITY && !greedy && q.k == 0 && q.u > 0.0f && draw_parts(a, r, q, row, Weights{top, 1.44269504088896340736 / (double)q.t, a.shift}, s)) continue;
-    draw_row(a, r, whole, s.sh);
+    first = block_min(first, s.sh);
+    if (greedy) {
+      if (threadIdx.x == 0) {
+        a.token[r] = (int32_t)(first & ((1ull << a.index_bits) - 1));
+        if (a.logprob) a.logprob[r] = 0.0f;
+      }
+    } else if (s.count <= (unsigned)kPairs) {
+      draw_pairs(a, r, q, Weights(top, q.t, q.m, a.shift), first, s, (int)s.count);
+    } else if (threadIdx.x == 0) {
+      a.token[r] = kLeft;
+    }
+  }
+}
+
+// FIRST: no kernel before it has drawn rows
+template <class T, bool TOPS, bool FIRST>
+__global__ void __launch_bounds__(kThreads, 4) k_sample_parts(SampleArgs a) {
+  __shared__ PartsShared s;
+  for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    if (!FIRST && a.token[r] != kLeft) continue;
+    __syncthreads();
+    const T *logits = static_cast<const T *>(a.logits) + r * a.stride;
+    const Params q = params_of(a, r);
+    if (q.k > 0) continue;
+    const float top = row_top<T, TOPS>(a, r, Chunks<T>(logits, (int64_t)a.cols), s.sh);
+    if (top == -INFINITY) {
+      write_none(a, r);
+      continue;
+    }
+    if (is_greedy(q)) {
+      const Chunks<T> row(logits, (int64_t)a.cols);
+      unsigned long long first = ~0ull;
+      for (int64_t c = threadIdx.x; c < row.count; c += kThreads) {
+        const vec_t<T, 16 / sizeof(T)> x = row.load(c, (T)-INFINITY);
+#pragma unroll
+        for (int k = 16 / sizeof(T) - 1; k >= 0; --k)
+          if ((float)x[k] == top) first = (unsigned long long)(c * (int64_t)(16 / sizeof(T)) + k - row.lead);
+        if (first != ~0ull) break;
+      }
+      first = block_min(first, s.sh);
+      if (threadIdx.x == 0) {
+        a.token[r] = (int32_t)first;
+        if (a.logprob) a.logprob[r] = 0.0f;
+      }
+      continue;
+    }
+    const bool done = q.u > 0.0f && top < INFINITY &&
+                      draw_parts(a, r, q, Chunks<T, 8>(logits, (int64_t)a.cols), Weights(top, q.t, q.m, a.shift), s);
+    if (!done && threadIdx.x == 0) a.token[r] = kLeft;
+  }
+}
+
+template <class T, bool TOPS>
+__global__ void __launch_bounds__(kThreads) k_sample_any(SampleArgs a) {
+  __shared__ Shared sh;
+  for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    if (a.token[r] != kLeft) continue;
+    __syncthreads();
+    const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int64_t)a.cols);
+    const Params q = params_of(a, r);
+    const float top = row_top<T, TOPS>(a, r, row, sh);
+    const RowSource<T> source{row.base + row.lead, row.cols};
+    unsigned long long first = ~0ull;
+    source.each([&](float x, uint32_t j) {
+      const unsigned long long o = (unsigned long long)key_of(x) << a.index_bits | j;
+      first = o < first ? o : first;
+    });
+    first = block_min(first, sh);
+    if (is_greedy(q)) {
+      if (threadIdx.x == 0) {
+        a.token[r] = (int32_t)(first & ((1ull << a.index_bits) - 1));
+        if (a.logprob) a.logprob[r] = 0.0f;
+      }
+    } else {
+      draw_row(a, r, q, Weights(top, q.t, q.m, a.shift), first, source, sh);
+    }
   }
 }
 
@@ -689,9 +770,15 @@ static uint64_t tops_groups(uint64_t cols, uint64_t per) { return ((cols + per -
 template <class T>
 static int sample(admm_ctx *ctx, SampleArgs a) {
   a.groups = (int64_t)tops_groups(a.cols, 16 / sizeof(T));
-  const dim3 grid(blocks_for(a.rows, 1));
+  const dim3 grid(blocks_for(a.rows, 1)), block(kThreads);
   if (a.cols <= kTopsFrom) {
-    hipLaunchKernelGGL((k_sample_rows<T, false>), grid, dim3(kThreads), 0, ctx->stream, a);
+    if (a.top_k) {
+      hipLaunchKernelGGL((k_sample_list<T, false>), grid, block, 0, ctx->stream, a);
+      hipLaunchKernelGGL((k_sample_parts<T, false, false>), grid, block, 0, ctx->stream, a);
+    } else {
+      hipLaunchKernelGGL((k_sample_parts<T, false, true>), grid, block, 0, ctx->stream, a);
+    }
+    hipLaunchKernelGGL((k_sample_any<T, false>), grid, block, 0, ctx->stream, a);
   } else {
     const unsigned per_row = (unsigned)((a.groups * kGroup + kTopsPer - 1) / kTopsPer);
     for (uint64_t r = 0; r < a.rows; r += 65535) {  // rows are the second dimension of the grid
@@ -701,7 +788,13 @@ static int sample(admm_ctx *ctx, SampleArgs a) {
       const unsigned rows = (unsigned)(a.rows - r < 65535 ? a.rows - r : 65535);
       hipLaunchKernelGGL(k_sample_tops<T>, dim3(per_row, rows), dim3(256), 0, ctx->stream, b);
     }
-    hipLaunchKernelGGL((k_sample_rows<T, true>), grid, dim3(kThreads), 0, ctx->stream, a);
+    if (a.top_k) {
+      hipLaunchKernelGGL((k_sample_list<T, true>), grid, block, 0, ctx->stream, a);
+      hipLaunchKernelGGL((k_sample_parts<T, true, false>), grid, block, 0, ctx->stream, a);
+    } else {
+      hipLaunchKernelGGL((k_sample_parts<T, true, true>), grid, block, 0, ctx->stream, a);
+    }
+    hipLaunchKernelGGL((k_sample_any<T, true>), grid, block, 0, ctx->stream, a);
   }
   ADMM_HIP_CHECK(hipGetLastError());
   return ADMM_OK;
