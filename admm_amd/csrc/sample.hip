@@ -25,6 +25,7 @@ struct SampleArgs {
   int index_bits, shift;  // 2^index_bits >= cols; S
   float *tops;            // [rows][groups] largest logits of kGroup granules each
   int64_t groups;
+  unsigned long long *sums;  // [rows of a batch][kParts][kSums]
 };
 
 // larger logits have smaller keys; -0 counts as 0 and NaN as -inf
@@ -87,6 +88,7 @@ struct Shared {
   unsigned long long found, before;
 };
 
+template <int NT = kThreads>
 __device__ inline unsigned long long block_sum(unsigned long long v, Shared &sh) {
   for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
   __syncthreads();
@@ -94,10 +96,11 @@ __device__ inline unsigned long long block_sum(unsigned long long v, Shared &sh)
   __syncthreads();
   v = 0;
 #pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i) v += sh.sums[i];
+  for (int i = 0; i < NT / 64; ++i) v += sh.sums[i];
   return v;
 }
 
+template <int NT = kThreads>
 __device__ inline unsigned long long block_min(unsigned long long v, Shared &sh) {
   for (int off = 1; off < 64; off <<= 1) {
     const unsigned long long o = __shfl_xor(v, off, 64);
@@ -108,7 +111,7 @@ __device__ inline unsigned long long block_min(unsigned long long v, Shared &sh)
   __syncthreads();
   v = sh.sums[0];
 #pragma unroll
-  for (int i = 1; i < kThreads / 64; ++i) v = sh.sums[i] < v ? sh.sums[i] : v;
+  for (int i = 1; i < NT / 64; ++i) v = sh.sums[i] < v ? sh.sums[i] : v;
   return v;
 }
 
@@ -232,20 +235,19 @@ __device__ inline void draw_row(const SampleArgs &a, uint64_t r, const Params &q
 
 // ---- rows in a few launches ----------------------------------------------------------------------------
 //
-// k_sample_tops reads the logits once, with as many workgroups as there are, and leaves the largest logit of every kGroup
-// granules.  The other kernels have a workgroup per row, know from those the row's largest logit, and read the row again
-// (from the caches), or little of it:
-//  * k_sample_list (where top-k is given): the k-th largest logit is not below the k-th largest of the groups'.  The classes from
-//    that bound on are few; everything else happens among them in LDS.
-//  * k_sample_parts (the rows without top-k).  For top-p the weights are summed by kBuckets buckets of the logit and by kParts
-//    parts of the row.  The target falls into one bucket, whose classes are put in order; what is kept of each part is known
-//    then, and only the part where the draw falls is read again.  Weights below (1 - p) / cols of the largest take no part in
-//    the buckets: together they are less than 1 - p of the whole.  Without top-p the same parts, without buckets; min-p is a
-//    bound on the weight.
-//  * k_sample_any: rows that do not fit this (too many classes between a bound and a border, a k larger than the number of
-//    groups, u <= 0, logits of +inf) are drawn by draw_row from the whole row, to the same result: all sums are the same integers.
-// A row that is left to a later kernel has the token kLeft.  One kernel for all of it is slower: it takes so many registers
-// that it spills, and a single row of 128000 classes with top-k took 43 us in it.
+//  * k_sample_tops reads the logits once, with as many workgroups as there are, and leaves the largest logit of every kGroup
+//    granules.  What follows knows from those the row's largest logit and reads the row again from the caches.
+//  * k_sample_list (where top-k is given), a workgroup per row: the k-th largest logit is not below the k-th largest of the
+//    groups'.  The classes from that bound on are few; everything else happens among them in LDS.
+//  * k_sample_sums (the rows without top-k), kParts workgroups per row: for top-p the weights are summed by kBuckets buckets of
+//    the logit.  Weights below (1 - p) / cols of the largest take no part in the buckets: together they are less than 1 - p of
+//    the whole.  Without top-p there is one sum; min-p is a bound on the weight.
+//  * k_sample_rest, a workgroup per row: the target of top-p falls into one bucket, whose classes are put in order; what is kept
+//    of each part is known then, and only the part where the draw falls is read again.  Rows that do not fit any of this
+//    (too many classes between a bound and a border, a large k, u <= 0, logits of +inf) are drawn by draw_row from the whole
+//    row, to the same result: all sums are the same integers.
+// A row that is left to a later kernel has the token kLeft.  One kernel for all of it took 43 us for a row of 128000 classes
+// with top-k, where k_sample_list takes 15, and 290 for 512 rows with top-p.
 
 constexpr int kGroup = 32;       // granules
 constexpr int kTopsPer = 512;    // granules per workgroup of k_sample_tops
@@ -253,6 +255,8 @@ constexpr int kMaxGroups = 4096; // groups whose largest logits fit LDS beside t
 constexpr int kList = 2048;      // classes kept in LDS
 constexpr int kPairs = 512;      // of which all pairs are compared, not sorted digit by digit
 constexpr int kBuckets = 512, kParts = 8;
+constexpr int kSums = kBuckets + 2;   // the buckets of a part, what is below them, what passes min-p
+constexpr uint64_t kBatch = 1024;     // rows whose sums the workspace holds at once
 constexpr int32_t kLeft = -2;
 
 struct ListShared {
@@ -264,7 +268,7 @@ struct ListShared {
   unsigned int count, nhits, bound;
 };
 
-struct PartsShared {
+struct RestShared {
   unsigned long long hist[kParts][kBuckets];
   unsigned long long list[kList], units[kPairs];
   Shared sh;
@@ -284,22 +288,27 @@ __device__ inline void write_none(const SampleArgs &a, uint64_t r) {
   if (a.logprob) a.logprob[r] = -INFINITY;
 }
 
-// the row's largest logit, from the groups' or (rows so short that k_sample_tops has not run) the row itself
-template <class T, bool TOPS>
-__device__ inline float row_top(const SampleArgs &a, uint64_t r, const Chunks<T> &row, Shared &sh) {
-  constexpr int K = 16 / sizeof(T);
+// the row's largest logit, from the groups'
+template <int NT>
+__device__ inline float row_top(const SampleArgs &a, uint64_t r, Shared &sh) {
   float top = -INFINITY;
-  if (TOPS) {
-    for (int64_t g = threadIdx.x; g < (row.count + kGroup - 1) / kGroup; g += kThreads) top = fmaxf(top, a.tops[r * a.groups + g]);
-  } else {
-    for (int64_t c = threadIdx.x; c < row.count; c += kThreads) {
-      const vec_t<T, K> x = row.load(c, (T)-INFINITY);
-#pragma unroll
-      for (int k = 0; k < K; ++k) top = fmaxf(top, (float)x[k]);
-    }
-  }
-  return logit_of((uint32_t)block_min(key_of(top), sh));
+  for (int64_t g = threadIdx.x; g < a.groups; g += NT) top = fmaxf(top, a.tops[r * a.groups + g]);
+  return logit_of((uint32_t)block_min<NT>(key_of(top), sh));
 }
+
+// Buckets of equal width in the logit, for top-p: down to weights of (1 - p) / cols, and one power of two more for the
+// roundings; kBuckets and beyond: below them.
+struct Buckets {
+  float top, scale;
+  __device__ Buckets(const Params &q, const Weights &w, uint64_t cols) : top(w.top) {
+    const double depth = log2((double)cols / (1.0 - (double)q.p)) + 1.0;
+    scale = fminf((float)(w.per * kBuckets / (depth > 1.0 ? depth : 1.0)), 0x1p100f);  // 0 times infinity would be no bucket
+  }
+  __device__ int of(float x) const { return (int)fminf((top - x) * scale, (float)kBuckets); }
+};
+
+// is a row of this kind drawn by its sums?
+__device__ inline bool by_sums(const Params &q, float top) { return q.k == 0 && q.u > 0.0f && top > -INFINITY && top < INFINITY && !is_greedy(q); }
 
 template <class T>
 __global__ void __launch_bounds__(256) k_sample_tops(SampleArgs a) {
@@ -418,109 +427,153 @@ __device__ inline void find_class(const Chunks<T, 8> &row, int64_t c0, int64_t c
   }
 }
 
-// top-p, min-p or neither, by buckets and parts; false where the row does not fit this
+// granules of a part of a row
+struct Part {
+  int64_t first, last;
+  __device__ Part(int64_t count, int part) {
+    const int64_t span = (count + kParts - 1) / kParts;
+    first = part * span < count ? part * span : count;
+    last = first + span < count ? first + span : count;
+  }
+};
+
 template <class T>
-__device__ inline bool draw_parts(const SampleArgs &a, uint64_t r, const Params &q, const Chunks<T, 8> &row, const Weights &weight, PartsShared &s) {
+__global__ void __launch_bounds__(256) k_sample_sums(SampleArgs a, uint64_t r0) {
   constexpr int K = 8 / sizeof(T);  // narrow granules: the arithmetic is the bound, and eight classes at once take too many registers
+  __shared__ unsigned long long hist[kBuckets];
+  __shared__ Shared sh;
+  const uint64_t r = r0 + blockIdx.y;
+  if (a.top_k && a.token[r] != kLeft) return;
+  const Params q = params_of(a, r);
+  const float top = row_top<256>(a, r, sh);
+  if (!by_sums(q, top)) return;
+  const Weights weight(top, q.t, q.m, a.shift);
+  const Chunks<T, 8> row(static_cast<const T *>(a.logits) + r * a.stride, (int64_t)a.cols);
+  const Part part(row.count, (int)blockIdx.x);
   const T none = (T)-INFINITY;
-  const int64_t span = (row.count + kParts - 1) / kParts;
-  const float top = weight.top;
-  auto start = [&](int part) { return part * span < row.count ? part * span : row.count; };
-  auto in_row = [&](int64_t j) { return j >= 0 && j < row.cols; };
-  __syncthreads();  // tops and list are free
+  unsigned long long *to = a.sums + (blockIdx.y * kParts + blockIdx.x) * (uint64_t)kSums;
+  unsigned long long rest = 0, above = 0;  // below the buckets; passing min-p
   if (q.p < 1.0f) {
-    // buckets of equal width in the logit, down to weights of (1 - p) / cols, and one power of two more for the roundings
-    const double depth = log2((double)row.cols / (1.0 - (double)q.p)) + 1.0;
-    const float scale = fminf((float)(weight.per * kBuckets / (depth > 1.0 ? depth : 1.0)), 0x1p100f);  // (0 times infinity is no bucket)
-    auto bucket = [&](float x) { return (int)fminf((top - x) * scale, (float)kBuckets); };
-    for (int i = threadIdx.x; i < kParts * kBuckets; i += kThreads) (&s.hist[0][0])[i] = 0;
+    const Buckets buckets(q, weight, a.cols);
+    for (int i = threadIdx.x; i < kBuckets; i += 256) hist[i] = 0;
+    __syncthreads();
+    for (int64_t c = part.first + threadIdx.x; c < part.last; c += 256) {
+      const vec_t<T, K> x = row.load(c, none);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const double w = weight.scaled((float)x[k]);
+        const unsigned long long u = weight.units(w);
+        const int b = buckets.of((float)x[k]);
+        if (b < kBuckets) atomicAdd(&hist[b], u);
+        else rest += u;
+        if (q.m > 0.0f) above += w >= weight.least ? u : 0;
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBuckets; i += 256) to[i] = hist[i];
+    rest = block_sum<256>(rest, sh);
+  }
+  if (q.p < 1.0f && q.m > 0.0f) {
+    above = block_sum<256>(above, sh);
+  } else if (!(q.p < 1.0f)) {
+    for (int64_t c = part.first + threadIdx.x; c < part.last; c += 256) {
+      const vec_t<T, K> x = row.load(c, none);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const double w = weight.scaled((float)x[k]);
+        above += w >= weight.least ? weight.units(w) : 0;
+      }
+    }
+    above = block_sum<256>(above, sh);
+  }
+  if (threadIdx.x == 0) {
+    to[kBuckets] = rest;
+    to[kBuckets + 1] = above;
+  }
+}
+
+// A row with its parts' sums; false where its border's bucket holds too many classes.
+template <class T>
+__device__ inline bool draw_sums(const SampleArgs &a, uint64_t r, const unsigned long long *sums, const Params &q, const Weights &weight, RestShared &s) {
+  const Chunks<T, 8> row(static_cast<const T *>(a.logits) + r * a.stride, (int64_t)a.cols);
+  bool nucleus = q.p < 1.0f;
+  const Buckets buckets(q, weight, a.cols);
+  int border = 0;
+  unsigned long long last = 0;
+  if (nucleus) {
+    unsigned long long mine = 0, above = 0;
+    static_assert(kThreads == kBuckets, "a bucket each");
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+      const unsigned long long v = sums[part * kSums + threadIdx.x];
+      s.hist[part][threadIdx.x] = v;
+      mine += v;
+      above += sums[part * kSums + kBuckets + 1];
+    }
+    unsigned long long up = mine;  // of the buckets up to this one
+    for (int off = 1; off < 64; off <<= 1) {
+      const unsigned long long y = __shfl_up(up, off, 64);
+      if ((int)(threadIdx.x & 63) >= off) up += y;
+    }
     if (threadIdx.x == 0) {
       s.count = 0;
       s.sh.found = ~0ull;
     }
+    if ((threadIdx.x & 63) == 63) s.sh.sums[threadIdx.x >> 6] = up;
     __syncthreads();
-    unsigned long long rest = 0, above = 0;  // below the buckets; passing min-p
-#pragma unroll 1
-    for (int part = 0; part < kParts; ++part) {
-#pragma unroll 1
-      for (int64_t c = start(part) + threadIdx.x; c < start(part + 1); c += kThreads) {
-        const vec_t<T, K> x = row.load(c, none);
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const double w = weight.scaled((float)x[k]);
-          const unsigned long long u = weight.units(w);
-          const int b = bucket((float)x[k]);
-          if (b < kBuckets) atomicAdd(&s.hist[part][b], u);
-          else rest += u;
-          if (q.m > 0.0f) above += w >= weight.least ? u : 0;
-        }
-      }
+    unsigned long long total = 0;
+    for (int i = 0; i < kThreads / 64; ++i) {
+      if (i == (int)(threadIdx.x >> 6)) up += total;
+      total += s.sh.sums[i];
     }
-    __syncthreads();
-    unsigned long long mine = rest;
-    if (threadIdx.x < kBuckets) {
-      unsigned long long col = 0;
-#pragma unroll
-      for (int part = 0; part < kParts; ++part) col += s.hist[part][threadIdx.x];
-      s.list[threadIdx.x] = col;
-      mine += col;
-    }
-    const unsigned long long total = block_sum(mine, s.sh), target = mass_target(q.p, total);
-    if (q.m > 0.0f) above = block_sum(above, s.sh);
-    if (!(q.m > 0.0f && target > above)) {  // else every class that passes min-p is among those that top-p keeps
-      if (threadIdx.x < 64) {
-        constexpr int kEach = kBuckets / 64;
-        unsigned long long x[kEach], sum = 0;
-#pragma unroll
-        for (int k = 0; k < kEach; ++k) {
-          x[k] = s.list[threadIdx.x * kEach + k];
-          sum += x[k];
-        }
-        unsigned long long up = sum;
-        for (int off = 1; off < 64; off <<= 1) {
-          const unsigned long long y = __shfl_up(up, off, 64);
-          if ((int)threadIdx.x >= off) up += y;
-        }
-        up -= sum;
-#pragma unroll
-        for (int k = 0; k < kEach; ++k) {
-          if (up < target && target <= up + x[k]) {
-            s.sh.found = threadIdx.x * kEach + k;
-            s.sh.before = up;
-          }
-          up += x[k];
-        }
+    for (int part = 0; part < kParts; ++part) total += sums[part * kSums + kBuckets];
+    const unsigned long long target = mass_target(q.p, total);
+    // where the target is beyond all that passes min-p, top-p keeps all of that and more
+    nucleus = !(q.m > 0.0f && target > above);
+    if (nucleus) {
+      if (up - mine < target && target <= up) {
+        s.sh.found = threadIdx.x;
+        s.sh.before = up - mine;
       }
       __syncthreads();
       if (s.sh.found == ~0ull) return false;
-      const int border = (int)s.sh.found;
+      border = (int)s.sh.found;
       const unsigned long long within = target - s.sh.before;
       // the classes of the bucket that the target falls into
-#pragma unroll 1
-      for (int64_t c = threadIdx.x; c < row.count; c += kThreads) {
-        const vec_t<T, K> x = row.load(c, none);
+      const Chunks<T> wide(static_cast<const T *>(a.logits) + r * a.stride, (int64_t)a.cols);
+      constexpr int K = 16 / sizeof(T), kAhead = 4;
+      for (int64_t c0 = threadIdx.x; c0 < wide.count; c0 += kAhead * kThreads) {
+        vec_t<T, K> x[kAhead];
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const int64_t j = c * K + k - row.lead;
-          if (bucket((float)x[k]) == border && in_row(j)) {
+        for (int u = 0; u < kAhead; ++u) {
+          x[u] = (T)-INFINITY;
+          if (c0 + u * kThreads < wide.count) x[u] = wide.load(c0 + u * kThreads, (T)-INFINITY);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            if (buckets.of((float)x[u][k]) != border) continue;  // what is not of the row is below all buckets
             const unsigned at = atomicAdd(&s.count, 1u);
-            if (at < (unsigned)kList) s.list[at] = (unsigned long long)key_of((float)x[k]) << a.index_bits | (unsigned long long)j;
+            if (at < (unsigned)kList) s.list[at] = (unsigned long long)key_of((float)x[u][k]) << a.index_bits | (unsigned long long)((c0 + u * kThreads) * K + k - wide.lead);
           }
         }
       }
       __syncthreads();
-      const unsigned count = s.count;
-      if (count > (unsigned)kList) return false;
-      const ListSource list{s.list, (int)count, a.index_bits};
-      unsigned long long last;
-      if (count <= (unsigned)kPairs) {
-        const unsigned long long o = threadIdx.x < count ? s.list[threadIdx.x] : ~0ull;
-        if (threadIdx.x < count) s.units[threadIdx.x] = weight.units(weight.scaled(logit_of((uint32_t)(o >> a.index_bits))));
+      const int count = (int)(s.count < (unsigned)kList + 1 ? s.count : (unsigned)kList + 1);
+      if (count > kList) return false;
+      const ListSource list{s.list, count, a.index_bits};
+      if (count <= kPairs) {
+        int log_each = 0;
+        while (log_each < 6 && (count << (log_each + 1)) <= kThreads) ++log_each;
+        const int each = 1 << log_each, me = threadIdx.x >> log_each;
+        const unsigned long long o = me < count ? s.list[me] : ~0ull;
+        if (threadIdx.x < count) s.units[threadIdx.x] = weight.units(weight.scaled(logit_of((uint32_t)(s.list[threadIdx.x] >> a.index_bits))));
         __syncthreads();
         unsigned long long upto = 0;
-        if (threadIdx.x < count)
-          for (unsigned i = 0; i < count; ++i) upto += s.list[i] <= o ? s.units[i] : 0;
-        last = block_min(threadIdx.x < count && upto >= within ? o : ~0ull, s.sh);
+        for (int i = threadIdx.x & (each - 1); i < count; i += each) upto += s.list[i] <= o ? s.units[i] : 0;
+        upto = among(upto, each);
+        last = block_min(me < count && upto >= within ? o : ~0ull, s.sh);
       } else {
         last = select_key(32 + a.index_bits, within, s.sh, [&](auto f) {
           list.each([&](float x, uint32_t j) { f((unsigned long long)key_of(x) << a.index_bits | j, weight.units(weight.scaled(x))); });
@@ -529,63 +582,43 @@ __device__ inline bool draw_parts(const SampleArgs &a, uint64_t r, const Params 
       // what is kept of every part
       if (threadIdx.x < kParts) s.hist[threadIdx.x][border] = 0;
       __syncthreads();
+      const int64_t span = (row.count + kParts - 1) / kParts;
       list.each([&](float x, uint32_t j) {
         if (((unsigned long long)key_of(x) << a.index_bits | j) > last) return;
-        atomicAdd(&s.hist[((int64_t)j + row.lead) / K / span][border], weight.units(weight.scaled(x)));
+        atomicAdd(&s.hist[((int64_t)j + row.lead) / (8 / (int)sizeof(T)) / span][border], weight.units(weight.scaled(x)));
       });
       __syncthreads();
-      unsigned long long part_mass = 0;
-      if (threadIdx.x / 64 < kParts) {
-#pragma unroll 1
-        for (int b = threadIdx.x & 63; b <= border; b += 64) part_mass += s.hist[threadIdx.x / 64][b];
-        for (int off = 1; off < 64; off <<= 1) part_mass += __shfl_xor(part_mass, off, 64);
-        if ((threadIdx.x & 63) == 0) s.units[threadIdx.x / 64] = part_mass;
-      }
-      __syncthreads();
+      static_assert(kThreads / 64 == kParts, "a wave each");
       unsigned long long kept = 0;
-#pragma unroll 1
-      for (int part = 0; part < kParts; ++part) kept += s.units[part];
-      unsigned long long at = draw_target(q.u, kept);
-      int part = 0;
-      while (part < kParts - 1 && at > s.units[part]) at -= s.units[part++];
-      find_class(row, start(part), start(part + 1), at, s.sh,
-                 [&](float x, int64_t j) -> unsigned long long {
-                   const int b = bucket(x);
-                   if (b > border || (b == border && ((unsigned long long)key_of(x) << a.index_bits | (unsigned long long)j) > last)) return 0;
-                   return weight.units(weight.scaled(x));
-                 },
-                 [&](float x, int64_t j) { write_token(a, r, (uint32_t)j, x, weight, q.t, kept); });
-      return true;
+      for (int b = threadIdx.x & 63; b <= border; b += 64) kept += s.hist[threadIdx.x / 64][b];
+      for (int off = 1; off < 64; off <<= 1) kept += __shfl_xor(kept, off, 64);
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) s.units[threadIdx.x / 64] = kept;
     }
   }
-  unsigned long long total = 0;
-  auto amount = [&](float x, int64_t) -> unsigned long long {
-    const double w = weight.scaled(x);
-    return w >= weight.least ? weight.units(w) : 0;
-  };
-#pragma unroll 1
-  for (int part = 0; part < kParts; ++part) {
-    unsigned long long mine = 0;
-#pragma unroll 1
-    for (int64_t c = start(part) + threadIdx.x; c < start(part + 1); c += kThreads) {
-      const vec_t<T, K> x = row.load(c, none);
-#pragma unroll
-      for (int k = 0; k < K; ++k) mine += amount((float)x[k], 0);
-    }
-    mine = block_sum(mine, s.sh);
-    if (threadIdx.x == 0) s.units[part] = mine;
-    total += mine;
-  }
+  if (!nucleus && threadIdx.x < kParts) s.units[threadIdx.x] = sums[threadIdx.x * kSums + kBuckets + 1];
   __syncthreads();
+  unsigned long long total = 0;
+  for (int part = 0; part < kParts; ++part) total += s.units[part];
   unsigned long long at = draw_target(q.u, total);
   int part = 0;
   while (part < kParts - 1 && at > s.units[part]) at -= s.units[part++];
-  find_class(row, start(part), start(part + 1), at, s.sh, amount,
+  const Part span(row.count, part);
+  find_class(row, span.first, span.last, at, s.sh,
+             [&](float x, int64_t j) -> unsigned long long {
+               const double w = weight.scaled(x);
+               bool kept = w >= weight.least;
+               if (nucleus) {
+                 const int b = buckets.of(x);
+                 kept = b < border || (b == border && ((unsigned long long)key_of(x) << a.index_bits | (unsigned long long)j) <= last);
+               }
+               return kept ? weight.units(w) : 0;
+             },
              [&](float x, int64_t j) { write_token(a, r, (uint32_t)j, x, weight, q.t, total); });
   return true;
 }
 
-template <class T, bool TOPS>
+template <class T>
 __global__ void __launch_bounds__(kThreads, 4) k_sample_list(SampleArgs a) {
   constexpr int K = 16 / sizeof(T);
   __shared__ ListShared s;
@@ -598,25 +631,11 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample_list(SampleArgs a) {
     const int groups = (int)((small + size - 1) / size);  // of `size` times kGroup granules
     // the groups' largest logits, and the row's
     float top = -INFINITY;
-    if (TOPS) {
-      for (int g = threadIdx.x; g < groups; g += kThreads) {
-        float m = -INFINITY;
-        for (int64_t i = g * size; i < (g + 1) * size && i < small; ++i) m = fmaxf(m, a.tops[r * a.groups + i]);
-        s.tops[g] = m;
-        top = fmaxf(top, m);
-      }
-    } else {
-      for (int64_t c = threadIdx.x; c < (int64_t)groups * kGroup; c += kThreads) {
-        float m = -INFINITY;
-        if (c < row.count) {
-          const vec_t<T, K> x = row.load(c, none);
-#pragma unroll
-          for (int k = 0; k < K; ++k) m = fmaxf(m, (float)x[k]);
-        }
-        for (int off = 1; off < kGroup; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-        if (c % kGroup == 0) s.tops[c / kGroup] = m;
-        top = fmaxf(top, m);
-      }
+    for (int g = threadIdx.x; g < groups; g += kThreads) {
+      float m = -INFINITY;
+      for (int64_t i = g * size; i < (g + 1) * size && i < small; ++i) m = fmaxf(m, a.tops[r * a.groups + i]);
+      s.tops[g] = m;
+      top = fmaxf(top, m);
     }
     if (threadIdx.x == 0) s.count = s.nhits = 0;
     top = logit_of((uint32_t)block_min(key_of(top), s.sh));
@@ -696,105 +715,63 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample_list(SampleArgs a) {
   }
 }
 
-// FIRST: no kernel before it has drawn rows
-template <class T, bool TOPS, bool FIRST>
-__global__ void __launch_bounds__(kThreads, 4) k_sample_parts(SampleArgs a) {
-  __shared__ PartsShared s;
-  for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    if (!FIRST && a.token[r] != kLeft) continue;
-    __syncthreads();
-    const T *logits = static_cast<const T *>(a.logits) + r * a.stride;
-    const Params q = params_of(a, r);
-    if (q.k > 0) continue;
-    const float top = row_top<T, TOPS>(a, r, Chunks<T>(logits, (int64_t)a.cols), s.sh);
-    if (top == -INFINITY) {
-      write_none(a, r);
-      continue;
-    }
-    if (is_greedy(q)) {
-      const Chunks<T> row(logits, (int64_t)a.cols);
-      unsigned long long first = ~0ull;
-      for (int64_t c = threadIdx.x; c < row.count; c += kThreads) {
-        const vec_t<T, 16 / sizeof(T)> x = row.load(c, (T)-INFINITY);
+template <class T>
+__global__ void __launch_bounds__(kThreads) k_sample_rest(SampleArgs a, uint64_t r0, uint64_t r1) {
+  __shared__ RestShared s;
+  const uint64_t r = r0 + blockIdx.x;
+  if (r >= r1 || (a.top_k && a.token[r] != kLeft)) return;
+  const Params q = params_of(a, r);
+  const float top = row_top<kThreads>(a, r, s.sh);
+  if (top == -INFINITY) {
+    write_none(a, r);
+    return;
+  }
+  const Weights weight(top, q.t, q.m, a.shift);
+  __syncthreads();
+  if (by_sums(q, top) && draw_sums<T>(a, r, a.sums + blockIdx.x * (uint64_t)(kParts * kSums), q, weight, s)) return;
+  __syncthreads();
+  const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int64_t)a.cols);
+  unsigned long long first = ~0ull;  // the lowest index of the largest logit
+  for (int64_t c = threadIdx.x; c < row.count && first == ~0ull; c += kThreads) {
+    const vec_t<T, 16 / sizeof(T)> x = row.load(c, (T)-INFINITY);
 #pragma unroll
-        for (int k = 16 / sizeof(T) - 1; k >= 0; --k)
-          if ((float)x[k] == top) first = (unsigned long long)(c * (int64_t)(16 / sizeof(T)) + k - row.lead);
-        if (first != ~0ull) break;
-      }
-      first = block_min(first, s.sh);
-      if (threadIdx.x == 0) {
-        a.token[r] = (int32_t)first;
-        if (a.logprob) a.logprob[r] = 0.0f;
-      }
-      continue;
-    }
-    const bool done = q.u > 0.0f && top < INFINITY &&
-                      draw_parts(a, r, q, Chunks<T, 8>(logits, (int64_t)a.cols), Weights(top, q.t, q.m, a.shift), s);
-    if (!done && threadIdx.x == 0) a.token[r] = kLeft;
+    for (int k = 16 / sizeof(T) - 1; k >= 0; --k)
+      if ((float)x[k] == top) first = (unsigned long long)(c * (int64_t)(16 / sizeof(T)) + k - row.lead);
   }
-}
-
-template <class T, bool TOPS>
-__global__ void __launch_bounds__(kThreads) k_sample_any(SampleArgs a) {
-  __shared__ Shared sh;
-  for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    if (a.token[r] != kLeft) continue;
-    __syncthreads();
-    const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int64_t)a.cols);
-    const Params q = params_of(a, r);
-    const float top = row_top<T, TOPS>(a, r, row, sh);
-    const RowSource<T> source{row.base + row.lead, row.cols};
-    unsigned long long first = ~0ull;
-    source.each([&](float x, uint32_t j) {
-      const unsigned long long o = (unsigned long long)key_of(x) << a.index_bits | j;
-      first = o < first ? o : first;
-    });
-    first = block_min(first, sh);
-    if (is_greedy(q)) {
-      if (threadIdx.x == 0) {
-        a.token[r] = (int32_t)(first & ((1ull << a.index_bits) - 1));
-        if (a.logprob) a.logprob[r] = 0.0f;
-      }
-    } else {
-      draw_row(a, r, q, Weights(top, q.t, q.m, a.shift), first, source, sh);
+  first = block_min(first, s.sh);
+  if (is_greedy(q)) {
+    if (threadIdx.x == 0) {
+      a.token[r] = (int32_t)first;
+      if (a.logprob) a.logprob[r] = 0.0f;
     }
+    return;
   }
+  draw_row(a, r, q, weight, (unsigned long long)key_of(top) << a.index_bits | first, RowSource<T>{row.base + row.lead, row.cols}, s.sh);
 }
-
-// From this many columns on the largest logits of the groups come from a launch of their own; below, the row's workgroup has
-// read the row before a second launch could begin.
-constexpr uint64_t kTopsFrom = 16384;
 
 static uint64_t tops_groups(uint64_t cols, uint64_t per) { return ((cols + per - 1) / per + 1 + kGroup - 1) / kGroup; }
 
+static uint64_t tops_bytes(uint64_t rows, uint64_t groups) { return round_up(rows * groups * sizeof(float), 256); }
+
 template <class T>
-static int sample(admm_ctx *ctx, SampleArgs a) {
+static int sample(admm_ctx *ctx, SampleArgs a, void *workspace) {
   a.groups = (int64_t)tops_groups(a.cols, 16 / sizeof(T));
-  const dim3 grid(blocks_for(a.rows, 1)), block(kThreads);
-  if (a.cols <= kTopsFrom) {
-    if (a.top_k) {
-      hipLaunchKernelGGL((k_sample_list<T, false>), grid, block, 0, ctx->stream, a);
-      hipLaunchKernelGGL((k_sample_parts<T, false, false>), grid, block, 0, ctx->stream, a);
-    } else {
-      hipLaunchKernelGGL((k_sample_parts<T, false, true>), grid, block, 0, ctx->stream, a);
-    }
-    hipLaunchKernelGGL((k_sample_any<T, false>), grid, block, 0, ctx->stream, a);
-  } else {
-    const unsigned per_row = (unsigned)((a.groups * kGroup + kTopsPer - 1) / kTopsPer);
-    for (uint64_t r = 0; r < a.rows; r += 65535) {  // rows are the second dimension of the grid
-      SampleArgs b = a;
-      b.logits = static_cast<const T *>(a.logits) + r * a.stride;
-      b.tops = a.tops + r * a.groups;
-      const unsigned rows = (unsigned)(a.rows - r < 65535 ? a.rows - r : 65535);
-      hipLaunchKernelGGL(k_sample_tops<T>, dim3(per_row, rows), dim3(256), 0, ctx->stream, b);
-    }
-    if (a.top_k) {
-      hipLaunchKernelGGL((k_sample_list<T, true>), grid, block, 0, ctx->stream, a);
-      hipLaunchKernelGGL((k_sample_parts<T, true, false>), grid, block, 0, ctx->stream, a);
-    } else {
-      hipLaunchKernelGGL((k_sample_parts<T, true, true>), grid, block, 0, ctx->stream, a);
-    }
-    hipLaunchKernelGGL((k_sample_any<T, true>), grid, block, 0, ctx->stream, a);
+  a.tops = static_cast<float *>(workspace);
+  a.sums = reinterpret_cast<unsigned long long *>(static_cast<char *>(workspace) + tops_bytes(a.rows, a.groups));
+  const dim3 block(kThreads);
+  const unsigned per_row = (unsigned)((a.groups * kGroup + kTopsPer - 1) / kTopsPer);
+  for (uint64_t r = 0; r < a.rows; r += 65535) {  // rows are the second dimension of the grid
+    SampleArgs b = a;
+    b.logits = static_cast<const T *>(a.logits) + r * a.stride;
+    b.tops = a.tops + r * a.groups;
+    const unsigned rows = (unsigned)(a.rows - r < 65535 ? a.rows - r : 65535);
+    hipLaunchKernelGGL(k_sample_tops<T>, dim3(per_row, rows), dim3(256), 0, ctx->stream, b);
+  }
+  if (a.top_k) hipLaunchKernelGGL(k_sample_list<T>, dim3(blocks_for(a.rows, 1)), block, 0, ctx->stream, a);
+  for (uint64_t r = 0; r < a.rows; r += kBatch) {
+    const uint64_t end = r + kBatch < a.rows ? r + kBatch : a.rows;
+    hipLaunchKernelGGL(k_sample_sums<T>, dim3(kParts, (unsigned)(end - r)), dim3(256), 0, ctx->stream, a, r);
+    hipLaunchKernelGGL(k_sample_rest<T>, dim3((unsigned)(end - r)), block, 0, ctx->stream, a, r, end);
   }
   ADMM_HIP_CHECK(hipGetLastError());
   return ADMM_OK;
@@ -808,7 +785,8 @@ extern "C" int admm_sample_workspace(uint64_t rows, uint64_t cols, uint64_t *byt
   ADMM_REQUIRE(bytes, "admm_sample_workspace: bytes is NULL");
   ADMM_REQUIRE(rows < (1ull << 40) && cols < (1ull << 31), "admm_sample_workspace: %llu x %llu logits", (unsigned long long)rows,
                (unsigned long long)cols);
-  *bytes = cols > kTopsFrom ? round_up(rows * tops_groups(cols, 4), 64) * 4 : 0;  // of the narrowest granules
+  // enough for logits of any type: granules of four floats are the most
+  *bytes = tops_bytes(rows, tops_groups(cols, 4)) + (rows < kBatch ? rows : kBatch) * (kParts * kSums * sizeof(unsigned long long));
   return ADMM_OK;
 }
 
@@ -843,6 +821,5 @@ extern "C" int admm_sample(admm_ctx *ctx, const admm_mat *logits, const admm_sam
   a.index_bits = 1;
   while ((1ull << a.index_bits) < a.cols) ++a.index_bits;
   a.shift = 62 - a.index_bits < 51 ? 62 - a.index_bits : 51;
-  a.tops = static_cast<float *>(workspace);
-  return logits->type == ADMM_F32 ? sample<float>(ctx, a) : logits->type == ADMM_BF16 ? sample<bf16_t>(ctx, a) : sample<f16_t>(ctx, a);
+  return logits->type == ADMM_F32 ? sample<float>(ctx, a, workspace) : logits->type == ADMM_BF16 ? sample<bf16_t>(ctx, a, workspace) : sample<f16_t>(ctx, a, workspace);
 }
