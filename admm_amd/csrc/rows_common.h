@@ -48,39 +48,44 @@ template <class T, int BYTES = 16>
 struct Chunks {
   static constexpr int kPer = BYTES / sizeof(T);
   const T *base;  // on BYTES bytes; the row begins `lead` elements after it
-  int64_t lead, cols, count;
-  __device__ Chunks(const T *row, int64_t n) {
-    lead = (int64_t)((reinterpret_cast<uintptr_t>(row) & (BYTES - 1)) / sizeof(T));
+  int lead, cols, count;
+  int whole_from, whole_to;  // chunks that lie in the row altogether
+  __device__ Chunks(const T *row, int n) {
+    lead = (int)((reinterpret_cast<uintptr_t>(row) & (BYTES - 1)) / sizeof(T));
     base = row - lead;
     cols = n;
-    count = (lead + n + kPer - 1) / kPer;
+    count = (int)(((unsigned)lead + (unsigned)n + kPer - 1) / kPer);
+    whole_from = lead ? 1 : 0;
+    whole_to = (int)(((unsigned)lead + (unsigned)n) / kPer);
   }
-  __device__ bool whole(int64_t c) const { return c * kPer >= lead && (c + 1) * kPer <= lead + cols; }
-  __device__ vec_t<T, kPer> load(int64_t c, T other) const {
-    if (whole(c)) return *reinterpret_cast<const vec_t<T, kPer> *>(base + c * kPer);
+  __device__ int column(int c, int k) const { return c * kPer + k - lead; }
+  __device__ vec_t<T, kPer> load(int c, T other) const {
+    if (c >= whole_from && c < whole_to) return *reinterpret_cast<const vec_t<T, kPer> *>(base + (int64_t)c * kPer);
     vec_t<T, kPer> x;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      const int64_t j = c * kPer + k - lead;
+      const int j = column(c, k);
       x[k] = other;
-      if (j >= 0 && j < cols) x[k] = base[c * kPer + k];
+      if (j >= 0 && j < cols) x[k] = base[(int64_t)c * kPer + k];
     }
     return x;
   }
   // to another row; `apart`: of another alignment
-  __device__ void store(T *row, bool apart, int64_t c, vec_t<T, kPer> x) const {
+  __device__ void store(T *row, bool apart, int c, vec_t<T, kPer> x) const {
     T *to = row - lead;
-    if (!apart && whole(c)) {
-      *reinterpret_cast<vec_t<T, kPer> *>(to + c * kPer) = x;
+    if (!apart && c >= whole_from && c < whole_to) {
+      *reinterpret_cast<vec_t<T, kPer> *>(to + (int64_t)c * kPer) = x;
       return;
     }
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      const int64_t j = c * kPer + k - lead;
-      if (j >= 0 && j < cols) to[c * kPer + k] = x[k];
+      const int j = column(c, k);
+      if (j >= 0 && j < cols) to[(int64_t)c * kPer + k] = x[k];
     }
   }
 };
+
+constexpr uint64_t kMaxClasses = 0x7FFFFF00;  // chunks and columns of a row of logits are counted in ints
 
 // ---- host side ----------------------------------------------------------------------------------
 

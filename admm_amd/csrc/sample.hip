@@ -13,7 +13,8 @@
 namespace admm_impl {
 
 constexpr int kThreads = 512;
-constexpr int kDigit = 8;
+constexpr int kDigit = 9;  // a value of the digit for every thread
+static_assert(1 << kDigit == kThreads, "");
 
 struct SampleArgs {
   const void *logits;
@@ -38,6 +39,14 @@ __device__ inline float logit_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key : ~key & 0x7FFFFFFFu);
 }
 
+// p f + c.  The compiler's own choice for a polynomial is the form that adds to its third operand in place, with a copy of
+// the coefficient before every step: a tenth of k_sample_sums.
+__device__ inline double fma3(double p, double f, double c) {
+  double d;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(p), "v"(f), "v"(c));
+  return d;
+}
+
 struct Weights {
   float top;      // the row's largest logit
   double per;     // L / T
@@ -47,25 +56,27 @@ struct Weights {
     per = fmax(1.44269504088896340736 / (double)t, 1e-300);  // not 0 at an infinite temperature: -inf stays -inf
     least = min_p > 0.0f ? ldexp((double)min_p, shift) : 0.0;
   }
-  // 2^S times the weight of a class: 2^(n + S) times a polynomial of the rest of the exponent (|f ln 2| <= 0.35: the series'
-  // term of degree 11 is 2e-13, where the draw of a flat row of 2^17 classes sees 8e-6 a class).  0 for -inf and NaN; a top of
-  // +inf is not meant here.
-  __device__ double scaled(float x) const {
-    const double y = fmax(((double)x - (double)top) * per, -1100.0);
-    const double n = rint(y), f = y - n;
-    double p = 7.054911620801121e-09;  // ln(2)^k / k!
-    p = fma(p, f, 1.0178086009239699e-07);
-    p = fma(p, f, 1.3215486790144307e-06);
-    p = fma(p, f, 1.525273380405984e-05);
-    p = fma(p, f, 0.0001540353039338161);
-    p = fma(p, f, 0.0013333558146428443);
-    p = fma(p, f, 0.009618129107628477);
-    p = fma(p, f, 0.05550410866482158);
-    p = fma(p, f, 0.2402265069591007);
-    p = fma(p, f, 0.6931471805599453);
-    p = fma(p, f, 1.0);
-    return ldexp(p, (int)n + shift);
+  // The exponent of a class' weight, at least -64 (less than half a unit for every S); NaN counts as -inf.  A top of +inf is
+  // not meant here.
+  __device__ double exponent(float x) const { return fmax(((double)x - (double)top) * per, -64.0); }
+  // 2^(y + S): the integer part n of y is what is left in the low bits of y + 1.5 2^52 and goes to the exponent of 2^S times a
+  // polynomial of the rest.  That is 1 + f q(f), q through the Chebyshev points of (2^f - 1) / f on [-1/2, 1/2]: off by
+  // 2.2e-12 of the weight at most (the draw from a flat row of 2^17 classes sees 8e-6 a class), and 1 where f is 0.
+  __device__ double scaled(double y) const {
+    const double t = y + 0x1.8p52, f = y - (t - 0x1.8p52);
+    double p = 1.325080551750225e-06;
+    p = fma3(p, f, 1.5303700711365693e-05);
+    p = fma3(p, f, 0.00015403475186530786);
+    p = fma3(p, f, 0.0013333478473685416);
+    p = fma3(p, f, 0.00961812913523614);
+    p = fma3(p, f, 0.055504109063258665);
+    p = fma3(p, f, 0.24022650695888503);
+    p = fma3(p, f, 0.6931471805568324);
+    p = fma3(p, f, 1.0);
+    const int n = (int)(unsigned)__double_as_longlong(t);
+    return __hiloint2double(__double2hiint(p) + ((n + shift) << 20), __double2loint(p));
   }
+  __device__ double scaled(float x) const { return scaled(exponent(x)); }
   // rounded to an integer below 2^52: what is left in the mantissa after 2^52 is added
   __device__ static unsigned long long units(double v) { return __double_as_longlong(v + 0x1p52) & 0xFFFFFFFFFFFFFull; }
 };
@@ -74,7 +85,7 @@ struct Weights {
 template <class T>
 struct RowSource {
   const T *row;
-  int64_t cols;
+  int cols;
   template <class F>
   __device__ void each(F f) const {
 #pragma unroll 1
@@ -84,7 +95,7 @@ struct RowSource {
 
 struct Shared {
   unsigned long long hist[1 << kDigit];
-  unsigned long long sums[kThreads / 64];
+  unsigned long long sums[kThreads / 64], tops[kThreads / 64];
   unsigned long long found, before;
 };
 
@@ -115,51 +126,101 @@ __device__ inline unsigned long long block_min(unsigned long long v, Shared &sh)
   return v;
 }
 
+// Sums over sh.hist up to and with every thread's value: where they reach `target` goes to sh.found (else all ones), what comes
+// before it to sh.before; everybody waits.  Returns the sum of all.
+__device__ inline unsigned long long find_value(Shared &sh, unsigned long long v, unsigned long long target) {
+  unsigned long long up = v;
+  for (int off = 1; off < 64; off <<= 1) {
+    const unsigned long long y = __shfl_up(up, off, 64);
+    if ((int)(threadIdx.x & 63) >= off) up += y;
+  }
+  if (threadIdx.x == 0) sh.found = ~0ull;
+  if ((threadIdx.x & 63) == 63) sh.sums[threadIdx.x >> 6] = up;
+  __syncthreads();
+  unsigned long long all = 0;
+#pragma unroll
+  for (int i = 0; i < kThreads / 64; ++i) {
+    if (i == (int)(threadIdx.x >> 6)) up += all;
+    all += sh.sums[i];
+  }
+  if (up - v < target && target <= up) {
+    sh.found = threadIdx.x;
+    sh.before = up - v;
+  }
+  __syncthreads();
+  return all;
+}
+
 // The key of `bits` bits of the first class, in ascending order of the keys, at which the amounts add up to `target` (>= 1);
 // all ones where they never do.  visit(f) calls f(key, amount) for this thread's classes.
 template <class Visit>
 __device__ inline unsigned long long select_key(int bits, unsigned long long target, Shared &sh, Visit visit) {
   unsigned long long prefix = 0;
-  const unsigned long long all = bits >= 64 ? ~0ull : (1ull << bits) - 1;
   for (int top = bits; top > 0;) {
     const int width = top < kDigit ? top : kDigit, low = top - width;
     __syncthreads();
-    for (int i = threadIdx.x; i < 1 << kDigit; i += kThreads) sh.hist[i] = 0;
-    if (threadIdx.x == 0) sh.found = ~0ull;
+    sh.hist[threadIdx.x] = 0;
     __syncthreads();
     visit([&](unsigned long long key, unsigned long long amount) {
       if (amount && (top >= 64 || key >> top == prefix)) atomicAdd(&sh.hist[(key >> low) & ((1u << width) - 1)], amount);
     });
     __syncthreads();
-    if (threadIdx.x < 64) {  // 4 values a lane
-      unsigned long long x[4], s = 0;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        x[k] = sh.hist[threadIdx.x * 4 + k];
-        s += x[k];
-      }
-      unsigned long long up = s;
-      for (int off = 1; off < 64; off <<= 1) {
-        const unsigned long long y = __shfl_up(up, off, 64);
-        if ((int)threadIdx.x >= off) up += y;
-      }
-      up -= s;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (up < target && target <= up + x[k]) {
-          sh.found = threadIdx.x * 4 + k;
-          sh.before = up;
-        }
-        up += x[k];
-      }
-    }
-    __syncthreads();
-    if (sh.found == ~0ull) return all;
+    find_value(sh, sh.hist[threadIdx.x], target);
+    if (sh.found == ~0ull) return ~0ull;
     prefix = prefix << width | sh.found;
     target -= sh.before;
     top = low;
   }
   return prefix;
+}
+
+// The same among classes that the threads hold, kHeld each, with keys that differ; an amount of 0: not among them.  The range
+// of the keys that are left is cut into 512 until there is one.
+constexpr int kHeld = 4;
+__device__ inline unsigned long long select_held(const unsigned long long (&key)[kHeld], const unsigned long long (&amount)[kHeld],
+                                                 unsigned long long target, Shared &sh) {
+  bool on[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) on[i] = amount[i] != 0;
+  for (;;) {
+    unsigned long long lo = ~0ull, hi = 0;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      if (on[i] && key[i] < lo) lo = key[i];
+      if (on[i] && key[i] > hi) hi = key[i];
+    }
+    for (int off = 1; off < 64; off <<= 1) {
+      const unsigned long long l = __shfl_xor(lo, off, 64), h = __shfl_xor(hi, off, 64);
+      lo = l < lo ? l : lo;
+      hi = h > hi ? h : hi;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+      sh.sums[threadIdx.x >> 6] = lo;
+      sh.tops[threadIdx.x >> 6] = hi;
+    }
+    sh.hist[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) {
+      lo = sh.sums[i] < lo ? sh.sums[i] : lo;
+      hi = sh.tops[i] > hi ? sh.tops[i] : hi;
+    }
+    if (lo >= hi) return lo;  // one, or none: all ones
+    const int bits = 64 - __clzll((long long)(lo ^ hi)), shift = bits > kDigit ? bits - kDigit : 0;
+    const unsigned long long from = lo >> shift;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (on[i]) atomicAdd(&sh.hist[(key[i] >> shift) - from], amount[i]);
+    __syncthreads();
+    find_value(sh, sh.hist[threadIdx.x], target);
+    if (sh.found == ~0ull) return ~0ull;
+    target -= sh.before;
+    const unsigned long long at = from + sh.found;
+    if (shift == 0) return at;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) on[i] = on[i] && key[i] >> shift == at;
+  }
 }
 
 struct Params {
@@ -223,8 +284,8 @@ __device__ inline void draw_row(const SampleArgs &a, uint64_t r, const Params &q
     token = ~0ull;
     source.each([&](float x, uint32_t j) {
       const unsigned long long o = order(x, j);
-      const double w = scaled(x);
-      if (o <= last && w > 0.0 && (w >= weight.least || o == first) && j < token) token = j;
+      const bool any = x == weight.top || ((double)x - (double)weight.top) * weight.per > -1075.0;
+      if (o <= last && any && (scaled(x) >= weight.least || o == first) && j < token) token = j;
     });
     token = block_min(token, sh);
   }
@@ -252,8 +313,8 @@ __device__ inline void draw_row(const SampleArgs &a, uint64_t r, const Params &q
 constexpr int kGroup = 32;       // granules
 constexpr int kTopsPer = 512;    // granules per workgroup of k_sample_tops
 constexpr int kMaxGroups = 4096; // groups whose largest logits fit LDS beside the rest
-constexpr int kList = 2048;      // classes kept in LDS
-constexpr int kPairs = 512;      // of which all pairs are compared, not sorted digit by digit
+constexpr int kList = kHeld * kThreads;  // classes kept in LDS
+constexpr int kPairs = 128;      // up to so many all pairs are compared: 3 us for the filters and the draw, where selecting takes 12
 constexpr int kBuckets = 512, kParts = 8;
 constexpr int kSums = kBuckets + 2;   // the buckets of a part, what is below them, what passes min-p
 constexpr uint64_t kBatch = 1024;     // rows whose sums the workspace holds at once
@@ -262,7 +323,7 @@ constexpr int32_t kLeft = -2;
 struct ListShared {
   float tops[kMaxGroups];
   unsigned int hits[kMaxGroups];
-  unsigned long long list[kPairs];   // keys of draw_row's order
+  unsigned long long list[kList];    // keys of draw_row's order
   unsigned long long units[kPairs];  // their weights
   Shared sh;
   unsigned int count, nhits, bound;
@@ -270,7 +331,7 @@ struct ListShared {
 
 struct RestShared {
   unsigned long long hist[kParts][kBuckets];
-  unsigned long long list[kList], units[kPairs];
+  unsigned long long list[kList], units[kParts];
   Shared sh;
   unsigned int count;
 };
@@ -296,15 +357,16 @@ __device__ inline float row_top(const SampleArgs &a, uint64_t r, Shared &sh) {
   return logit_of((uint32_t)block_min<NT>(key_of(top), sh));
 }
 
-// Buckets of equal width in the logit, for top-p: down to weights of (1 - p) / cols, and one power of two more for the
-// roundings; kBuckets and beyond: below them.
+// Buckets of equal width in the weight's exponent, for top-p: down to weights of (1 - p) / cols, and one power of two more for
+// the roundings; kBuckets and beyond: below them.
 struct Buckets {
-  float top, scale;
-  __device__ Buckets(const Params &q, const Weights &w, uint64_t cols) : top(w.top) {
+  double per;
+  __device__ Buckets(const Params &q, uint64_t cols) {
     const double depth = log2((double)cols / (1.0 - (double)q.p)) + 1.0;
-    scale = fminf((float)(w.per * kBuckets / (depth > 1.0 ? depth : 1.0)), 0x1p100f);  // 0 times infinity would be no bucket
+    per = -kBuckets / (depth > 1.0 ? depth : 1.0);
   }
-  __device__ int of(float x) const { return (int)fminf((top - x) * scale, (float)kBuckets); }
+  // y in [-64, 0]: the rounded product is what is left in the low bits after 2^52 is added
+  __device__ unsigned of(double y) const { return (unsigned)__double_as_longlong(fma(y, per, 0x1p52)); }
 };
 
 // is a row of this kind drawn by its sums?
@@ -313,8 +375,8 @@ __device__ inline bool by_sums(const Params &q, float top) { return q.k == 0 && 
 template <class T>
 __global__ void __launch_bounds__(256) k_sample_tops(SampleArgs a) {
   constexpr int K = 16 / sizeof(T);
-  const Chunks<T> row(static_cast<const T *>(a.logits) + (uint64_t)blockIdx.y * a.stride, (int64_t)a.cols);
-  const int64_t c0 = (int64_t)blockIdx.x * kTopsPer + threadIdx.x;
+  const Chunks<T> row(static_cast<const T *>(a.logits) + (uint64_t)blockIdx.y * a.stride, (int)a.cols);
+  const int c0 = (int)(blockIdx.x * kTopsPer + threadIdx.x);
   vec_t<T, K> x[kTopsPer / 256];
 #pragma unroll
   for (int i = 0; i < kTopsPer / 256; ++i) {
@@ -327,20 +389,10 @@ __global__ void __launch_bounds__(256) k_sample_tops(SampleArgs a) {
 #pragma unroll
     for (int k = 0; k < K; ++k) m = fmaxf(m, (float)x[i][k]);
     for (int off = 1; off < kGroup; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-    const int64_t g = (c0 + i * 256) / kGroup;
+    const int g = (c0 + i * 256) / kGroup;
     if (threadIdx.x % kGroup == 0 && g < a.groups) a.tops[(uint64_t)blockIdx.y * a.groups + g] = m;
   }
 }
-
-// the classes in the list, each of them to one thread
-struct ListSource {
-  const unsigned long long *list;
-  int count, index_bits;
-  template <class F>
-  __device__ void each(F f) const {
-    for (int i = threadIdx.x; i < count; i += kThreads) f(logit_of((uint32_t)(list[i] >> index_bits)), (uint32_t)(list[i] & ((1ull << index_bits) - 1)));
-  }
-};
 
 // sum of `v` over the `each` threads that share a class
 template <class V>
@@ -385,41 +437,81 @@ __device__ inline void draw_pairs(const SampleArgs &a, uint64_t r, const Params 
   if (kept && part == 0 && (o & mask) == token) write_token(a, r, (uint32_t)token, x, weight, q.t, total);
 }
 
+// what a thread holds of a list
+struct Held {
+  unsigned long long o[kHeld], units[kHeld];
+  double w[kHeld];
+  __device__ Held(const unsigned long long *list, int count, const Weights &weight, int index_bits) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int at = threadIdx.x + i * kThreads;
+      o[i] = at < count ? list[at] : ~0ull;
+      w[i] = at < count ? weight.scaled(logit_of((uint32_t)(o[i] >> index_bits))) : 0.0;
+      units[i] = Weights::units(w[i]);
+    }
+  }
+};
+
+// All filters and the draw among up to kList classes.
+__device__ inline void draw_held(const SampleArgs &a, uint64_t r, const Params &q, const Weights &weight, unsigned long long first,
+                                 const unsigned long long *list, int count, Shared &sh) {
+  Held h(list, count, weight, a.index_bits);
+  unsigned long long amount[kHeld], last = ~0ull;
+  if (q.k > 0) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) amount[i] = (int)threadIdx.x + i * kThreads < count ? 1 : 0;
+    last = select_held(h.o, amount, (unsigned long long)q.k, sh);
+  }
+  if (q.p < 1.0f) {
+    unsigned long long mass = 0;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      amount[i] = h.o[i] <= last ? h.units[i] : 0;
+      mass += amount[i];
+    }
+    mass = block_sum(mass, sh);
+    const unsigned long long end = select_held(h.o, amount, mass_target(q.p, mass), sh);
+    last = end < last ? end : last;
+  }
+  unsigned long long total = 0, index[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    amount[i] = h.o[i] <= last && (h.w[i] >= weight.least || h.o[i] == first) ? h.units[i] : 0;
+    total += amount[i];
+    index[i] = h.o[i] & ((1ull << a.index_bits) - 1);
+  }
+  total = block_sum(total, sh);
+  const unsigned long long token = select_held(index, amount, draw_target(q.u, total), sh);
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (amount[i] && index[i] == token) write_token(a, r, (uint32_t)token, logit_of((uint32_t)(h.o[i] >> a.index_bits)), weight, q.t, total);
+}
+
 // The first class, in the order of the indexes, at which the amounts of the granules [c0, c1) reach `target`; visit(x, j) is
 // a class's amount, hit(x, j) gets the class.
 template <class T, class Amount, class Hit>
-__device__ inline void find_class(const Chunks<T, 8> &row, int64_t c0, int64_t c1, unsigned long long target, Shared &sh, Amount amount, Hit hit) {
+__device__ inline void find_class(const Chunks<T, 8> &row, int c0, int c1, unsigned long long target, Shared &sh, Amount amount, Hit hit) {
   constexpr int K = 8 / sizeof(T);
-#pragma unroll 1
-  for (int64_t b = c0; b < c1; b += kThreads) {
-    const int64_t c = b + threadIdx.x;
+  for (int b = c0; b < c1; b += kThreads) {
+    const int c = b + (int)threadIdx.x;
     vec_t<T, K> x = (T)-INFINITY;
     if (c < c1) x = row.load(c, (T)-INFINITY);
     unsigned long long u[K], mine = 0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      u[k] = amount((float)x[k], c * K + k - row.lead);
+      u[k] = amount((float)x[k], row.column(c, k));
       mine += u[k];
     }
-    unsigned long long up = mine;
-    for (int off = 1; off < 64; off <<= 1) {
-      const unsigned long long y = __shfl_up(up, off, 64);
-      if ((int)(threadIdx.x & 63) >= off) up += y;
-    }
     __syncthreads();
-    if ((threadIdx.x & 63) == 63) sh.sums[threadIdx.x >> 6] = up;
-    __syncthreads();
-    unsigned long long all = 0;
-    for (int i = 0; i < kThreads / 64; ++i) {
-      if (i == (int)(threadIdx.x >> 6)) up += all;
-      all += sh.sums[i];
-    }
+    const unsigned long long all = find_value(sh, mine, target);
     if (all >= target) {  // uniform
-      unsigned long long sum = up - mine;
+      if (sh.found == threadIdx.x) {
+        unsigned long long sum = sh.before;
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (sum < target && target <= sum + u[k]) hit((float)x[k], c * K + k - row.lead);
-        sum += u[k];
+        for (int k = 0; k < K; ++k) {
+          if (sum < target && target <= sum + u[k]) hit((float)x[k], row.column(c, k));
+          sum += u[k];
+        }
       }
       return;
     }
@@ -429,9 +521,9 @@ __device__ inline void find_class(const Chunks<T, 8> &row, int64_t c0, int64_t c
 
 // granules of a part of a row
 struct Part {
-  int64_t first, last;
-  __device__ Part(int64_t count, int part) {
-    const int64_t span = (count + kParts - 1) / kParts;
+  int first, last;
+  __device__ Part(int count, int part) {
+    const int span = (count + kParts - 1) / kParts;
     first = part * span < count ? part * span : count;
     last = first + span < count ? first + span : count;
   }
@@ -448,44 +540,45 @@ __global__ void __launch_bounds__(256) k_sample_sums(SampleArgs a, uint64_t r0) 
   const float top = row_top<256>(a, r, sh);
   if (!by_sums(q, top)) return;
   const Weights weight(top, q.t, q.m, a.shift);
-  const Chunks<T, 8> row(static_cast<const T *>(a.logits) + r * a.stride, (int64_t)a.cols);
+  const Chunks<T, 8> row(static_cast<const T *>(a.logits) + r * a.stride, (int)a.cols);
   const Part part(row.count, (int)blockIdx.x);
   const T none = (T)-INFINITY;
   unsigned long long *to = a.sums + (blockIdx.y * kParts + blockIdx.x) * (uint64_t)kSums;
   unsigned long long rest = 0, above = 0;  // below the buckets; passing min-p
-  if (q.p < 1.0f) {
-    const Buckets buckets(q, weight, a.cols);
-    for (int i = threadIdx.x; i < kBuckets; i += 256) hist[i] = 0;
-    __syncthreads();
-    for (int64_t c = part.first + threadIdx.x; c < part.last; c += 256) {
+  auto each = [&](auto f) {
+    for (int c = part.first + (int)threadIdx.x; c < part.last; c += 256) {
       const vec_t<T, K> x = row.load(c, none);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const double w = weight.scaled((float)x[k]);
-        const unsigned long long u = weight.units(w);
-        const int b = buckets.of((float)x[k]);
-        if (b < kBuckets) atomicAdd(&hist[b], u);
-        else rest += u;
-        if (q.m > 0.0f) above += w >= weight.least ? u : 0;
+        const double y = weight.exponent((float)x[k]), w = weight.scaled(y);
+        f(y, w, weight.units(w));
       }
+    }
+  };
+  if (q.p < 1.0f) {
+    const Buckets buckets(q, a.cols);
+    for (int i = threadIdx.x; i < kBuckets; i += 256) hist[i] = 0;
+    __syncthreads();
+    auto put = [&](double y, unsigned long long u) {
+      const unsigned b = buckets.of(y);
+      if (b < (unsigned)kBuckets) atomicAdd(&hist[b], u);
+      else rest += u;
+    };
+    if (q.m > 0.0f) {
+      each([&](double y, double w, unsigned long long u) {
+        put(y, u);
+        above += w >= weight.least ? u : 0;
+      });
+    } else {
+      each([&](double y, double, unsigned long long u) { put(y, u); });
     }
     __syncthreads();
     for (int i = threadIdx.x; i < kBuckets; i += 256) to[i] = hist[i];
     rest = block_sum<256>(rest, sh);
+  } else {
+    each([&](double, double w, unsigned long long u) { above += w >= weight.least ? u : 0; });
   }
-  if (q.p < 1.0f && q.m > 0.0f) {
-    above = block_sum<256>(above, sh);
-  } else if (!(q.p < 1.0f)) {
-    for (int64_t c = part.first + threadIdx.x; c < part.last; c += 256) {
-      const vec_t<T, K> x = row.load(c, none);
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const double w = weight.scaled((float)x[k]);
-        above += w >= weight.least ? weight.units(w) : 0;
-      }
-    }
-    above = block_sum<256>(above, sh);
-  }
+  above = block_sum<256>(above, sh);
   if (threadIdx.x == 0) {
     to[kBuckets] = rest;
     to[kBuckets + 1] = above;
@@ -495,10 +588,10 @@ __global__ void __launch_bounds__(256) k_sample_sums(SampleArgs a, uint64_t r0) 
 // A row with its parts' sums; false where its border's bucket holds too many classes.
 template <class T>
 __device__ inline bool draw_sums(const SampleArgs &a, uint64_t r, const unsigned long long *sums, const Params &q, const Weights &weight, RestShared &s) {
-  const Chunks<T, 8> row(static_cast<const T *>(a.logits) + r * a.stride, (int64_t)a.cols);
+  const Chunks<T, 8> row(static_cast<const T *>(a.logits) + r * a.stride, (int)a.cols);
   bool nucleus = q.p < 1.0f;
-  const Buckets buckets(q, weight, a.cols);
-  int border = 0;
+  const Buckets buckets(q, a.cols);
+  unsigned border = 0;
   unsigned long long last = 0;
   if (nucleus) {
     unsigned long long mine = 0, above = 0;
@@ -510,39 +603,23 @@ __device__ inline bool draw_sums(const SampleArgs &a, uint64_t r, const unsigned
       mine += v;
       above += sums[part * kSums + kBuckets + 1];
     }
-    unsigned long long up = mine;  // of the buckets up to this one
-    for (int off = 1; off < 64; off <<= 1) {
-      const unsigned long long y = __shfl_up(up, off, 64);
-      if ((int)(threadIdx.x & 63) >= off) up += y;
-    }
-    if (threadIdx.x == 0) {
-      s.count = 0;
-      s.sh.found = ~0ull;
-    }
-    if ((threadIdx.x & 63) == 63) s.sh.sums[threadIdx.x >> 6] = up;
-    __syncthreads();
-    unsigned long long total = 0;
-    for (int i = 0; i < kThreads / 64; ++i) {
-      if (i == (int)(threadIdx.x >> 6)) up += total;
-      total += s.sh.sums[i];
-    }
-    for (int part = 0; part < kParts; ++part) total += sums[part * kSums + kBuckets];
+    unsigned long long total = mine;
+    if (threadIdx.x < kParts) total += sums[threadIdx.x * kSums + kBuckets];
+    total = block_sum(total, s.sh);
     const unsigned long long target = mass_target(q.p, total);
     // where the target is beyond all that passes min-p, top-p keeps all of that and more
     nucleus = !(q.m > 0.0f && target > above);
     if (nucleus) {
-      if (up - mine < target && target <= up) {
-        s.sh.found = threadIdx.x;
-        s.sh.before = up - mine;
-      }
+      if (threadIdx.x == 0) s.count = 0;
       __syncthreads();
+      find_value(s.sh, mine, target);
       if (s.sh.found == ~0ull) return false;
-      border = (int)s.sh.found;
+      border = (unsigned)s.sh.found;
       const unsigned long long within = target - s.sh.before;
       // the classes of the bucket that the target falls into
-      const Chunks<T> wide(static_cast<const T *>(a.logits) + r * a.stride, (int64_t)a.cols);
+      const Chunks<T> wide(static_cast<const T *>(a.logits) + r * a.stride, (int)a.cols);
       constexpr int K = 16 / sizeof(T), kAhead = 4;
-      for (int64_t c0 = threadIdx.x; c0 < wide.count; c0 += kAhead * kThreads) {
+      for (int c0 = threadIdx.x; c0 < wide.count; c0 += kAhead * kThreads) {
         vec_t<T, K> x[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
@@ -553,44 +630,32 @@ __device__ inline bool draw_sums(const SampleArgs &a, uint64_t r, const unsigned
         for (int u = 0; u < kAhead; ++u) {
 #pragma unroll
           for (int k = 0; k < K; ++k) {
-            if (buckets.of((float)x[u][k]) != border) continue;  // what is not of the row is below all buckets
+            if (buckets.of(weight.exponent((float)x[u][k])) != border) continue;
+            const int j = wide.column(c0 + u * kThreads, k);
+            if (j < 0 || j >= wide.cols) continue;
             const unsigned at = atomicAdd(&s.count, 1u);
-            if (at < (unsigned)kList) s.list[at] = (unsigned long long)key_of((float)x[u][k]) << a.index_bits | (unsigned long long)((c0 + u * kThreads) * K + k - wide.lead);
+            if (at < (unsigned)kList) s.list[at] = (unsigned long long)key_of((float)x[u][k]) << a.index_bits | (unsigned long long)j;
           }
         }
       }
       __syncthreads();
-      const int count = (int)(s.count < (unsigned)kList + 1 ? s.count : (unsigned)kList + 1);
-      if (count > kList) return false;
-      const ListSource list{s.list, count, a.index_bits};
-      if (count <= kPairs) {
-        int log_each = 0;
-        while (log_each < 6 && (count << (log_each + 1)) <= kThreads) ++log_each;
-        const int each = 1 << log_each, me = threadIdx.x >> log_each;
-        const unsigned long long o = me < count ? s.list[me] : ~0ull;
-        if (threadIdx.x < count) s.units[threadIdx.x] = weight.units(weight.scaled(logit_of((uint32_t)(s.list[threadIdx.x] >> a.index_bits))));
-        __syncthreads();
-        unsigned long long upto = 0;
-        for (int i = threadIdx.x & (each - 1); i < count; i += each) upto += s.list[i] <= o ? s.units[i] : 0;
-        upto = among(upto, each);
-        last = block_min(me < count && upto >= within ? o : ~0ull, s.sh);
-      } else {
-        last = select_key(32 + a.index_bits, within, s.sh, [&](auto f) {
-          list.each([&](float x, uint32_t j) { f((unsigned long long)key_of(x) << a.index_bits | j, weight.units(weight.scaled(x))); });
-        });
-      }
+      if (s.count > (unsigned)kList) return false;
+      const Held h(s.list, (int)s.count, weight, a.index_bits);
+      last = select_held(h.o, h.units, within, s.sh);
       // what is kept of every part
       if (threadIdx.x < kParts) s.hist[threadIdx.x][border] = 0;
       __syncthreads();
-      const int64_t span = (row.count + kParts - 1) / kParts;
-      list.each([&](float x, uint32_t j) {
-        if (((unsigned long long)key_of(x) << a.index_bits | j) > last) return;
-        atomicAdd(&s.hist[((int64_t)j + row.lead) / (8 / (int)sizeof(T)) / span][border], weight.units(weight.scaled(x)));
-      });
+      const int span = (row.count + kParts - 1) / kParts;
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        if ((int)threadIdx.x + i * kThreads >= (int)s.count || h.o[i] > last) continue;
+        const int j = (int)(h.o[i] & ((1ull << a.index_bits) - 1));
+        atomicAdd(&s.hist[(j + row.lead) / (8 / (int)sizeof(T)) / span][border], h.units[i]);
+      }
       __syncthreads();
       static_assert(kThreads / 64 == kParts, "a wave each");
       unsigned long long kept = 0;
-      for (int b = threadIdx.x & 63; b <= border; b += 64) kept += s.hist[threadIdx.x / 64][b];
+      for (unsigned b = threadIdx.x & 63; b <= border; b += 64) kept += s.hist[threadIdx.x / 64][b];
       for (int off = 1; off < 64; off <<= 1) kept += __shfl_xor(kept, off, 64);
       __syncthreads();
       if ((threadIdx.x & 63) == 0) s.units[threadIdx.x / 64] = kept;
@@ -605,35 +670,35 @@ __device__ inline bool draw_sums(const SampleArgs &a, uint64_t r, const unsigned
   while (part < kParts - 1 && at > s.units[part]) at -= s.units[part++];
   const Part span(row.count, part);
   find_class(row, span.first, span.last, at, s.sh,
-             [&](float x, int64_t j) -> unsigned long long {
-               const double w = weight.scaled(x);
+             [&](float x, int j) -> unsigned long long {
+               const double y = weight.exponent(x), w = weight.scaled(y);
                bool kept = w >= weight.least;
                if (nucleus) {
-                 const int b = buckets.of(x);
+                 const unsigned b = buckets.of(y);
                  kept = b < border || (b == border && ((unsigned long long)key_of(x) << a.index_bits | (unsigned long long)j) <= last);
                }
                return kept ? weight.units(w) : 0;
              },
-             [&](float x, int64_t j) { write_token(a, r, (uint32_t)j, x, weight, q.t, total); });
+             [&](float x, int j) { write_token(a, r, (uint32_t)j, x, weight, q.t, total); });
   return true;
 }
 
 template <class T>
-__global__ void __launch_bounds__(kThreads, 4) k_sample_list(SampleArgs a) {
+__global__ void __launch_bounds__(kThreads) k_sample_list(SampleArgs a) {
   constexpr int K = 16 / sizeof(T);
   __shared__ ListShared s;
   const T none = (T)-INFINITY;
   for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     __syncthreads();
-    const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int64_t)a.cols);
+    const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int)a.cols);
     const Params q = params_of(a, r);
-    const int64_t small = (row.count + kGroup - 1) / kGroup, size = (small + kMaxGroups - 1) / kMaxGroups;
-    const int groups = (int)((small + size - 1) / size);  // of `size` times kGroup granules
+    const int small = (row.count + kGroup - 1) / kGroup, size = (small + kMaxGroups - 1) / kMaxGroups;
+    const int groups = (small + size - 1) / size;  // of `size` times kGroup granules
     // the groups' largest logits, and the row's
     float top = -INFINITY;
     for (int g = threadIdx.x; g < groups; g += kThreads) {
       float m = -INFINITY;
-      for (int64_t i = g * size; i < (g + 1) * size && i < small; ++i) m = fmaxf(m, a.tops[r * a.groups + i]);
+      for (int i = g * size; i < (g + 1) * size && i < small; ++i) m = fmaxf(m, a.tops[r * a.groups + i]);
       s.tops[g] = m;
       top = fmaxf(top, m);
     }
@@ -678,11 +743,11 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample_list(SampleArgs a) {
     const unsigned per = (unsigned)(size * kGroup), granules = s.nhits * per;  // at most the row's 2^31 / K and kMaxGroups' rounding
     for (unsigned i = threadIdx.x; i < granules; i += 4 * kThreads) {
       vec_t<T, K> x[4];
-      int64_t c[4];
+      int c[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const unsigned at = i + u * kThreads;
-        c[u] = at < granules ? (int64_t)s.hits[at / per] * per + at % per : row.count;
+        c[u] = at < granules ? (int)(s.hits[at / per] * per + at % per) : row.count;
         if (c[u] < row.count) x[u] = row.load(c[u], none);
       }
 #pragma unroll
@@ -691,11 +756,11 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample_list(SampleArgs a) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           const float v = (float)x[u][k];
-          const int64_t j = c[u] * K + k - row.lead;
+          const int j = row.column(c[u], k);
           if (v >= bound && j >= 0 && j < row.cols) {
             const unsigned at = atomicAdd(&s.count, 1u);
             const unsigned long long o = (unsigned long long)key_of(v) << a.index_bits | (unsigned long long)j;
-            if (at < (unsigned)kPairs) s.list[at] = o;
+            if (at < (unsigned)kList) s.list[at] = o;
             first = o < first ? o : first;
           }
         }
@@ -709,6 +774,8 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample_list(SampleArgs a) {
       }
     } else if (s.count <= (unsigned)kPairs) {
       draw_pairs(a, r, q, Weights(top, q.t, q.m, a.shift), first, s, (int)s.count);
+    } else if (s.count <= (unsigned)kList) {
+      draw_held(a, r, q, Weights(top, q.t, q.m, a.shift), first, s.list, (int)s.count, s.sh);
     } else if (threadIdx.x == 0) {
       a.token[r] = kLeft;
     }
@@ -730,13 +797,13 @@ __global__ void __launch_bounds__(kThreads) k_sample_rest(SampleArgs a, uint64_t
   __syncthreads();
   if (by_sums(q, top) && draw_sums<T>(a, r, a.sums + blockIdx.x * (uint64_t)(kParts * kSums), q, weight, s)) return;
   __syncthreads();
-  const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int64_t)a.cols);
+  const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int)a.cols);
   unsigned long long first = ~0ull;  // the lowest index of the largest logit
-  for (int64_t c = threadIdx.x; c < row.count && first == ~0ull; c += kThreads) {
+  for (int c = threadIdx.x; c < row.count && first == ~0ull; c += kThreads) {
     const vec_t<T, 16 / sizeof(T)> x = row.load(c, (T)-INFINITY);
 #pragma unroll
     for (int k = 16 / sizeof(T) - 1; k >= 0; --k)
-      if ((float)x[k] == top) first = (unsigned long long)(c * (int64_t)(16 / sizeof(T)) + k - row.lead);
+      if ((float)x[k] == top) first = (unsigned long long)row.column(c, k);
   }
   first = block_min(first, s.sh);
   if (is_greedy(q)) {
@@ -783,7 +850,7 @@ using namespace admm_impl;
 
 extern "C" int admm_sample_workspace(uint64_t rows, uint64_t cols, uint64_t *bytes) {
   ADMM_REQUIRE(bytes, "admm_sample_workspace: bytes is NULL");
-  ADMM_REQUIRE(rows < (1ull << 40) && cols < (1ull << 31), "admm_sample_workspace: %llu x %llu logits", (unsigned long long)rows,
+  ADMM_REQUIRE(rows < (1ull << 40) && cols <= kMaxClasses, "admm_sample_workspace: %llu x %llu logits", (unsigned long long)rows,
                (unsigned long long)cols);
   // enough for logits of any type: granules of four floats are the most
   *bytes = tops_bytes(rows, tops_groups(cols, 4)) + (rows < kBatch ? rows : kBatch) * (kParts * kSums * sizeof(unsigned long long));
@@ -795,7 +862,7 @@ extern "C" int admm_sample(admm_ctx *ctx, const admm_mat *logits, const admm_sam
   ADMM_REQUIRE(ctx, "admm_sample: ctx is NULL");
   ADMM_TRY(check_mat(logits, "admm_sample", "logits"));
   if (logits->rows == 0) return ADMM_OK;
-  ADMM_REQUIRE(logits->cols > 0 && logits->cols < (1ull << 31), "admm_sample: %llu classes", (unsigned long long)logits->cols);
+  ADMM_REQUIRE(logits->cols > 0 && logits->cols <= kMaxClasses, "admm_sample: %llu classes", (unsigned long long)logits->cols);
   ADMM_REQUIRE(uniform && token, "admm_sample: uniform or token is NULL");
   uint64_t need = 0;
   ADMM_TRY(admm_sample_workspace(logits->rows, logits->cols, &need));

@@ -77,7 +77,7 @@ __device__ inline void stay_packed(V &x) {
 
 // the gradient of a chunk; `at`: which of its elements the label is, or anything else
 template <class T>
-__device__ inline vec_t<T, 16 / sizeof(T)> chunk_grad(const vec_t<T, 16 / sizeof(T)> &x, float l, float lse2, float g, int64_t at) {
+__device__ inline vec_t<T, 16 / sizeof(T)> chunk_grad(const vec_t<T, 16 / sizeof(T)> &x, float l, float lse2, float g, int at) {
   constexpr int K = 16 / sizeof(T);
   float v[K];
 #pragma unroll
@@ -112,12 +112,12 @@ __global__ void __launch_bounds__(256) k_softmax_lanes(SoftmaxArgs a) {
   for (uint64_t r = (uint64_t)blockIdx.x * per + (threadIdx.x >> a.lanes_log2); r < a.rows; r += (uint64_t)gridDim.x * per) {
     float w;
     const int64_t t = label_of(a, r, w);
-    const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, a.cols);
+    const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int)a.cols);
     T *to = a.grad ? static_cast<T *>(a.grad) + r * a.gstride : nullptr;
     vec_t<T, K> x[CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c)
-      if (c * lanes + lane < row.count) x[c] = row.load(c * lanes + lane, none);
+      if ((int)(c * lanes + lane) < row.count) x[c] = row.load(c * lanes + lane, none);
       else x[c] = none;
     const float xt = t >= 0 ? (float)row.base[row.lead + t] : 0.0f;
     float m = -INFINITY;
@@ -135,12 +135,12 @@ __global__ void __launch_bounds__(256) k_softmax_lanes(SoftmaxArgs a) {
     finish_row(a, r, b, s, t, w, xt, lane == 0, lse2);
     if (!to) continue;
     const float g = t < 0 ? 0.0f : w * a.grad_scale;
-    const int64_t tc = t < 0 ? -1 : t + row.lead;
+    const int tc = t < 0 ? -1 : (int)t + row.lead;
 #pragma unroll
     for (int c = 0; c < CH; ++c) stay_packed(x[c]);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int64_t at = c * lanes + lane;
+      const int at = c * (int)lanes + (int)lane;
       if (at >= row.count) continue;
       const vec_t<T, K> zero = (T)0.0f;
       row.store(to, a.apart, at, t < 0 || s == 0.0f ? zero : chunk_grad<T>(x[c], b.l, lse2, g, tc - at * K));
@@ -179,12 +179,12 @@ __global__ void __launch_bounds__(NT) k_softmax_block(SoftmaxArgs a) {
   for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     float w;
     const int64_t t = label_of(a, r, w);
-    const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, a.cols);
+    const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int)a.cols);
     T *to = a.grad ? static_cast<T *>(a.grad) + r * a.gstride : nullptr;
     const vec_t<T, K> zero = (T)0.0f;
     if (t < 0 && !a.lse) {  // nothing of the row is needed
       if (to)
-        for (int64_t c = threadIdx.x; c < row.count; c += NT) row.store(to, a.apart, c, zero);
+        for (int c = threadIdx.x; c < row.count; c += NT) row.store(to, a.apart, c, zero);
       if (threadIdx.x == 0) a.loss[r] = 0.0f;
       continue;
     }
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(NT) k_softmax_block(SoftmaxArgs a) {
     if (CH) {
 #pragma unroll
       for (int c = 0; c < CH; ++c)
-        if (c * NT + threadIdx.x < row.count) x[c] = row.load(c * NT + threadIdx.x, none);
+        if (c * NT + (int)threadIdx.x < row.count) x[c] = row.load(c * NT + threadIdx.x, none);
         else x[c] = none;
 #pragma unroll
       for (int c = 0; c < CH; ++c) m = chunk_max<T>(x[c], m);
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(NT) k_softmax_block(SoftmaxArgs a) {
       for (int c = 0; c < CH; ++c) s += chunk_sum<T>(x[c], b);
     } else {
       // one pass: the sum is kept relative to the running maximum
-      for (int64_t c = threadIdx.x; c < row.count; c += NT) {
+      for (int c = threadIdx.x; c < row.count; c += NT) {
         const vec_t<T, K> y = row.load(c, none);
         const float mc = chunk_max<T>(y, m);
         if (mc > m) {
@@ -228,18 +228,18 @@ __global__ void __launch_bounds__(NT) k_softmax_block(SoftmaxArgs a) {
     finish_row(a, r, b, s, t, w, xt, threadIdx.x == 0, lse2);
     if (to) {
       const float g = t < 0 ? 0.0f : w * a.grad_scale;
-      const int64_t tc = t < 0 ? -1 : t + row.lead;
+      const int tc = t < 0 ? -1 : (int)t + row.lead;
       const bool no = t < 0 || s == 0.0f;
       if (CH) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) stay_packed(x[c]);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-          const int64_t at = c * NT + threadIdx.x;
+          const int at = c * NT + (int)threadIdx.x;
           if (at < row.count) row.store(to, a.apart, at, no ? zero : chunk_grad<T>(x[c], b.l, lse2, g, tc - at * K));
         }
       } else {
-        for (int64_t c = threadIdx.x; c < row.count; c += NT)
+        for (int c = threadIdx.x; c < row.count; c += NT)
           row.store(to, a.apart, c, no ? zero : chunk_grad<T>(row.load(c, none), b.l, lse2, g, tc - c * K));
       }
     }
@@ -277,7 +277,7 @@ using namespace admm_impl;
 
 extern "C" int admm_softmax_loss_workspace(uint64_t rows, uint64_t cols, uint64_t *bytes) {
   ADMM_REQUIRE(bytes, "admm_softmax_loss_workspace: bytes is NULL");
-  ADMM_REQUIRE(rows < (1ull << 40) && cols < (1ull << 40), "admm_softmax_loss_workspace: %llu x %llu logits", (unsigned long long)rows,
+  ADMM_REQUIRE(rows < (1ull << 40) && cols <= kMaxClasses, "admm_softmax_loss_workspace: %llu x %llu logits", (unsigned long long)rows,
                (unsigned long long)cols);
   *bytes = 0;
   return ADMM_OK;
@@ -298,6 +298,7 @@ extern "C" int admm_softmax_loss(admm_ctx *ctx, const admm_mat *logits, const vo
   }
   if (logits->rows == 0) return ADMM_OK;
   ADMM_REQUIRE(logits->cols > 0, "admm_softmax_loss: no classes");
+  ADMM_REQUIRE(logits->cols <= kMaxClasses, "admm_softmax_loss: %llu classes", (unsigned long long)logits->cols);
   ADMM_REQUIRE(labels && loss, "admm_softmax_loss: labels or loss is NULL");
   uint64_t need = 0;
   ADMM_TRY(admm_softmax_loss_workspace(logits->rows, logits->cols, &need));

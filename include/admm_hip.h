@@ -369,7 +369,7 @@ int admm_embed_grad(admm_ctx *ctx, const admm_bags *bags, const void *order, uin
  * is outside [0, cols) or whose weight is 0 is not trained on: loss 0, gradient 0.  Logits of -inf are classes that are
  * masked out: probability 0, gradient 0.  A row whose label is masked has loss +inf; one with no class left has loss +inf
  * and gradient 0 (lse -inf).  A NaN, or a logit of +inf, makes its row NaN.
- * lse and grad may be NULL (not wanted); grad has the logits' shape and type and may be the logits' own memory (same data
+ * cols <= 2^31 - 256.  lse and grad may be NULL (not wanted); grad has the logits' shape and type and may be the logits' own memory (same data
  * and stride), else it may not overlap them. */
 int admm_softmax_loss_workspace(uint64_t rows, uint64_t cols, uint64_t *bytes);
 int admm_softmax_loss(admm_ctx *ctx, const admm_mat *logits, const void *labels, int label_type, const float *weight,
@@ -388,7 +388,7 @@ int admm_softmax_loss(admm_ctx *ctx, const admm_mat *logits, const void *labels,
  * NULL: 1, and no filter.  uniform is in [0, 1); what is outside counts as the nearest end.  NaN logits count as -inf; a
  * row without any logit above -inf gives token -1 and logprob -inf; logits of +inf share all the mass.
  * Weights are rounded to multiples of 2^-51 of the row's largest (for more than 2^11 classes of 2^-(62 - ceil(log2 cols)))
- * and summed as integers, so a draw does not depend on the batch it is in.  cols < 2^31. */
+ * and summed as integers, so a draw does not depend on the batch it is in.  cols <= 2^31 - 256. */
 typedef struct admm_sample_params {
   const float *temperature;
   const int32_t *top_k;
