@@ -3,9 +3,8 @@
 
 namespace admm_impl {
 
-constexpr int kRun = 64;         // entries of one id that one unit sums; longer runs are cut at multiples of it
-constexpr int kSortTile = 4096;  // entries per workgroup of the sort's passes
-constexpr int kSortSmall = 8192; // entries that one workgroup sorts in its LDS
+constexpr uint64_t kMaxCount = 0xFFFFFF00ull;  // entries, rows: counted in 32 bits with room for a step beyond
+constexpr int kSortSmall = 16384;  // entries that one workgroup can sort in its LDS
 
 // ---- lookup -----------------------------------------------------------------------------------
 
@@ -154,10 +153,11 @@ __device__ inline uint32_t key_of(Id id, uint32_t trows) {
 // Stable ranks among equal digits, wave by wave: the lanes with the same digit find each other by one ballot per bit, and
 // the first of them takes their places from the wave's counter of that digit.
 template <int ITEMS>
-__device__ inline void rank_items(const uint32_t (&digit)[ITEMS], uint32_t (&rank)[ITEMS], int bits, uint32_t *counters) {
+__device__ inline void rank_items(const uint32_t (&digit)[ITEMS], uint32_t (&rank)[ITEMS], int items, int bits, uint32_t *counters) {
   const unsigned lane = threadIdx.x & 63;
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
+    if (i >= items) break;
     unsigned long long same = ~0ull;
     for (int b = 0; b < bits; ++b) {
       const bool bit = (digit[i] >> b) & 1;
@@ -174,12 +174,12 @@ __device__ inline void rank_items(const uint32_t (&digit)[ITEMS], uint32_t (&ran
 
 // counters[wave][digit] -> first place of that wave's items with that digit, counted from `from(digit)`; one thread a digit
 template <int WAVES, class From>
-__device__ inline void waves_before(uint32_t *counters, int digits, From from) {
-  for (int d = threadIdx.x; d < digits; d += WAVES * 64) {
-    uint32_t sum = from(d);
+__device__ inline void waves_before(uint32_t *counters, From from) {
+  if (threadIdx.x < 256) {
+    uint32_t sum = from(threadIdx.x);
     for (int w = 0; w < WAVES; ++w) {
-      const uint32_t n = counters[w * 256 + d];
-      counters[w * 256 + d] = sum;
+      const uint32_t n = counters[w * 256 + threadIdx.x];
+      counters[w * 256 + threadIdx.x] = sum;
       sum += n;
     }
   }
@@ -216,36 +216,72 @@ struct Sorted {
   float *val;
   const uint32_t *row_of;  // row of every entry in the caller's order; NULL: entry e is row e
   const float *val_of;     // the caller's factors or NULL
-  __device__ void put(uint32_t at, uint32_t key, uint32_t entry) const {
-    ids[at] = key;
-    rows[at] = row_of ? row_of[entry] : entry;
-    if (val_of) val[at] = val_of[entry];
-  }
 };
 
-// up to kSortSmall entries: all passes in one workgroup, keys and entries in its LDS
+// Up to kSortSmall entries, in one launch: every workgroup looks at all keys and sorts those of its own range of them in its
+// LDS; how many are below its range says where they go.  (All passes over all keys in one workgroup: 17.5 us for 4001 keys of
+// 15 bits; this: 9.)
 template <class Id>
-__global__ void __launch_bounds__(1024) k_sort_small(const Id *__restrict__ ids, uint32_t n, uint32_t trows, int bits, Sorted to) {
+__global__ void __launch_bounds__(1024) k_sort_small(const Id *__restrict__ ids, uint32_t n, uint32_t trows, Sorted to) {
   constexpr int kItems = kSortSmall / 1024;
-  extern __shared__ uint32_t sort_sh[];  // keys [kSortSmall], entries [kSortSmall], counters [16][256], totals [256]
-  uint32_t *keys = sort_sh, *entries = keys + kSortSmall, *counters = entries + kSortSmall, *totals = counters + 16 * 256;
+  extern __shared__ uint32_t sort_sh[];  // counters [16][256], totals [256], 16 + 16 counts of the waves, keys [n], entries [n]
+  uint32_t *counters = sort_sh, *totals = counters + 16 * 256, *mine = totals + 256, *less = mine + 16, *keys = less + 16, *entries = keys + n;
   const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t base = wave * (kItems * 64) + lane;  // a wave's items are consecutive, so ranks follow the order
+  const uint32_t width = (uint32_t)(((uint64_t)trows + gridDim.x) / gridDim.x);  // of the trows + 1 keys
+  const uint64_t from = (uint64_t)width * blockIdx.x, to_key = from + width;
   uint32_t key[kItems], entry[kItems];
+  int items = (int)((n + 1023) / 1024);
+  // a wave's items are consecutive, so what it keeps of them follows the order
+  const uint32_t base = wave * (uint32_t)(items * 64) + lane;
+  uint32_t kept = 0, below = 0;
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
+    if (i >= items) break;
     const uint32_t at = base + i * 64;
     key[i] = at < n ? key_of(ids[at], trows) : 0xFFFFFFFFu;
-    entry[i] = at;
+    const bool in = at < n && key[i] >= from && key[i] < to_key;
+    const unsigned long long on = __ballot(in);
+    below += (uint32_t)__popcll(__ballot(key[i] < from));
+    entry[i] = in ? kept + (uint32_t)__popcll(on & ((1ull << lane) - 1)) : 0xFFFFFFFFu;
+    kept += (uint32_t)__popcll(on);
   }
-  const int passes = (bits + 7) / 8, width = (bits + passes - 1) / passes;
+  if (lane == 0) {
+    mine[wave] = kept;
+    less[wave] = below;
+  }
+  __syncthreads();
+  uint32_t count = 0, first = 0, place = 0;
+  for (unsigned w = 0; w < 16; ++w) {
+    if (w == wave) place = count;
+    count += mine[w];
+    first += less[w];
+  }
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    if (i >= items) break;
+    if (entry[i] == 0xFFFFFFFFu) continue;
+    keys[place + entry[i]] = key[i] - (uint32_t)from;
+    entries[place + entry[i]] = base + i * 64;
+  }
+  __syncthreads();
+  int bits = 0;
+  while (bits < 32 && (width - 1) >> bits) ++bits;
+  const int passes = (bits + 7) / 8, digits = passes ? (bits + passes - 1) / passes : 0;
+  items = (int)((count + 1023) / 1024);
+  const uint32_t b2 = wave * (uint32_t)(items * 64) + lane;
   for (int p = 0; p < passes; ++p) {
     uint32_t digit[kItems], rank[kItems];
     for (int i = threadIdx.x; i < 16 * 256; i += 1024) counters[i] = 0;
-    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) digit[i] = (key[i] >> (p * width)) & ((1u << width) - 1);
-    rank_items<kItems>(digit, rank, width, counters + wave * 256);
+    for (int i = 0; i < kItems; ++i) {
+      if (i >= items) break;
+      const uint32_t at = b2 + i * 64;
+      key[i] = at < count ? keys[at] : 0xFFFFFFFFu;
+      entry[i] = at < count ? entries[at] : 0;
+      digit[i] = (key[i] >> (p * digits)) & ((1u << digits) - 1);
+    }
+    __syncthreads();
+    rank_items<kItems>(digit, rank, items, digits, counters + wave * 256);
     __syncthreads();
     if (threadIdx.x < 256) {
       uint32_t s = 0;
@@ -253,62 +289,53 @@ __global__ void __launch_bounds__(1024) k_sort_small(const Id *__restrict__ ids,
       totals[threadIdx.x] = s;
     }
     scan_256(totals);
-    waves_before<16>(counters, 256, [&](int d) { return totals[d]; });
+    waves_before<16>(counters, [&](int d) { return totals[d]; });
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
+      if (i >= items) break;
+      // the padding's digit is the largest and it comes behind everything: its places are `count` and beyond
       const uint32_t at = counters[wave * 256 + digit[i]] + rank[i];
+      if (at >= count) continue;
       keys[at] = key[i];
       entries[at] = entry[i];
     }
     __syncthreads();
-    if (p + 1 < passes) {
-#pragma unroll
-      for (int i = 0; i < kItems; ++i) {
-        key[i] = keys[base + i * 64];
-        entry[i] = entries[base + i * 64];
-      }
-      __syncthreads();
-    }
   }
-  // the padding's keys are all ones in every digit and came last in every pass: they are behind the n entries
-  for (uint32_t at = threadIdx.x; at < n; at += 1024) to.put(at, keys[at], entries[at]);
-}
-
-// one pass over more entries, least significant digit first: counts per tile, their sums, the move
-template <class Id, bool FIRST>
-__device__ inline void load_tile(const Id *ids, const uint32_t *keys, const uint32_t *entries, uint32_t n, uint32_t trows,
-                                 uint32_t base, uint32_t (&key)[kSortTile / 256], uint32_t (&entry)[kSortTile / 256]) {
-#pragma unroll
-  for (int i = 0; i < kSortTile / 256; ++i) {
-    const uint32_t at = base + i * 64;
-    key[i] = 0xFFFFFFFFu;
-    entry[i] = 0;
-    if (at < n) {
-      key[i] = FIRST ? key_of(ids[at], trows) : keys[at];
-      entry[i] = FIRST ? at : entries[at];
-    }
+  for (uint32_t i = threadIdx.x; i < count; i += 1024) {
+    const uint32_t e = entries[i];
+    to.ids[first + i] = keys[i] + (uint32_t)from;
+    to.rows[first + i] = to.row_of ? to.row_of[e] : e;
+    if (to.val_of) to.val[first + i] = to.val_of[e];
   }
 }
 
+// More entries: one pass per digit, least significant first: counts per tile, their sums, the move.  What is moved with the key
+// is the entry's row, and its factor in the upper half where there are factors.
 template <class Id, bool FIRST>
+__device__ inline uint32_t sort_key(const Id *ids, const uint32_t *keys, uint32_t at, uint32_t trows) {
+  return FIRST ? key_of(ids[at], trows) : keys[at];
+}
+
+template <class Id, bool FIRST, int TILE>
 __global__ void __launch_bounds__(256) k_sort_count(const Id *__restrict__ ids, const uint32_t *__restrict__ keys, uint32_t n,
                                                     uint32_t trows, int shift, int width, uint32_t *__restrict__ counts) {
   __shared__ uint32_t hist[256];
   hist[threadIdx.x] = 0;
   __syncthreads();
-  const uint32_t base = blockIdx.x * (uint32_t)kSortTile;
-  for (int i = 0; i < kSortTile / 256; ++i) {
+  const uint32_t base = blockIdx.x * (uint32_t)TILE;
+#pragma unroll 4
+  for (int i = 0; i < TILE / 256; ++i) {
     const uint32_t at = base + i * 256 + threadIdx.x;
-    if (at < n) atomicAdd(&hist[((FIRST ? key_of(ids[at], trows) : keys[at]) >> shift) & ((1u << width) - 1)], 1u);
+    if (at < n) atomicAdd(&hist[(sort_key<Id, FIRST>(ids, keys, at, trows) >> shift) & ((1u << width) - 1)], 1u);
   }
   __syncthreads();
-  counts[(uint64_t)threadIdx.x * gridDim.x + blockIdx.x] = hist[threadIdx.x];
+  if (threadIdx.x < (1u << width)) counts[(uint64_t)threadIdx.x * gridDim.x + blockIdx.x] = hist[threadIdx.x];
 }
 
 // per digit: exclusive sums of its counts over the tiles, and its total
 __global__ void __launch_bounds__(256) k_sort_scan(uint32_t *__restrict__ counts, uint32_t ntiles, uint32_t *__restrict__ totals) {
-  __shared__ uint32_t sums[256];
+  __shared__ uint32_t sums[4];
   uint32_t *c = counts + (uint64_t)blockIdx.x * ntiles;
   uint32_t carry = 0;
   for (uint32_t t0 = 0; t0 < ntiles; t0 += 1024) {
@@ -319,17 +346,19 @@ __global__ void __launch_bounds__(256) k_sort_scan(uint32_t *__restrict__ counts
       x[k] = t < ntiles ? c[t] : 0;
       s += x[k];
     }
-    sums[threadIdx.x] = s;
-    __syncthreads();
-    for (int off = 1; off < 256; off <<= 1) {
-      const uint32_t y = (int)threadIdx.x >= off ? sums[threadIdx.x - off] : 0;
-      __syncthreads();
-      sums[threadIdx.x] += y;
-      __syncthreads();
+    uint32_t up = s;
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint32_t y = __shfl_up(up, off, 64);
+      if ((int)(threadIdx.x & 63) >= off) up += y;
     }
-    uint32_t up = carry + sums[threadIdx.x] - s;
-    carry += sums[255];
     __syncthreads();
+    if ((threadIdx.x & 63) == 63) sums[threadIdx.x >> 6] = up;
+    __syncthreads();
+    up += carry - s;
+    for (unsigned w = 0; w < 4; ++w) {
+      if (w < threadIdx.x >> 6) up += sums[w];
+      carry += sums[w];
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const uint32_t t = t0 + threadIdx.x * 4 + k;
@@ -340,36 +369,66 @@ __global__ void __launch_bounds__(256) k_sort_scan(uint32_t *__restrict__ counts
   if (threadIdx.x == 0) totals[blockIdx.x] = carry;
 }
 
-template <class Id, bool FIRST, bool LAST>
-__global__ void __launch_bounds__(256) k_sort_move(const Id *__restrict__ ids, const uint32_t *__restrict__ keys,
-                                                   const uint32_t *__restrict__ entries, uint32_t n, uint32_t trows, int shift,
-                                                   int width, const uint32_t *__restrict__ counts,
+// The tile is put in order in LDS first, so that what goes to one digit's place is written side by side.
+template <class Id, class Load, bool FIRST, bool LAST, int TILE>
+__global__ void __launch_bounds__(256) k_sort_move(const Id *__restrict__ ids, const uint32_t *__restrict__ keys, const Load *__restrict__ loads,
+                                                   uint32_t n, uint32_t trows, int shift, int width, const uint32_t *__restrict__ counts,
                                                    const uint32_t *__restrict__ totals, uint32_t *__restrict__ keys_to,
-                                                   uint32_t *__restrict__ entries_to, Sorted to) {
-  constexpr int kItems = kSortTile / 256;
-  __shared__ uint32_t counters[4 * 256], start[256];
+                                                   Load *__restrict__ loads_to, Sorted to) {
+  constexpr int kItems = TILE / 256;
+  __shared__ uint32_t counters[4 * 256], start[256], local[256], tile_keys[TILE];
+  __shared__ Load tile_loads[TILE];
   const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t key[kItems], entry[kItems], digit[kItems], rank[kItems];
-  load_tile<Id, FIRST>(ids, keys, entries, n, trows, blockIdx.x * (uint32_t)kSortTile + wave * (kItems * 64) + lane, key, entry);
-  for (int i = threadIdx.x; i < 4 * 256; i += 256) counters[i] = 0;
-  start[threadIdx.x] = totals[threadIdx.x];
-  scan_256(start);
+  const uint32_t tile = blockIdx.x * (uint32_t)TILE, count = n - tile < (uint32_t)TILE ? n - tile : (uint32_t)TILE;
+  const uint32_t base = wave * (kItems * 64) + lane, mask = (1u << width) - 1;
+  uint32_t key[kItems], digit[kItems], rank[kItems];
+  Load load[kItems];
 #pragma unroll
-  for (int i = 0; i < kItems; ++i) digit[i] = (key[i] >> shift) & ((1u << width) - 1);
-  rank_items<kItems>(digit, rank, width, counters + wave * 256);
+  for (int i = 0; i < kItems; ++i) {
+    const uint32_t in = base + i * 64, at = tile + in;
+    key[i] = 0xFFFFFFFFu;
+    load[i] = 0;
+    if (in < count) {
+      key[i] = sort_key<Id, FIRST>(ids, keys, at, trows);
+      if (FIRST) {
+        load[i] = to.row_of ? to.row_of[at] : at;
+        if (sizeof(Load) == 8) load[i] |= (Load)((unsigned long long)__float_as_uint(to.val_of[at]) << 32);
+      } else {
+        load[i] = loads[at];
+      }
+    }
+    digit[i] = (key[i] >> shift) & mask;
+  }
+  for (int i = threadIdx.x; i < 4 * 256; i += 256) counters[i] = 0;
+  start[threadIdx.x] = threadIdx.x <= mask ? totals[threadIdx.x] : 0;
+  scan_256(start);
+  rank_items<kItems>(digit, rank, kItems, width, counters + wave * 256);
   __syncthreads();
-  waves_before<4>(counters, 256, [&](int d) { return start[d] + counts[(uint64_t)d * gridDim.x + blockIdx.x]; });
+  local[threadIdx.x] = counters[threadIdx.x] + counters[256 + threadIdx.x] + counters[512 + threadIdx.x] + counters[768 + threadIdx.x];
+  scan_256(local);
+  waves_before<4>(counters, [&](int d) { return local[d]; });
+  // a digit's place in the whole, less its place in the tile
+  if (threadIdx.x <= mask) start[threadIdx.x] += counts[(uint64_t)threadIdx.x * gridDim.x + blockIdx.x] - local[threadIdx.x];
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
-    // what pads the last tile has the last digit and comes behind everything: its places are n and beyond
+    // what pads the last tile has the last digit and comes behind everything: its places are `count` and beyond
     const uint32_t at = counters[wave * 256 + digit[i]] + rank[i];
-    if (at >= n) continue;
+    tile_keys[at] = key[i];
+    tile_loads[at] = load[i];
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < count; i += 256) {
+    const uint32_t k = tile_keys[i], at = start[(k >> shift) & mask] + i;
+    const Load l = tile_loads[i];
     if (LAST) {
-      to.put(at, key[i], entry[i]);
+      to.ids[at] = k;
+      to.rows[at] = (uint32_t)l;
+      if (sizeof(Load) == 8) to.val[at] = __uint_as_float((uint32_t)((unsigned long long)l >> 32));
     } else {
-      keys_to[at] = key[i];
-      entries_to[at] = entry[i];
+      keys_to[at] = k;
+      loads_to[at] = l;
     }
   }
 }
@@ -390,204 +449,251 @@ __global__ void __launch_bounds__(256) k_fill_u32(uint32_t *p, uint64_t n, uint3
 
 // ---- gradient ---------------------------------------------------------------------------------
 
-// first position whose id is at least `id`
-__device__ inline uint64_t lower_bound(const uint32_t *ids, uint64_t n, uint32_t id) {
-  uint64_t lo = 0, hi = n;
-  while (lo < hi) {
-    const uint64_t mid = (lo + hi) >> 1;
-    if (ids[mid] < id) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
-}
-
 template <class T, class TO>
 struct GradArgs {
   const uint32_t *ids, *rows;  // sorted by id
   const float *val;            // or NULL
-  uint64_t n;
+  uint32_t n;
   const T *from;  // grad_out
   uint64_t fstride, frows;
   TO *to;  // grad_table
-  uint64_t tstride, trows, cols;
+  uint64_t tstride, cols;
+  uint32_t trows;
   float scale;
   int accumulate, lanes_log2;
-  float *parts;  // [chunk][2][cols] sums of the parts of runs longer than kRun
-  unsigned run_blocks, chunk_blocks, zero_blocks;
+  uint32_t chunk, nchunks;  // entries per chunk
+  float *parts;             // [chunk][2][cols]
+  unsigned chunk_blocks, zero_blocks;
 };
 
-// factor of entry e and its row's values; 0 for an entry without a row
-template <int N, class T, class TO>
-__device__ inline float load_entry(const GradArgs<T, TO> &a, uint64_t e, uint64_t col, int here, float (&v)[N]) {
-  const uint64_t row = a.rows[e];
-  if (row >= a.frows || here == 0) return 0.0f;
-  const T *from = a.from + row * a.fstride + col;
-  if (here == N) {
-    load_n<T, N>(from, v);
-  } else {
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = k < here ? (float)from[k < here ? k : 0] : 0.0f;
+// where this thread works: its columns, and its group of lanes among its workgroup's
+template <int N>
+struct Place {
+  unsigned lane, wave, lanes, groups, group, sub;
+  uint64_t col;
+  int here;  // columns of this thread
+  __device__ Place(int lanes_log2, uint64_t cols) {
+    lane = threadIdx.x & 63;
+    wave = threadIdx.x >> 6;
+    lanes = 1u << lanes_log2;
+    groups = 64u >> lanes_log2;
+    group = lane >> lanes_log2;
+    sub = lane & (lanes - 1);
+    col = ((uint64_t)blockIdx.y * lanes + sub) * N;
+    here = col >= cols ? 0 : cols - col < N ? (int)(cols - col) : N;
   }
-  return a.val ? a.val[e] : 1.0f;
-}
+};
 
 template <int N, class T, class TO>
-__device__ inline void put_row(const GradArgs<T, TO> &a, uint32_t id, uint64_t col, int here, float (&acc)[N]) {
-  TO *to = a.to + (uint64_t)id * a.tstride + col;
-  if (here == N) {
-    float old[N];
+__device__ inline void put_row(const GradArgs<T, TO> &a, uint32_t id, const Place<N> &p, const float (&acc)[N]) {
+  TO *to = a.to + (uint64_t)id * a.tstride + p.col;
+  if (p.here == N) {
+    float old[N], v[N];
     if (a.accumulate) load_n<TO, N>(to, old);
 #pragma unroll
-    for (int k = 0; k < N; ++k) acc[k] = a.accumulate ? old[k] + acc[k] * a.scale : acc[k] * a.scale;
-    store_n<TO, N>(to, acc);
+    for (int k = 0; k < N; ++k) v[k] = a.accumulate ? old[k] + acc[k] * a.scale : acc[k] * a.scale;
+    store_n<TO, N>(to, v);
   } else {
 #pragma unroll
     for (int k = 0; k < N; ++k)
-      if (k < here) to[k] = (TO)(a.accumulate ? (float)to[k] + acc[k] * a.scale : acc[k] * a.scale);
+      if (k < p.here) to[k] = (TO)(a.accumulate ? (float)to[k] + acc[k] * a.scale : acc[k] * a.scale);
   }
 }
 
-// Three kinds of blocks, every one over one tile of columns (blockIdx.y):
-//  * chunks: kRun sorted entries that may hold parts of at most two runs longer than kRun (the one that holds the first entry
-//    and the one that holds the last): their sums go to `parts`;
-//  * runs: one group of lanes per sorted entry; where a run of at most kRun entries begins it sums the run and writes the
-//    row.  Every row is written by one group, in a fixed order, without atomics;
+template <int N, class T, class TO>
+__device__ inline void put_part(const GradArgs<T, TO> &a, uint32_t chunk, int slot, const Place<N> &p, const float (&acc)[N]) {
+  float *to = a.parts + ((uint64_t)chunk * 2 + slot) * a.cols + p.col;
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (k < p.here) to[k] = acc[k];
+}
+
+// Two kinds of blocks, every one over one tile of columns (blockIdx.y):
+//  * chunks: a group of lanes sums a.chunk consecutive entries of the sorted order, however they fall into runs of one id.  A run
+//    that lies in the chunk is written at once; the sum of one that comes in from the chunk before goes to slot 0 of `parts`, that
+//    of one that begins here and goes on to slot 1.  So every group has the same work, every row is written by one group, in a
+//    fixed order and without atomics, whatever the ids.
 //  * zeros (only where every row has to be written): rows of the table that no entry names.
 template <class T, class TO, int N>
 __global__ void __launch_bounds__(256) k_grad(GradArgs<T, TO> a) {
-  const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const unsigned lanes = 1u << a.lanes_log2, groups = 64u >> a.lanes_log2;
-  const unsigned group = lane >> a.lanes_log2, sub = lane & (lanes - 1);
-  const uint64_t col = ((uint64_t)blockIdx.y * lanes + sub) * N;
-  const int here = col >= a.cols ? 0 : a.cols - col < N ? (int)(a.cols - col) : N;
+  const Place<N> p(a.lanes_log2, a.cols);
   if (blockIdx.x < a.chunk_blocks) {
-    const uint64_t nchunks = (a.n + kRun - 1) / kRun;
-    for (uint64_t c = (uint64_t)blockIdx.x * 4 + wave; c < nchunks; c += (uint64_t)a.chunk_blocks * 4) {
-      const uint64_t p0 = c * kRun, end = p0 + kRun < a.n ? p0 + kRun : a.n;
-      const uint32_t mine = p0 + lane < end ? a.ids[p0 + lane] : 0xFFFFFFFFu;
-      const uint32_t first = a.ids[p0], last = a.ids[end - 1];
-      for (int s = 0; s < 2; ++s) {
-        const uint32_t id = s == 0 ? first : last;
-        if (id >= a.trows || (s == 1 && last == first)) continue;
-        const uint64_t count = (uint64_t)__popcll(__ballot(p0 + lane < end && mine == id));
-        const uint64_t b = s == 0 ? p0 : end - count, e = b + count;
-        const uint64_t head = s == 0 ? lower_bound(a.ids, a.n, id) : b;
-        if (head + kRun >= a.n || a.ids[head + kRun] != id) continue;
-        float acc[N];
-        sum_entries<N>(b, e, a.lanes_log2, group, groups, [&](uint64_t j, float(&v)[N]) -> float { return load_entry<N>(a, j, col, here, v); }, acc);
-        add_groups<N>(a.lanes_log2, acc);
-        if (group == 0 && here) {
-          float *to = a.parts + (c * 2 + s) * a.cols + col;
-          for (int k = 0; k < N; ++k)
-            if (k < here) to[k] = acc[k];
-        }
-      }
-    }
-  } else if (blockIdx.x < a.chunk_blocks + a.run_blocks) {
-    const uint64_t per = 4u * groups;
-    for (uint64_t i = (uint64_t)(blockIdx.x - a.chunk_blocks) * per + wave * groups + group; i < a.n; i += (uint64_t)a.run_blocks * per) {
-      const uint32_t id = a.ids[i];
-      if (id >= a.trows || (i > 0 && a.ids[i - 1] == id) || (i + kRun < a.n && a.ids[i + kRun] == id)) continue;
+    constexpr int kAhead = 4;
+    for (uint64_t c = ((uint64_t)blockIdx.x * 4 + p.wave) * p.groups + p.group; c < a.nchunks; c += (uint64_t)a.chunk_blocks * 4 * p.groups) {
+      const uint32_t b = (uint32_t)c * a.chunk, end = a.n - b < a.chunk ? a.n : b + a.chunk;
+      uint32_t cur = a.ids[b];
+      bool open = b > 0 && a.ids[b - 1] == cur;
       float acc[N];
 #pragma unroll
       for (int k = 0; k < N; ++k) acc[k] = 0.0f;
-      bool on = true;
-      for (uint64_t e = i; on; e += 4) {
-        float v[4][N], f[4];
-        bool in[4];
+      for (uint32_t e = b; e < end; e += kAhead) {
+        float v[kAhead][N], f[kAhead];
+        uint32_t id[kAhead], row[kAhead];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          on = on && e + u < a.n && a.ids[e + u < a.n ? e + u : i] == id;
-          in[u] = on;
-          f[u] = 0.0f;
-          if (on) f[u] = load_entry<N>(a, e + u, col, here, v[u]);
+        for (int u = 0; u < kAhead; ++u) {
+          const uint32_t at = end - e > (uint32_t)u ? e + u : end - 1;
+          id[u] = a.ids[at];
+          row[u] = a.rows[at];
+          f[u] = a.val ? a.val[at] : 1.0f;
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (!in[u] || f[u] == 0.0f) continue;
+        for (int u = 0; u < kAhead; ++u) {
+          // an entry without a row, a row beyond grad_out (of an order that is not these bags'), the chunk's end
+          if (row[u] >= a.frows || end - e <= (uint32_t)u || id[u] >= a.trows) f[u] = 0.0f;
+          if (f[u] == 0.0f) continue;
+          const T *from = a.from + row[u] * a.fstride + p.col;
+          if (p.here == N) {
+            load_n<T, N>(from, v[u]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+              v[u][k] = 0.0f;
+              if (k < p.here) v[u][k] = (float)from[k];
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          if (end - e <= (uint32_t)u) continue;
+          if (id[u] != cur) {
+            if (cur < a.trows && p.here) {
+              if (open) put_part<N>(a, (uint32_t)c, 0, p, acc);
+              else put_row<N>(a, cur, p, acc);
+            }
+            cur = id[u];
+            open = false;
+#pragma unroll
+            for (int k = 0; k < N; ++k) acc[k] = 0.0f;
+          }
+          if (f[u] == 0.0f) continue;
 #pragma unroll
           for (int k = 0; k < N; ++k) acc[k] += v[u][k] * f[u];
         }
       }
-      if (here) put_row<N>(a, id, col, here, acc);
+      if (cur >= a.trows || !p.here) continue;
+      if (open) put_part<N>(a, (uint32_t)c, 0, p, acc);
+      else if (end < a.n && a.ids[end] == cur) put_part<N>(a, (uint32_t)c, 1, p, acc);
+      else put_row<N>(a, cur, p, acc);
     }
   } else {
-    const uint64_t nsets = (a.trows + 63) / 64;
-    for (uint64_t q = (uint64_t)(blockIdx.x - a.chunk_blocks - a.run_blocks) * 4 + wave; q < nsets; q += (uint64_t)a.zero_blocks * 4) {
-      const uint64_t v0 = q * 64 + lane;
-      bool absent = v0 < a.trows;
-      if (absent) {
-        const uint64_t at = lower_bound(a.ids, a.n, (uint32_t)v0);
-        absent = at >= a.n || a.ids[at] != (uint32_t)v0;
+    const uint32_t nsets = (uint32_t)(((uint64_t)a.trows + 63) / 64);
+    for (uint32_t q = (blockIdx.x - a.chunk_blocks) * 4 + p.wave; q < nsets; q += a.zero_blocks * 4) {
+      // which of the 64 rows from v0 on have entries
+      const uint32_t v0 = q * 64;
+      unsigned long long there = 0;
+      uint32_t next = v0;  // rows before it are known
+      while (next - v0 < 64) {
+        // first position whose id is at least `next`, 64 probes at a time
+        uint32_t lo = 0, hi = a.n;
+        while (hi > lo) {
+          const uint32_t step = (hi - lo + 63) / 64;
+          const uint64_t at = lo + (uint64_t)p.lane * step;
+          const int small = __popcll(__ballot(at < hi && a.ids[at < hi ? at : hi - 1] < next));  // the first `small` probes are below
+          if (small == 0) {
+            hi = lo;
+          } else {
+            const uint64_t to = lo + (uint64_t)small * step;
+            lo = lo + (uint32_t)(small - 1) * step + 1;
+            hi = to < hi ? (uint32_t)to : hi;
+          }
+        }
+        const uint32_t id = lo + p.lane < a.n ? a.ids[lo + p.lane] : 0xFFFFFFFFu;
+        const bool in = id - v0 < 64 && id < a.trows;
+        unsigned long long mark = in ? 1ull << (id - v0) : 0;
+        for (int off = 1; off < 64; off <<= 1) mark |= __shfl_xor(mark, off, 64);
+        there |= mark;
+        const uint32_t last = __shfl(id, 63, 64);
+        if (last - v0 >= 64) break;  // the ids from here on are beyond the set
+        next = last + 1;
       }
-      const unsigned long long todo = __ballot(absent);
-      for (unsigned r = group; r < 64; r += groups) {
-        if (!((todo >> r) & 1) || !here) continue;
-        TO *to = a.to + (q * 64 + r) * a.tstride + col;
-        float zero[N];
+      if (!p.here) continue;
+      float zero[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k) zero[k] = 0.0f;
-        if (here == N) {
+      for (int k = 0; k < N; ++k) zero[k] = 0.0f;
+      const unsigned rows = a.trows - v0 < 64 ? a.trows - v0 : 64;
+      for (unsigned r = p.group; r < rows; r += p.groups) {
+        if ((there >> r) & 1) continue;
+        TO *to = a.to + (uint64_t)(v0 + r) * a.tstride + p.col;
+        if (p.here == N) {
           store_n<TO, N>(to, zero);
         } else {
           for (int k = 0; k < N; ++k)
-            if (k < here) to[k] = (TO)0.0f;
+            if (k < p.here) to[k] = (TO)0.0f;
         }
       }
     }
   }
 }
 
-// Runs longer than kRun: the sums of their parts, in the order of the chunks, by the block of the chunk they begin in
-// (only the run that holds a chunk's last entry can begin in it and be that long).
+// Runs that go over the end of the chunk they begin in: the sums of their parts, in the order of the chunks.  Runs of up to
+// kShort chunks after the first are summed by a group of lanes each; longer ones by a workgroup, a set of 64 chunks after
+// another looking for them.
+constexpr uint32_t kShort = 16;
+
+template <class T, class TO>
+__device__ inline bool run_leaves(const GradArgs<T, TO> &a, uint32_t c, uint32_t &id) {
+  const uint32_t b = c * a.chunk;
+  if (c + 1 >= a.nchunks) return false;
+  id = a.ids[b + a.chunk];
+  if (id >= a.trows || a.ids[b + a.chunk - 1] != id) return false;
+  return a.ids[b] != id || b == 0 || a.ids[b - 1] != id;  // and begins here
+}
+
 template <class T, class TO, int N>
-__global__ void __launch_bounds__(256) k_grad_join(GradArgs<T, TO> a) {
+__global__ void __launch_bounds__(256) k_grad_join(GradArgs<T, TO> a, unsigned short_blocks) {
   __shared__ float sh[4][64 * N];
-  const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const unsigned lanes = 1u << a.lanes_log2, groups = 64u >> a.lanes_log2;
-  const unsigned group = lane >> a.lanes_log2, sub = lane & (lanes - 1);
-  const uint64_t col = ((uint64_t)blockIdx.y * lanes + sub) * N;
-  const int here = col >= a.cols ? 0 : a.cols - col < N ? (int)(a.cols - col) : N;
-  const uint64_t nchunks = (a.n + kRun - 1) / kRun;
-  for (uint64_t c = blockIdx.x; c < nchunks; c += gridDim.x) {  // uniform over the block, so are the conditions below
-    const uint64_t p0 = c * kRun, end = p0 + kRun < a.n ? p0 + kRun : a.n;
-    const uint32_t id = a.ids[end - 1];
-    if (id >= a.trows || end >= a.n || a.ids[end] != id) continue;  // ends in this chunk
-    const bool whole = a.ids[p0] == id;
-    if (whole && p0 > 0 && a.ids[p0 - 1] == id) continue;  // began before it
-    uint64_t b = p0;
-    if (!whole) {
-      uint64_t lo = p0, hi = end;
-      while (lo < hi) {
-        const uint64_t mid = (lo + hi) >> 1;
-        if (a.ids[mid] < id) lo = mid + 1;
+  const Place<N> p(a.lanes_log2, a.cols);
+  auto add = [&](float(&acc)[N], uint32_t c, int slot) {
+    const float *from = a.parts + ((uint64_t)c * 2 + slot) * a.cols + p.col;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (k < p.here) acc[k] += from[k];
+  };
+  float acc[N];
+  if (blockIdx.x < short_blocks) {
+    for (uint64_t c = ((uint64_t)blockIdx.x * 4 + p.wave) * p.groups + p.group; c < a.nchunks; c += (uint64_t)short_blocks * 4 * p.groups) {
+      uint32_t id;
+      if (!p.here || !run_leaves(a, (uint32_t)c, id)) continue;
+      if (c + 1 + kShort < a.nchunks && a.ids[(c + 1 + kShort) * a.chunk] == id) continue;  // a long one
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[k] = 0.0f;
+      add(acc, (uint32_t)c, 1);
+      for (uint32_t q = (uint32_t)c + 1; q < a.nchunks && a.ids[(uint64_t)q * a.chunk] == id; ++q) add(acc, q, 0);
+      put_row<N>(a, id, p, acc);
+    }
+    return;
+  }
+  for (uint32_t set = blockIdx.x - short_blocks; set * 64ull < a.nchunks; set += gridDim.x - short_blocks) {
+    const uint32_t mine = set * 64 + p.lane;
+    uint32_t id = 0;
+    bool is = false;
+    if (mine + 1ull + kShort < a.nchunks && run_leaves(a, mine, id)) is = a.ids[(mine + 1ull + kShort) * a.chunk] == id;
+    for (unsigned long long todo = __ballot(is); todo; todo &= todo - 1) {  // the same in every wave
+      const int l = __ffsll(todo) - 1;
+      const uint32_t c = set * 64 + l, run = __shfl(id, l, 64);
+      // the last chunk that begins with it
+      uint32_t lo = c + 1 + kShort, hi = a.nchunks;
+      while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (a.ids[(uint64_t)mid * a.chunk] == run) lo = mid;
         else hi = mid;
       }
-      b = lo;
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[k] = 0.0f;
+      const uint32_t step = 4 * p.groups;
+      for (uint32_t q = c + p.wave * p.groups + p.group; q <= lo; q += step) add(acc, q, q == c ? 1 : 0);
+      add_groups<N>(a.lanes_log2, acc);
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < N; ++k) sh[p.wave][k * 64 + p.lane] = acc[k];
+      __syncthreads();
+      if (p.wave == 0 && p.group == 0 && p.here) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          acc[k] = (sh[0][k * 64 + p.lane] + sh[1][k * 64 + p.lane]) + (sh[2][k * 64 + p.lane] + sh[3][k * 64 + p.lane]);
+        put_row<N>(a, run, p, acc);
+      }
     }
-    if (b + kRun >= a.n || a.ids[b + kRun] != id) continue;
-    const uint64_t stop = lower_bound(a.ids, a.n, id + 1);
-    const uint64_t clast = (stop - 1) / kRun;
-    float acc[N];
-#pragma unroll
-    for (int k = 0; k < N; ++k) acc[k] = 0.0f;
-    for (uint64_t q = c + wave * groups + group; q <= clast; q += 4 * groups) {
-      const float *p = a.parts + (q * 2 + (q == c && !whole ? 1 : 0)) * a.cols + col;
-#pragma unroll
-      for (int k = 0; k < N; ++k)
-        if (k < here) acc[k] += p[k];
-    }
-    add_groups<N>(a.lanes_log2, acc);
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < N; ++k) sh[wave][k * 64 + lane] = acc[k];
-    __syncthreads();
-    if (wave == 0 && group == 0 && here) {
-#pragma unroll
-      for (int k = 0; k < N; ++k) acc[k] = (sh[0][k * 64 + lane] + sh[1][k * 64 + lane]) + (sh[2][k * 64 + lane] + sh[3][k * 64 + lane]);
-      put_row<N>(a, id, col, here, acc);
-    }
-    __syncthreads();
   }
 }
 
@@ -596,7 +702,7 @@ __global__ void __launch_bounds__(256) k_grad_join(GradArgs<T, TO> a) {
 static int check_bags(const admm_bags *b, const char *who) {
   ADMM_REQUIRE(b, "%s: bags is NULL", who);
   ADMM_REQUIRE(b->id_type == ADMM_I32 || b->id_type == ADMM_I64, "%s: ids of type %d", who, b->id_type);
-  ADMM_REQUIRE(b->nrows < 0xFFFFFFFFull && b->nnz < 0xFFFFFFFFull, "%s: %llu rows, %llu entries: fewer than 2^32 - 1 are supported",
+  ADMM_REQUIRE(b->nrows <= kMaxCount && b->nnz <= kMaxCount, "%s: %llu rows, %llu entries: at most 2^32 - 256 are supported",
                who, (unsigned long long)b->nrows, (unsigned long long)b->nnz);
   ADMM_REQUIRE(b->rowptr || b->nnz == b->nrows, "%s: %llu ids for %llu rows without row pointers", who, (unsigned long long)b->nnz,
                (unsigned long long)b->nrows);
@@ -645,10 +751,13 @@ static int check_tiles(uint64_t tiles, const char *who, uint64_t cols) {
   return ADMM_OK;
 }
 
+// Entries per tile of the sort's passes: large tiles write longer pieces side by side, small ones keep more of the GPU busy.
+static uint64_t sort_tile(uint64_t n) { return n <= (1u << 19) ? 1024 : 4096; }
+
 struct OrderLayout {
-  uint64_t ids, rows, val, row_of, keys_a, entries_a, keys_b, entries_b, counts, totals, bytes;
+  uint64_t ids, rows, val, row_of, keys_a, loads_a, keys_b, loads_b, counts, totals, bytes;
   explicit OrderLayout(const admm_bags *b) {
-    const uint64_t arr = round_up(4 * b->nnz, 256), tiles = (b->nnz + kSortTile - 1) / kSortTile;
+    const uint64_t arr = round_up(4 * b->nnz, 256), tile = sort_tile(b->nnz), tiles = (b->nnz + tile - 1) / tile;
     uint64_t at = 0;
     auto take = [&](uint64_t n) {
       const uint64_t here = at;
@@ -661,14 +770,47 @@ struct OrderLayout {
     row_of = take(b->rowptr ? arr : 0);
     const bool large = b->nnz > kSortSmall;
     keys_a = take(large ? arr : 0);
-    entries_a = take(large ? arr : 0);
+    loads_a = take(large ? (b->val ? 2 : 1) * arr : 0);
     keys_b = take(large ? arr : 0);
-    entries_b = take(large ? arr : 0);
+    loads_b = take(large ? (b->val ? 2 : 1) * arr : 0);
     counts = take(large ? round_up(4 * 256 * tiles, 256) : 0);
     totals = take(1024);
     bytes = at;
   }
 };
+
+template <class Id, class Load, int TILE>
+static int sort_large(admm_ctx *ctx, const Id *ids, uint32_t n, uint32_t trows, char *order, const OrderLayout &at, const Sorted &to) {
+  const int bits = ceil_log2((uint64_t)trows + 1);  // keys are 0 .. trows
+  auto u32 = [&](uint64_t off) { return reinterpret_cast<uint32_t *>(order + off); };
+  auto loads_at = [&](uint64_t off) { return reinterpret_cast<Load *>(order + off); };
+  const uint32_t tiles = (uint32_t)(((uint64_t)n + TILE - 1) / TILE);
+  const int passes = (bits + 7) / 8, width = (bits + passes - 1) / passes;
+  const uint32_t *keys = nullptr;
+  const Load *loads = nullptr;
+  for (int p = 0; p < passes; ++p) {
+    const int shift = p * width;
+    uint32_t *keys_to = u32(p & 1 ? at.keys_b : at.keys_a);
+    Load *loads_to = loads_at(p & 1 ? at.loads_b : at.loads_a);
+    if (p == 0)
+      hipLaunchKernelGGL((k_sort_count<Id, true, TILE>), dim3(tiles), dim3(256), 0, ctx->stream, ids, keys, n, trows, shift, width, u32(at.counts));
+    else
+      hipLaunchKernelGGL((k_sort_count<Id, false, TILE>), dim3(tiles), dim3(256), 0, ctx->stream, ids, keys, n, trows, shift, width, u32(at.counts));
+    hipLaunchKernelGGL(k_sort_scan, dim3(1u << width), dim3(256), 0, ctx->stream, u32(at.counts), tiles, u32(at.totals));
+#define ADMM_MOVE(FIRST, LAST)                                                                                                  \
+  hipLaunchKernelGGL((k_sort_move<Id, Load, FIRST, LAST, TILE>), dim3(tiles), dim3(256), 0, ctx->stream, ids, keys, loads, n, trows, \
+                     shift, width, u32(at.counts), u32(at.totals), keys_to, loads_to, to)
+    if (p == 0 && p + 1 == passes) ADMM_MOVE(true, true);
+    else if (p == 0) ADMM_MOVE(true, false);
+    else if (p + 1 == passes) ADMM_MOVE(false, true);
+    else ADMM_MOVE(false, false);
+#undef ADMM_MOVE
+    keys = keys_to;
+    loads = loads_to;
+  }
+  ADMM_HIP_CHECK(hipGetLastError());
+  return ADMM_OK;
+}
 
 template <class Id>
 static int sort_entries(admm_ctx *ctx, const admm_bags *b, uint32_t trows, char *order, const OrderLayout &at) {
@@ -680,38 +822,17 @@ static int sort_entries(admm_ctx *ctx, const admm_bags *b, uint32_t trows, char 
     hipLaunchKernelGGL(k_fill_u32, dim3(blocks_for(n, 2048, 4096)), dim3(256), 0, ctx->stream, u32(at.row_of), (uint64_t)n, 0xFFFFFFFFu);
     hipLaunchKernelGGL(k_entry_rows, dim3(blocks_for(b->nrows, 4)), dim3(256), 0, ctx->stream, b->rowptr, b->nrows, b->nnz, u32(at.row_of));
   }
-  const int bits = ceil_log2((uint64_t)trows + 1);  // keys are 0 .. trows
   if (n <= kSortSmall) {
-    constexpr size_t lds = 4 * (2 * kSortSmall + 17 * 256);
-    ADMM_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&k_sort_small<Id>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    hipLaunchKernelGGL(k_sort_small<Id>, dim3(1), dim3(1024), lds, ctx->stream, ids, n, trows, bits, to);
+    const size_t lds = 4 * (17 * 256 + 32 + 2 * (size_t)n);
+    ADMM_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&k_sort_small<Id>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                       4 * (17 * 256 + 32 + 2 * kSortSmall)));
+    hipLaunchKernelGGL(k_sort_small<Id>, dim3((n + 511) / 512), dim3(1024), lds, ctx->stream, ids, n, trows, to);
     ADMM_HIP_CHECK(hipGetLastError());
     return ADMM_OK;
   }
-  const uint32_t tiles = (n + kSortTile - 1) / kSortTile;
-  const int passes = (bits + 7) / 8, width = (bits + passes - 1) / passes;
-  const uint32_t *keys = nullptr, *entries = nullptr;
-  for (int p = 0; p < passes; ++p) {
-    const int shift = p * width;
-    uint32_t *keys_to = u32(p & 1 ? at.keys_b : at.keys_a), *entries_to = u32(p & 1 ? at.entries_b : at.entries_a);
-    if (p == 0)
-      hipLaunchKernelGGL((k_sort_count<Id, true>), dim3(tiles), dim3(256), 0, ctx->stream, ids, keys, n, trows, shift, width, u32(at.counts));
-    else
-      hipLaunchKernelGGL((k_sort_count<Id, false>), dim3(tiles), dim3(256), 0, ctx->stream, ids, keys, n, trows, shift, width, u32(at.counts));
-    hipLaunchKernelGGL(k_sort_scan, dim3(256), dim3(256), 0, ctx->stream, u32(at.counts), tiles, u32(at.totals));
-#define ADMM_MOVE(FIRST, LAST)                                                                                             \
-  hipLaunchKernelGGL((k_sort_move<Id, FIRST, LAST>), dim3(tiles), dim3(256), 0, ctx->stream, ids, keys, entries, n, trows, \
-                     shift, width, u32(at.counts), u32(at.totals), keys_to, entries_to, to)
-    if (p == 0 && p + 1 == passes) ADMM_MOVE(true, true);
-    else if (p == 0) ADMM_MOVE(true, false);
-    else if (p + 1 == passes) ADMM_MOVE(false, true);
-    else ADMM_MOVE(false, false);
-#undef ADMM_MOVE
-    keys = keys_to;
-    entries = entries_to;
-  }
-  ADMM_HIP_CHECK(hipGetLastError());
-  return ADMM_OK;
+  if (sort_tile(n) == 1024)
+    return b->val ? sort_large<Id, unsigned long long, 1024>(ctx, ids, n, trows, order, at, to) : sort_large<Id, uint32_t, 1024>(ctx, ids, n, trows, order, at, to);
+  return b->val ? sort_large<Id, unsigned long long, 4096>(ctx, ids, n, trows, order, at, to) : sort_large<Id, uint32_t, 4096>(ctx, ids, n, trows, order, at, to);
 }
 
 template <class Id>
@@ -749,7 +870,13 @@ static int embed(admm_ctx *ctx, const admm_bags *b, const admm_mat *table, float
   });
 }
 
-static uint64_t grad_parts_bytes(uint64_t nnz, uint64_t cols) { return (nnz + kRun - 1) / kRun * 2 * cols * sizeof(float); }
+// Entries per chunk: short chunks keep the GPU busy where there are few entries; every chunk may write two rows of floats, so
+// they are longer where there are enough.
+static uint64_t grad_chunk(uint64_t nnz) { return nnz <= (1u << 15) ? 8 : nnz <= (1u << 18) ? 16 : 32; }
+
+static uint64_t grad_parts_bytes(uint64_t nnz, uint64_t cols) {
+  return (nnz + grad_chunk(nnz) - 1) / grad_chunk(nnz) * 2 * cols * sizeof(float);
+}
 
 static int embed_grad(admm_ctx *ctx, const admm_bags *b, const char *order, const admm_mat *from, float scale, int accumulate,
                       const admm_mat *to, float *parts) {
@@ -767,25 +894,29 @@ static int embed_grad(admm_ctx *ctx, const admm_bags *b, const char *order, cons
     a.ids = reinterpret_cast<const uint32_t *>(order + at.ids);
     a.rows = reinterpret_cast<const uint32_t *>(order + at.rows);
     a.val = b->val ? reinterpret_cast<const float *>(order + at.val) : nullptr;
-    a.n = b->nnz;
+    a.n = (uint32_t)b->nnz;
     a.from = static_cast<const T *>(from->data);
     a.fstride = from->stride;
     a.frows = b->nrows;
     a.to = static_cast<TO *>(to->data);
     a.tstride = to->stride;
-    a.trows = to->rows;
+    a.trows = (uint32_t)to->rows;
     a.cols = from->cols;
     a.scale = scale;
     a.accumulate = accumulate != 0;
     a.lanes_log2 = lanes;
+    a.chunk = (uint32_t)grad_chunk(b->nnz);
+    a.nchunks = (uint32_t)((b->nnz + a.chunk - 1) / a.chunk);
     a.parts = parts;
-    a.chunk_blocks = b->nnz > kRun ? blocks_for(b->nnz, 4 * kRun) : 0;  // a run longer than kRun needs more entries than that
-    a.run_blocks = b->nnz ? blocks_for(b->nnz, 4u * (64u >> lanes)) : 0;
+    const unsigned groups = 4u * (64u >> lanes);
+    a.chunk_blocks = a.nchunks ? blocks_for(a.nchunks, groups) : 0;
     a.zero_blocks = accumulate ? 0 : blocks_for(to->rows, 256);
-    if (a.chunk_blocks + a.run_blocks + a.zero_blocks == 0) return ADMM_OK;
-    hipLaunchKernelGGL((k_grad<T, TO, N>), dim3(a.chunk_blocks + a.run_blocks + a.zero_blocks, (unsigned)tiles), dim3(256), 0, ctx->stream, a);
-    if (a.chunk_blocks)
-      hipLaunchKernelGGL((k_grad_join<T, TO, N>), dim3(blocks_for(b->nnz, kRun), (unsigned)tiles), dim3(256), 0, ctx->stream, a);
+    if (a.chunk_blocks + a.zero_blocks == 0) return ADMM_OK;
+    hipLaunchKernelGGL((k_grad<T, TO, N>), dim3(a.chunk_blocks + a.zero_blocks, (unsigned)tiles), dim3(256), 0, ctx->stream, a);
+    if (a.nchunks > 1) {
+      const unsigned short_blocks = blocks_for(a.nchunks, groups), long_blocks = a.nchunks > kShort + 1 ? blocks_for(a.nchunks, 64) : 0;
+      hipLaunchKernelGGL((k_grad_join<T, TO, N>), dim3(short_blocks + long_blocks, (unsigned)tiles), dim3(256), 0, ctx->stream, a, short_blocks);
+    }
     ADMM_HIP_CHECK(hipGetLastError());
     return ADMM_OK;
   });
@@ -802,7 +933,7 @@ extern "C" int admm_csr_bags(const admm_csr *csr, admm_bags *out) {
     set_error("admm_csr_bags: the set is relabelled: its stored ids are frequency ranks");
     return ADMM_ERR_STATE;
   }
-  ADMM_REQUIRE(csr->nnz < 0xFFFFFFFFull, "admm_csr_bags: %llu entries: fewer than 2^32 - 1 are supported", (unsigned long long)csr->nnz);
+  ADMM_REQUIRE(csr->nnz <= kMaxCount, "admm_csr_bags: %llu entries: at most 2^32 - 256 are supported", (unsigned long long)csr->nnz);
   out->ids = csr->d_col;
   out->rowptr = csr->d_rowptr;
   out->val = csr->d_val;
@@ -817,7 +948,7 @@ extern "C" int admm_embed(admm_ctx *ctx, const admm_bags *bags, const admm_mat *
   ADMM_TRY(check_bags(bags, "admm_embed"));
   ADMM_TRY(check_mat(table, "admm_embed", "table"));
   ADMM_TRY(check_mat(out, "admm_embed", "out"));
-  ADMM_REQUIRE(table->rows > 0 && table->rows < 0xFFFFFFFFull, "admm_embed: a table of %llu rows", (unsigned long long)table->rows);
+  ADMM_REQUIRE(table->rows > 0 && table->rows <= kMaxCount, "admm_embed: a table of %llu rows", (unsigned long long)table->rows);
   ADMM_REQUIRE(out->cols == table->cols && out->rows >= bags->nrows, "admm_embed: out is %llu x %llu for %llu rows of %llu columns",
                (unsigned long long)out->rows, (unsigned long long)out->cols, (unsigned long long)bags->nrows, (unsigned long long)table->cols);
   ADMM_REQUIRE(out->type == table->type || out->type == ADMM_F32, "admm_embed: out has the table's type or ADMM_F32");
@@ -832,7 +963,7 @@ extern "C" int admm_embed(admm_ctx *ctx, const admm_bags *bags, const admm_mat *
 extern "C" int admm_embed_order_bytes(const admm_bags *bags, uint64_t table_rows, uint64_t *bytes) {
   ADMM_REQUIRE(bytes, "admm_embed_order_bytes: bytes is NULL");
   ADMM_TRY(check_bags(bags, "admm_embed_order_bytes"));
-  ADMM_REQUIRE(table_rows > 0 && table_rows < 0xFFFFFFFFull, "admm_embed_order_bytes: a table of %llu rows", (unsigned long long)table_rows);
+  ADMM_REQUIRE(table_rows > 0 && table_rows <= kMaxCount, "admm_embed_order_bytes: a table of %llu rows", (unsigned long long)table_rows);
   *bytes = OrderLayout(bags).bytes;
   return ADMM_OK;
 }
@@ -857,7 +988,7 @@ extern "C" int admm_embed_grad_workspace(const admm_bags *bags, uint64_t cols, u
   ADMM_REQUIRE(bytes, "admm_embed_grad_workspace: bytes is NULL");
   ADMM_TRY(check_bags(bags, "admm_embed_grad_workspace"));
   ADMM_REQUIRE(cols < (1ull << 40), "admm_embed_grad_workspace: %llu columns", (unsigned long long)cols);
-  *bytes = bags->nnz > kRun ? grad_parts_bytes(bags->nnz, cols) : 0;
+  *bytes = bags->nnz > grad_chunk(bags->nnz) ? grad_parts_bytes(bags->nnz, cols) : 0;
   return ADMM_OK;
 }
 
@@ -867,7 +998,7 @@ extern "C" int admm_embed_grad(admm_ctx *ctx, const admm_bags *bags, const void 
   ADMM_TRY(check_bags(bags, "admm_embed_grad"));
   ADMM_TRY(check_mat(grad_out, "admm_embed_grad", "grad_out"));
   ADMM_TRY(check_mat(grad_table, "admm_embed_grad", "grad_table"));
-  ADMM_REQUIRE(grad_table->rows > 0 && grad_table->rows < 0xFFFFFFFFull, "admm_embed_grad: a table of %llu rows",
+  ADMM_REQUIRE(grad_table->rows > 0 && grad_table->rows <= kMaxCount, "admm_embed_grad: a table of %llu rows",
                (unsigned long long)grad_table->rows);
   ADMM_REQUIRE(grad_out->cols == grad_table->cols && grad_out->rows >= bags->nrows,
                "admm_embed_grad: grad_out is %llu x %llu for %llu rows of %llu columns", (unsigned long long)grad_out->rows,

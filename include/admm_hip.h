@@ -329,7 +329,7 @@ typedef struct admm_mat {
 /* Rows of ids in DEVICE memory.  rowptr == NULL: one id per row (tokens), nnz == nrows.  Else row r holds the entries
  * [rowptr[r], rowptr[r+1]) (a sample set's rows; a row may be empty; what lies beyond nnz is not read).  An id outside
  * the table (-1 in a padded batch) stands for nothing: it adds zero and receives no gradient.
- * Limits: nrows, nnz and the table's rows below 2^32 - 1. */
+ * Limits: nrows, nnz and the table's rows at most 2^32 - 256. */
 typedef struct admm_bags {
   const void *ids;
   const uint64_t *rowptr;
