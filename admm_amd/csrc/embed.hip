@@ -172,16 +172,19 @@ __device__ inline void rank_items(const uint32_t (&digit)[ITEMS], uint32_t (&ran
   }
 }
 
-// counters[wave][digit] -> first place of that wave's items with that digit, counted from `from(digit)`; one thread a digit
-template <int WAVES, class From>
-__device__ inline void waves_before(uint32_t *counters, From from) {
+// counters[wave][digit] -> the items with that digit in the waves before; their sum to totals; one thread a digit
+template <int WAVES>
+__device__ inline void totals_of_waves(uint32_t *counters, uint32_t *totals) {
   if (threadIdx.x < 256) {
-    uint32_t sum = from(threadIdx.x);
+    uint32_t n[WAVES], sum = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) n[w] = counters[w * 256 + threadIdx.x];
+#pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-      const uint32_t n = counters[w * 256 + threadIdx.x];
       counters[w * 256 + threadIdx.x] = sum;
-      sum += n;
+      sum += n[w];
     }
+    totals[threadIdx.x] = sum;
   }
 }
 
@@ -283,19 +286,13 @@ __global__ void __launch_bounds__(1024) k_sort_small(const Id *__restrict__ ids,
     __syncthreads();
     rank_items<kItems>(digit, rank, items, digits, counters + wave * 256);
     __syncthreads();
-    if (threadIdx.x < 256) {
-      uint32_t s = 0;
-      for (int w = 0; w < 16; ++w) s += counters[w * 256 + threadIdx.x];
-      totals[threadIdx.x] = s;
-    }
+    totals_of_waves<16>(counters, totals);
     scan_256(totals);
-    waves_before<16>(counters, [&](int d) { return totals[d]; });
-    __syncthreads();
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       if (i >= items) break;
       // the padding's digit is the largest and it comes behind everything: its places are `count` and beyond
-      const uint32_t at = counters[wave * 256 + digit[i]] + rank[i];
+      const uint32_t at = totals[digit[i]] + counters[wave * 256 + digit[i]] + rank[i];
       if (at >= count) continue;
       keys[at] = key[i];
       entries[at] = entry[i];
@@ -404,16 +401,15 @@ __global__ void __launch_bounds__(256) k_sort_move(const Id *__restrict__ ids, c
   scan_256(start);
   rank_items<kItems>(digit, rank, kItems, width, counters + wave * 256);
   __syncthreads();
-  local[threadIdx.x] = counters[threadIdx.x] + counters[256 + threadIdx.x] + counters[512 + threadIdx.x] + counters[768 + threadIdx.x];
+  totals_of_waves<4>(counters, local);
   scan_256(local);
-  waves_before<4>(counters, [&](int d) { return local[d]; });
   // a digit's place in the whole, less its place in the tile
   if (threadIdx.x <= mask) start[threadIdx.x] += counts[(uint64_t)threadIdx.x * gridDim.x + blockIdx.x] - local[threadIdx.x];
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
     // what pads the last tile has the last digit and comes behind everything: its places are `count` and beyond
-    const uint32_t at = counters[wave * 256 + digit[i]] + rank[i];
+    const uint32_t at = local[digit[i]] + counters[wave * 256 + digit[i]] + rank[i];
     tile_keys[at] = key[i];
     tile_loads[at] = load[i];
   }
@@ -518,30 +514,45 @@ template <class T, class TO, int N>
 __global__ void __launch_bounds__(256) k_grad(GradArgs<T, TO> a) {
   const Place<N> p(a.lanes_log2, a.cols);
   if (blockIdx.x < a.chunk_blocks) {
+    // The workgroup's chunks lie side by side: their entries come through LDS, read in one piece.  (Every lane of a group
+    // reading its entry from memory cost as much address work as the rows themselves, 81 us for 2.6 million entries of 16 floats.)
+    extern __shared__ uint32_t stage[];
     constexpr int kAhead = 4;
-    for (uint64_t c = ((uint64_t)blockIdx.x * 4 + p.wave) * p.groups + p.group; c < a.nchunks; c += (uint64_t)a.chunk_blocks * 4 * p.groups) {
-      const uint32_t b = (uint32_t)c * a.chunk, end = a.n - b < a.chunk ? a.n : b + a.chunk;
-      uint32_t cur = a.ids[b];
+    const uint32_t per = 4 * p.groups, pitch = a.chunk + 1;  // one word more, so that the groups' words fall on different banks
+    uint32_t *const ids = stage, *const rows = ids + per * pitch;
+    float *const val = reinterpret_cast<float *>(rows + per * pitch);
+    const uint32_t mine = (p.wave * p.groups + p.group) * pitch;
+    for (uint64_t c0 = (uint64_t)blockIdx.x * per; c0 < a.nchunks; c0 += (uint64_t)a.chunk_blocks * per) {
+      const uint64_t first = c0 * a.chunk;
+      const uint32_t here = (uint32_t)(a.n - first < (uint64_t)per * a.chunk ? a.n - first : (uint64_t)per * a.chunk);
+      __syncthreads();
+      for (uint32_t i = threadIdx.x; i < here; i += 256) {
+        const uint32_t at = i / a.chunk * pitch + i % a.chunk;
+        ids[at] = a.ids[first + i];
+        rows[at] = a.rows[first + i];
+        if (a.val) val[at] = a.val[first + i];
+      }
+      __syncthreads();
+      const uint64_t c = c0 + p.wave * p.groups + p.group;
+      if (c >= a.nchunks) continue;
+      const uint32_t b = (uint32_t)(c * a.chunk), count = a.n - b < a.chunk ? a.n - b : a.chunk;
+      uint32_t cur = ids[mine];
       bool open = b > 0 && a.ids[b - 1] == cur;
       float acc[N];
 #pragma unroll
       for (int k = 0; k < N; ++k) acc[k] = 0.0f;
-      for (uint32_t e = b; e < end; e += kAhead) {
+      for (uint32_t e = 0; e < count; e += kAhead) {
         float v[kAhead][N], f[kAhead];
-        uint32_t id[kAhead], row[kAhead];
+        uint32_t id[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-          const uint32_t at = end - e > (uint32_t)u ? e + u : end - 1;
-          id[u] = a.ids[at];
-          row[u] = a.rows[at];
-          f[u] = a.val ? a.val[at] : 1.0f;
-        }
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
+          const uint32_t at = mine + (e + u < count ? e + u : count - 1), row = rows[at];
+          id[u] = ids[at];
+          f[u] = a.val ? val[at] : 1.0f;
           // an entry without a row, a row beyond grad_out (of an order that is not these bags'), the chunk's end
-          if (row[u] >= a.frows || end - e <= (uint32_t)u || id[u] >= a.trows) f[u] = 0.0f;
+          if (row >= a.frows || e + u >= count || id[u] >= a.trows) f[u] = 0.0f;
           if (f[u] == 0.0f) continue;
-          const T *from = a.from + row[u] * a.fstride + p.col;
+          const T *from = a.from + row * a.fstride + p.col;
           if (p.here == N) {
             load_n<T, N>(from, v[u]);
           } else {
@@ -554,7 +565,7 @@ __global__ void __launch_bounds__(256) k_grad(GradArgs<T, TO> a) {
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-          if (end - e <= (uint32_t)u) continue;
+          if (e + u >= count) continue;
           if (id[u] != cur) {
             if (cur < a.trows && p.here) {
               if (open) put_part<N>(a, (uint32_t)c, 0, p, acc);
@@ -572,7 +583,7 @@ __global__ void __launch_bounds__(256) k_grad(GradArgs<T, TO> a) {
       }
       if (cur >= a.trows || !p.here) continue;
       if (open) put_part<N>(a, (uint32_t)c, 0, p, acc);
-      else if (end < a.n && a.ids[end] == cur) put_part<N>(a, (uint32_t)c, 1, p, acc);
+      else if (b + count < a.n && a.ids[b + count] == cur) put_part<N>(a, (uint32_t)c, 1, p, acc);
       else put_row<N>(a, cur, p, acc);
     }
   } else {
@@ -626,9 +637,9 @@ __global__ void __launch_bounds__(256) k_grad(GradArgs<T, TO> a) {
 }
 
 // Runs that go over the end of the chunk they begin in: the sums of their parts, in the order of the chunks.  Runs of up to
-// kShort chunks after the first are summed by a group of lanes each; longer ones by a workgroup, a set of 64 chunks after
-// another looking for them.
-constexpr uint32_t kShort = 16;
+// kShort chunks after the first are summed by a group of lanes each; longer ones by a workgroup, which looks for them in
+// kSet chunks at a time.
+constexpr int kShort = 7, kSet = 16;
 
 template <class T, class TO>
 __device__ inline bool run_leaves(const GradArgs<T, TO> &a, uint32_t c, uint32_t &id) {
@@ -654,23 +665,28 @@ __global__ void __launch_bounds__(256) k_grad_join(GradArgs<T, TO> a, unsigned s
     for (uint64_t c = ((uint64_t)blockIdx.x * 4 + p.wave) * p.groups + p.group; c < a.nchunks; c += (uint64_t)short_blocks * 4 * p.groups) {
       uint32_t id;
       if (!p.here || !run_leaves(a, (uint32_t)c, id)) continue;
-      if (c + 1 + kShort < a.nchunks && a.ids[(c + 1 + kShort) * a.chunk] == id) continue;  // a long one
+      int more = 0;  // chunks after the first; the ids are sorted, so these are its
+#pragma unroll
+      for (int i = 1; i <= kShort + 1; ++i) more += c + i < a.nchunks && a.ids[(c + i) * a.chunk] == id;
+      if (more > kShort) continue;  // a long one
 #pragma unroll
       for (int k = 0; k < N; ++k) acc[k] = 0.0f;
       add(acc, (uint32_t)c, 1);
-      for (uint32_t q = (uint32_t)c + 1; q < a.nchunks && a.ids[(uint64_t)q * a.chunk] == id; ++q) add(acc, q, 0);
+#pragma unroll
+      for (int i = 1; i <= kShort; ++i)
+        if (i <= more) add(acc, (uint32_t)c + i, 0);
       put_row<N>(a, id, p, acc);
     }
     return;
   }
-  for (uint32_t set = blockIdx.x - short_blocks; set * 64ull < a.nchunks; set += gridDim.x - short_blocks) {
-    const uint32_t mine = set * 64 + p.lane;
+  for (uint32_t set = blockIdx.x - short_blocks; (uint64_t)set * kSet < a.nchunks; set += gridDim.x - short_blocks) {
+    const uint32_t mine = set * kSet + p.lane;
     uint32_t id = 0;
     bool is = false;
-    if (mine + 1ull + kShort < a.nchunks && run_leaves(a, mine, id)) is = a.ids[(mine + 1ull + kShort) * a.chunk] == id;
+    if (p.lane < kSet && mine + 1ull + kShort < a.nchunks && run_leaves(a, mine, id)) is = a.ids[(mine + 1ull + kShort) * a.chunk] == id;
     for (unsigned long long todo = __ballot(is); todo; todo &= todo - 1) {  // the same in every wave
       const int l = __ffsll(todo) - 1;
-      const uint32_t c = set * 64 + l, run = __shfl(id, l, 64);
+      const uint32_t c = set * kSet + l, run = __shfl(id, l, 64);
       // the last chunk that begins with it
       uint32_t lo = c + 1 + kShort, hi = a.nchunks;
       while (hi - lo > 1) {
@@ -681,6 +697,7 @@ __global__ void __launch_bounds__(256) k_grad_join(GradArgs<T, TO> a, unsigned s
 #pragma unroll
       for (int k = 0; k < N; ++k) acc[k] = 0.0f;
       const uint32_t step = 4 * p.groups;
+#pragma unroll 4
       for (uint32_t q = c + p.wave * p.groups + p.group; q <= lo; q += step) add(acc, q, q == c ? 1 : 0);
       add_groups<N>(a.lanes_log2, acc);
       __syncthreads();
@@ -752,7 +769,7 @@ static int check_tiles(uint64_t tiles, const char *who, uint64_t cols) {
 }
 
 // Entries per tile of the sort's passes: large tiles write longer pieces side by side, small ones keep more of the GPU busy.
-static uint64_t sort_tile(uint64_t n) { return n <= (1u << 19) ? 1024 : 4096; }
+static uint64_t sort_tile(uint64_t n) { return n <= (1u << 19) ? 1024 : 2048; }
 
 struct OrderLayout {
   uint64_t ids, rows, val, row_of, keys_a, loads_a, keys_b, loads_b, counts, totals, bytes;
@@ -832,7 +849,7 @@ static int sort_entries(admm_ctx *ctx, const admm_bags *b, uint32_t trows, char 
   }
   if (sort_tile(n) == 1024)
     return b->val ? sort_large<Id, unsigned long long, 1024>(ctx, ids, n, trows, order, at, to) : sort_large<Id, uint32_t, 1024>(ctx, ids, n, trows, order, at, to);
-  return b->val ? sort_large<Id, unsigned long long, 4096>(ctx, ids, n, trows, order, at, to) : sort_large<Id, uint32_t, 4096>(ctx, ids, n, trows, order, at, to);
+  return b->val ? sort_large<Id, unsigned long long, 2048>(ctx, ids, n, trows, order, at, to) : sort_large<Id, uint32_t, 2048>(ctx, ids, n, trows, order, at, to);
 }
 
 template <class Id>
@@ -912,9 +929,12 @@ static int embed_grad(admm_ctx *ctx, const admm_bags *b, const char *order, cons
     a.chunk_blocks = a.nchunks ? blocks_for(a.nchunks, groups) : 0;
     a.zero_blocks = accumulate ? 0 : blocks_for(to->rows, 256);
     if (a.chunk_blocks + a.zero_blocks == 0) return ADMM_OK;
-    hipLaunchKernelGGL((k_grad<T, TO, N>), dim3(a.chunk_blocks + a.zero_blocks, (unsigned)tiles), dim3(256), 0, ctx->stream, a);
+    const size_t lds = (size_t)groups * (a.chunk + 1) * (b->val ? 12 : 8);
+    if (lds > 64 * 1024)
+      ADMM_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&k_grad<T, TO, N>), hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
+    hipLaunchKernelGGL((k_grad<T, TO, N>), dim3(a.chunk_blocks + a.zero_blocks, (unsigned)tiles), dim3(256), lds, ctx->stream, a);
     if (a.nchunks > 1) {
-      const unsigned short_blocks = blocks_for(a.nchunks, groups), long_blocks = a.nchunks > kShort + 1 ? blocks_for(a.nchunks, 64) : 0;
+      const unsigned short_blocks = blocks_for(a.nchunks, groups), long_blocks = a.nchunks > kShort + 1 ? blocks_for(a.nchunks, kSet) : 0;
       hipLaunchKernelGGL((k_grad_join<T, TO, N>), dim3(short_blocks + long_blocks, (unsigned)tiles), dim3(256), 0, ctx->stream, a, short_blocks);
     }
     ADMM_HIP_CHECK(hipGetLastError());
