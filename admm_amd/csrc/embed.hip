@@ -458,7 +458,8 @@ struct GradArgs {
   float scale;
   int accumulate, lanes_log2;
   uint32_t chunk, nchunks;  // entries per chunk
-  float *parts;             // [chunk][2][cols]
+  float *parts;             // [chunk][2][pitch]
+  uint64_t pitch;           // cols, to a multiple of 8
   unsigned chunk_blocks, zero_blocks;
 };
 
@@ -498,10 +499,7 @@ __device__ inline void put_row(const GradArgs<T, TO> &a, uint32_t id, const Plac
 
 template <int N, class T, class TO>
 __device__ inline void put_part(const GradArgs<T, TO> &a, uint32_t chunk, int slot, const Place<N> &p, const float (&acc)[N]) {
-  float *to = a.parts + ((uint64_t)chunk * 2 + slot) * a.cols + p.col;
-#pragma unroll
-  for (int k = 0; k < N; ++k)
-    if (k < p.here) to[k] = acc[k];
+  store_n<float, N>(a.parts + ((uint64_t)chunk * 2 + slot) * a.pitch + p.col, acc);  // columns beyond cols are the pitch's
 }
 
 // Two kinds of blocks, every one over one tile of columns (blockIdx.y):
@@ -643,11 +641,11 @@ constexpr int kShort = 7, kSet = 16;
 
 template <class T, class TO>
 __device__ inline bool run_leaves(const GradArgs<T, TO> &a, uint32_t c, uint32_t &id) {
-  const uint32_t b = c * a.chunk;
   if (c + 1 >= a.nchunks) return false;
+  const uint32_t b = c * a.chunk;
   id = a.ids[b + a.chunk];
-  if (id >= a.trows || a.ids[b + a.chunk - 1] != id) return false;
-  return a.ids[b] != id || b == 0 || a.ids[b - 1] != id;  // and begins here
+  const uint32_t last = a.ids[b + a.chunk - 1], first = a.ids[b], before = a.ids[b ? b - 1 : 0];  // all at once
+  return id < a.trows && last == id && (first != id || b == 0 || before != id);  // goes on, and begins here
 }
 
 template <class T, class TO, int N>
@@ -655,10 +653,10 @@ __global__ void __launch_bounds__(256) k_grad_join(GradArgs<T, TO> a, unsigned s
   __shared__ float sh[4][64 * N];
   const Place<N> p(a.lanes_log2, a.cols);
   auto add = [&](float(&acc)[N], uint32_t c, int slot) {
-    const float *from = a.parts + ((uint64_t)c * 2 + slot) * a.cols + p.col;
+    float v[N];
+    load_n<float, N>(a.parts + ((uint64_t)c * 2 + slot) * a.pitch + p.col, v);
 #pragma unroll
-    for (int k = 0; k < N; ++k)
-      if (k < p.here) acc[k] += from[k];
+    for (int k = 0; k < N; ++k) acc[k] += v[k];
   };
   float acc[N];
   if (blockIdx.x < short_blocks) {
@@ -687,18 +685,22 @@ __global__ void __launch_bounds__(256) k_grad_join(GradArgs<T, TO> a, unsigned s
     for (unsigned long long todo = __ballot(is); todo; todo &= todo - 1) {  // the same in every wave
       const int l = __ffsll(todo) - 1;
       const uint32_t c = set * kSet + l, run = __shfl(id, l, 64);
-      // the last chunk that begins with it
+      // the last chunk that begins with it, 64 probes at a time
       uint32_t lo = c + 1 + kShort, hi = a.nchunks;
       while (hi - lo > 1) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if (a.ids[(uint64_t)mid * a.chunk] == run) lo = mid;
-        else hi = mid;
+        const uint32_t step = (hi - lo + 63) / 64;
+        const uint64_t at = lo + (uint64_t)p.lane * step;
+        const int is_run = __popcll(__ballot(at < hi && a.ids[(at < hi ? at : lo) * a.chunk] == run));  // the first one is
+        const uint64_t to = lo + (uint64_t)is_run * step;
+        lo += (uint32_t)(is_run - 1) * step;
+        hi = to < hi ? (uint32_t)to : hi;
       }
 #pragma unroll
       for (int k = 0; k < N; ++k) acc[k] = 0.0f;
       const uint32_t step = 4 * p.groups;
+      if (p.here)
 #pragma unroll 4
-      for (uint32_t q = c + p.wave * p.groups + p.group; q <= lo; q += step) add(acc, q, q == c ? 1 : 0);
+        for (uint32_t q = c + p.wave * p.groups + p.group; q <= lo; q += step) add(acc, q, q == c ? 1 : 0);
       add_groups<N>(a.lanes_log2, acc);
       __syncthreads();
 #pragma unroll
@@ -892,7 +894,7 @@ static int embed(admm_ctx *ctx, const admm_bags *b, const admm_mat *table, float
 static uint64_t grad_chunk(uint64_t nnz) { return nnz <= (1u << 15) ? 8 : nnz <= (1u << 18) ? 16 : 32; }
 
 static uint64_t grad_parts_bytes(uint64_t nnz, uint64_t cols) {
-  return (nnz + grad_chunk(nnz) - 1) / grad_chunk(nnz) * 2 * cols * sizeof(float);
+  return (nnz + grad_chunk(nnz) - 1) / grad_chunk(nnz) * 2 * round_up(cols, 8) * sizeof(float);
 }
 
 static int embed_grad(admm_ctx *ctx, const admm_bags *b, const char *order, const admm_mat *from, float scale, int accumulate,
@@ -925,6 +927,7 @@ static int embed_grad(admm_ctx *ctx, const admm_bags *b, const char *order, cons
     a.chunk = (uint32_t)grad_chunk(b->nnz);
     a.nchunks = (uint32_t)((b->nnz + a.chunk - 1) / a.chunk);
     a.parts = parts;
+    a.pitch = round_up(from->cols, 8);
     const unsigned groups = 4u * (64u >> lanes);
     a.chunk_blocks = a.nchunks ? blocks_for(a.nchunks, groups) : 0;
     a.zero_blocks = accumulate ? 0 : blocks_for(to->rows, 256);
