@@ -170,45 +170,81 @@ __device__ inline float block_sum(float v, float *sh) {
   return v;
 }
 
-// Rows of any length, one workgroup each, CH chunks a thread kept in registers (CH > 0) or read again (CH == 0).
+// The elements of a row outside its whole granules: up to kPer - 1 at either end, one to each of the first threads.
+template <class T>
+struct Edges {
+  int head, tail_from, count;
+  __device__ explicit Edges(const Chunks<T> &row) {
+    const int before = row.whole_from ? Chunks<T>::kPer - row.lead : 0;
+    head = before < row.cols ? before : row.cols;
+    const int after = row.column(row.whole_to, 0);
+    tail_from = after > head ? after : head;
+    count = head + row.cols - tail_from;
+  }
+  __device__ int column(int i) const { return i < head ? i : tail_from + i - head; }
+};
+
+// Rows of any length, one workgroup each: whole granules, CH a thread, kept in registers (CH > 0) or read again (CH == 0), and
+// the edges' elements one a thread.
 template <class T, int NT, int CH>
 __global__ void __launch_bounds__(NT) k_softmax_block(SoftmaxArgs a) {
   constexpr int K = 16 / sizeof(T);
+  typedef vec_t<T, K> chunk;
   __shared__ float sh[2][NT / 64];
   const T none = (T)-INFINITY;
+  const int tid = (int)threadIdx.x;
   for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     float w;
     const int64_t t = label_of(a, r, w);
     const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int)a.cols);
-    T *to = a.grad ? static_cast<T *>(a.grad) + r * a.gstride : nullptr;
-    const vec_t<T, K> zero = (T)0.0f;
+    const Edges<T> edges(row);
+    const T *const from = row.base + row.lead;
+    T *const to = a.grad ? static_cast<T *>(a.grad) + r * a.gstride : nullptr;
+    const chunk *const in = reinterpret_cast<const chunk *>(row.base) + row.whole_from;
+    const int count = row.whole_to - row.whole_from;  // may be negative: then all elements are edges
+    auto put = [&](int c, const chunk &x) {
+      if (!a.apart) {
+        reinterpret_cast<chunk *>(to - row.lead)[row.whole_from + c] = x;
+      } else {
+#pragma unroll
+        for (int k = 0; k < K; ++k) to[row.column(row.whole_from + c, k)] = x[k];
+      }
+    };
+    const chunk zero = (T)0.0f;
     if (t < 0 && !a.lse) {  // nothing of the row is needed
-      if (to)
-        for (int c = threadIdx.x; c < row.count; c += NT) row.store(to, a.apart, c, zero);
-      if (threadIdx.x == 0) a.loss[r] = 0.0f;
+      if (to) {
+        for (int c = tid; c < count; c += NT) put(c, zero);
+        if (tid < edges.count) to[edges.column(tid)] = (T)0.0f;
+      }
+      if (tid == 0) a.loss[r] = 0.0f;
       continue;
     }
-    const float xt = t >= 0 ? (float)row.base[row.lead + t] : 0.0f;  // before anyone writes over it
-    vec_t<T, K> x[CH ? CH : 1];
-    float m = -INFINITY, s = 0.0f;
+    const float xt = t >= 0 ? (float)from[t] : 0.0f;  // before anyone writes over it
+    const float edge = tid < edges.count ? (float)from[edges.column(tid)] : -INFINITY;
+    chunk x[CH ? CH : 1];
+    float m = edge, s;
     Shift b(m);
     if (CH) {
 #pragma unroll
-      for (int c = 0; c < CH; ++c)
-        if (c * NT + (int)threadIdx.x < row.count) x[c] = row.load(c * NT + threadIdx.x, none);
-        else x[c] = none;
+      for (int c = 0; c < CH; ++c) {
+        x[c] = none;
+        if (c * NT + tid < count) x[c] = in[c * NT + tid];
+      }
 #pragma unroll
       for (int c = 0; c < CH; ++c) m = chunk_max<T>(x[c], m);
       m = block_max<NT>(m, sh[0]);
       b = Shift(m);
+      s = exp2_fast(__fmaf_rn(edge, b.l, -b.m2));
 #pragma unroll
-      for (int c = 0; c < CH; ++c) stay_packed(x[c]);
-#pragma unroll
-      for (int c = 0; c < CH; ++c) s += chunk_sum<T>(x[c], b);
+      for (int c = 0; c < CH; ++c) {
+        stay_packed(x[c]);
+        s += chunk_sum<T>(x[c], b);
+      }
     } else {
       // one pass: the sum is kept relative to the running maximum
-      for (int c = threadIdx.x; c < row.count; c += NT) {
-        const vec_t<T, K> y = row.load(c, none);
+      s = exp2_fast(__fmaf_rn(edge, b.l, -b.m2));
+      for (int c = tid; c < count; c += NT) {
+        const chunk y = in[c];
         const float mc = chunk_max<T>(y, m);
         if (mc > m) {
           const Shift next(mc);
@@ -225,22 +261,24 @@ __global__ void __launch_bounds__(NT) k_softmax_block(SoftmaxArgs a) {
     }
     s = block_sum<NT>(s, sh[1]);
     float lse2;
-    finish_row(a, r, b, s, t, w, xt, threadIdx.x == 0, lse2);
+    finish_row(a, r, b, s, t, w, xt, tid == 0, lse2);
     if (to) {
       const float g = t < 0 ? 0.0f : w * a.grad_scale;
-      const int tc = t < 0 ? -1 : (int)t + row.lead;
+      const int tc = t < 0 ? -1 : (int)t + row.lead - row.whole_from * K;
       const bool no = t < 0 || s == 0.0f;
+      if (tid < edges.count) {
+        const int j = edges.column(tid);
+        to[j] = no ? (T)0.0f : (T)(g * exp2_fast(__fmaf_rn(edge, b.l, -lse2)) - (j == (int)t ? g : 0.0f));
+      }
       if (CH) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) stay_packed(x[c]);
-#pragma unroll
         for (int c = 0; c < CH; ++c) {
-          const int at = c * NT + (int)threadIdx.x;
-          if (at < row.count) row.store(to, a.apart, at, no ? zero : chunk_grad<T>(x[c], b.l, lse2, g, tc - at * K));
+          const int at = c * NT + tid;
+          stay_packed(x[c]);
+          if (at < count) put(at, no ? zero : chunk_grad<T>(x[c], b.l, lse2, g, tc - at * K));
         }
       } else {
-        for (int c = threadIdx.x; c < row.count; c += NT)
-          row.store(to, a.apart, c, no ? zero : chunk_grad<T>(row.load(c, none), b.l, lse2, g, tc - c * K));
+        for (int c = tid; c < count; c += NT) put(c, no ? zero : chunk_grad<T>(in[c], b.l, lse2, g, tc - c * K));
       }
     }
     __syncthreads();  // sh is free again
@@ -265,6 +303,7 @@ static int softmax_loss(admm_ctx *ctx, SoftmaxArgs a) {
     const dim3 grid(blocks_for(a.rows, 1));
     if (chunks <= 1024) hipLaunchKernelGGL((k_softmax_block<T, 256, 4>), grid, dim3(256), 0, ctx->stream, a);
     else if (chunks <= 4096) hipLaunchKernelGGL((k_softmax_block<T, 512, 8>), grid, dim3(512), 0, ctx->stream, a);
+    else if (chunks <= 16384) hipLaunchKernelGGL((k_softmax_block<T, 1024, 16>), grid, dim3(1024), 0, ctx->stream, a);
     else hipLaunchKernelGGL((k_softmax_block<T, 1024, 0>), grid, dim3(1024), 0, ctx->stream, a);
   }
   ADMM_HIP_CHECK(hipGetLastError());
