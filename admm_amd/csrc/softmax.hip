@@ -185,9 +185,10 @@ struct Edges {
 };
 
 // Rows of any length, one workgroup each: whole granules, CH a thread, kept in registers (CH > 0) or read again (CH == 0), and
-// the edges' elements one a thread.
+// the edges' elements one a thread.  (Keeping some in LDS so that two rows of 10^5 halves fit a CU gave 3.8 TB/s where one in
+// registers gives 4.)
 template <class T, int NT, int CH>
-__global__ void __launch_bounds__(NT) k_softmax_block(SoftmaxArgs a) {
+__global__ void __launch_bounds__(NT, NT == 512 ? 4 : 1) k_softmax_block(SoftmaxArgs a) {
   constexpr int K = 16 / sizeof(T);
   typedef vec_t<T, K> chunk;
   __shared__ float sh[2][NT / 64];
@@ -222,42 +223,51 @@ __global__ void __launch_bounds__(NT) k_softmax_block(SoftmaxArgs a) {
     const float xt = t >= 0 ? (float)from[t] : 0.0f;  // before anyone writes over it
     const float edge = tid < edges.count ? (float)from[edges.column(tid)] : -INFINITY;
     chunk x[CH ? CH : 1];
-    float m = edge, s;
+    // One pass: the sum is kept relative to the running maximum, so that the exponentials are computed while the row arrives: 179
+    // us for 8192 rows of 32000 where a maximum first and the sum after it takes 185.  With 16 granules a thread it needs more
+    // registers than there are: 97 us the other way for 1001 rows of 100003, 100 this way.
+    constexpr bool kOnePass = CH < 16;
+    float m = edge;
     Shift b(m);
+    float s = exp2_fast(__fmaf_rn(edge, b.l, -b.m2));
+    auto take = [&](const chunk &y) {
+      const float mc = chunk_max<T>(y, m);
+      if (mc > m) {
+        const Shift next(mc);
+        s *= m == -INFINITY ? 1.0f : exp2_fast(b.m2 - next.m2);  // s is 0 (or NaN) while no class was seen
+        m = mc;
+        b = next;
+      }
+      s += chunk_sum<T>(y, b);
+    };
     if (CH) {
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         x[c] = none;
         if (c * NT + tid < count) x[c] = in[c * NT + tid];
       }
+      if (kOnePass) {
 #pragma unroll
-      for (int c = 0; c < CH; ++c) m = chunk_max<T>(x[c], m);
-      m = block_max<NT>(m, sh[0]);
-      b = Shift(m);
+        for (int c = 0; c < CH; ++c) take(x[c]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) m = chunk_max<T>(x[c], m);
+      }
+    } else {
+      for (int c = tid; c < count; c += NT) take(in[c]);
+    }
+    const float mine = m, was = b.m2;
+    m = block_max<NT>(m, sh[0]);
+    b = Shift(m);
+    if (kOnePass) {
+      if (mine != -INFINITY) s *= exp2_fast(was - b.m2);
+    } else {
       s = exp2_fast(__fmaf_rn(edge, b.l, -b.m2));
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         stay_packed(x[c]);
         s += chunk_sum<T>(x[c], b);
       }
-    } else {
-      // one pass: the sum is kept relative to the running maximum
-      s = exp2_fast(__fmaf_rn(edge, b.l, -b.m2));
-      for (int c = tid; c < count; c += NT) {
-        const chunk y = in[c];
-        const float mc = chunk_max<T>(y, m);
-        if (mc > m) {
-          const Shift next(mc);
-          s *= m == -INFINITY ? 1.0f : exp2_fast(b.m2 - next.m2);  // s is 0 (or NaN) while no class was seen
-          m = mc;
-          b = next;
-        }
-        s += chunk_sum<T>(y, b);
-      }
-      const float mine = m, was = b.m2;
-      m = block_max<NT>(m, sh[0]);
-      b = Shift(m);
-      if (mine != -INFINITY) s *= exp2_fast(was - b.m2);
     }
     s = block_sum<NT>(s, sh[1]);
     float lse2;
@@ -303,6 +313,7 @@ static int softmax_loss(admm_ctx *ctx, SoftmaxArgs a) {
     const dim3 grid(blocks_for(a.rows, 1));
     if (chunks <= 1024) hipLaunchKernelGGL((k_softmax_block<T, 256, 4>), grid, dim3(256), 0, ctx->stream, a);
     else if (chunks <= 4096) hipLaunchKernelGGL((k_softmax_block<T, 512, 8>), grid, dim3(512), 0, ctx->stream, a);
+    else if (chunks <= 8192) hipLaunchKernelGGL((k_softmax_block<T, 512, 16>), grid, dim3(512), 0, ctx->stream, a);
     else if (chunks <= 16384) hipLaunchKernelGGL((k_softmax_block<T, 1024, 16>), grid, dim3(1024), 0, ctx->stream, a);
     else hipLaunchKernelGGL((k_softmax_block<T, 1024, 0>), grid, dim3(1024), 0, ctx->stream, a);
   }
