@@ -99,7 +99,9 @@ __device__ inline void finish_row(const SoftmaxArgs &a, uint64_t r, Shift b, flo
   if (!writes) return;
   const float nats = b.l == 1.0f ? 1.0f : kLn2;
   if (a.lse) a.lse[r] = s == 0.0f ? -INFINITY : b.m2 * nats + log2s * kLn2;
-  a.loss[r] = t < 0 ? 0.0f : s == 0.0f ? INFINITY * w : w * (kLn2 * log2s - nats * __fmaf_rn(xt, b.l, -b.m2));
+  // (a label masked by the type's lowest value: x_t L would overflow)
+  const float off = fabsf(xt) < 0x1p100f ? nats * __fmaf_rn(xt, b.l, -b.m2) : xt - nats * b.m2;
+  a.loss[r] = t < 0 ? 0.0f : s == 0.0f ? INFINITY * w : w * (kLn2 * log2s - off);
 }
 
 // Rows of up to 64 CH chunks: 2^lanes_log2 lanes hold a row, CH chunks each, and reduce it among themselves.
@@ -295,8 +297,92 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 4 : 1) k_softmax_block(Softmax
   }
 }
 
+// ---- few long rows: several workgroups each -------------------------------------------------------------
+//
+// A row is cut into pieces of kPiece granules.  The first launch leaves every piece's largest logit and its sum relative to
+// that; the second puts a row's pieces together (every workgroup for itself, in the same order) and writes the gradient of
+// its own, which it reads again from the cache.
+constexpr int kPiece = 2048;
+constexpr uint64_t kFewRows = 128;  // from here on the rows fill the GPU by themselves
+
+struct Piece {
+  float m, s;
+};
+
 template <class T>
-static int softmax_loss(admm_ctx *ctx, SoftmaxArgs a) {
+__global__ void __launch_bounds__(256) k_softmax_pieces(SoftmaxArgs a, Piece *pieces, float *label_logits) {
+  __shared__ float sh[2][4];
+  constexpr int K = 16 / sizeof(T);
+  const uint64_t r = blockIdx.y;
+  float w;
+  const int64_t t = label_of(a, r, w);
+  if (t < 0 && !a.lse) return;
+  const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int)a.cols);
+  const T none = (T)-INFINITY;
+  const int c0 = (int)blockIdx.x * kPiece + (int)threadIdx.x;
+  vec_t<T, K> x[kPiece / 256];
+  float m = -INFINITY, s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kPiece / 256; ++i) {
+    x[i] = none;
+    if (c0 + i * 256 < row.count) x[i] = row.load(c0 + i * 256, none);
+    m = chunk_max<T>(x[i], m);
+  }
+  m = block_max<256>(m, sh[0]);
+  const Shift b(m);
+#pragma unroll
+  for (int i = 0; i < kPiece / 256; ++i) {
+    stay_packed(x[i]);
+    s += chunk_sum<T>(x[i], b);
+  }
+  s = block_sum<256>(s, sh[1]);
+  if (threadIdx.x != 0) return;
+  pieces[r * gridDim.x + blockIdx.x] = Piece{m, s};
+  if (blockIdx.x == 0) label_logits[r] = t >= 0 ? (float)row.base[row.lead + t] : 0.0f;  // the next launch may write over it
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) k_softmax_pieces_grad(SoftmaxArgs a, const Piece *pieces, const float *label_logits, unsigned count) {
+  constexpr int K = 16 / sizeof(T);
+  const uint64_t r = blockIdx.y;
+  float w;
+  const int64_t t = label_of(a, r, w);
+  const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int)a.cols);
+  const vec_t<T, K> zero = (T)0.0f;
+  float s = 0.0f, lse2 = 0.0f;
+  Shift b(0.0f);
+  if (t >= 0 || a.lse) {
+    // every wave for itself: its lanes take pieces in turn
+    float m = -INFINITY;
+    for (unsigned i = threadIdx.x & 63; i < count; i += 64) m = fmaxf(m, pieces[r * count + i].m);
+    for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    b = Shift(m);
+    for (unsigned i = threadIdx.x & 63; i < count; i += 64) {
+      const Piece p = pieces[r * count + i];
+      s += p.m == -INFINITY ? p.s : p.s * exp2_fast(Shift(p.m).m2 - b.m2);  // s of a piece without classes: 0, or NaN
+    }
+    for (int off = 1; off < 64; off <<= 1) s += __shfl_xor(s, off, 64);
+    finish_row(a, r, b, s, t, w, label_logits[r], blockIdx.x == 0 && threadIdx.x == 0, lse2);
+  } else if (blockIdx.x == 0 && threadIdx.x == 0) {
+    a.loss[r] = 0.0f;
+  }
+  if (!a.grad) return;
+  T *const to = static_cast<T *>(a.grad) + r * a.gstride;
+  const float g = t < 0 ? 0.0f : w * a.grad_scale;
+  const int tc = t < 0 ? -1 : (int)t + row.lead;
+#pragma unroll
+  for (int i = 0; i < kPiece / 256; ++i) {
+    const int at = (int)blockIdx.x * kPiece + (int)threadIdx.x + i * 256;
+    if (at >= row.count) break;
+    row.store(to, a.apart, at, t < 0 || s == 0.0f ? zero : chunk_grad<T>(row.load(at, (T)-INFINITY), b.l, lse2, g, tc - at * K));
+  }
+}
+
+// pieces of a row, whatever its alignment
+static uint64_t piece_count(uint64_t cols, uint64_t per) { return ((cols + per - 1) / per + 1 + kPiece - 1) / kPiece; }
+
+template <class T>
+static int softmax_loss(admm_ctx *ctx, SoftmaxArgs a, void *workspace) {
   constexpr uint64_t K = 16 / sizeof(T);
   auto offset = [](const void *p) { return reinterpret_cast<uintptr_t>(p) & 15; };
   a.apart = a.grad && (offset(a.grad) != offset(a.logits) || (a.rows > 1 && (a.gstride - a.stride) * sizeof(T) % 16 != 0));
@@ -309,9 +395,16 @@ static int softmax_loss(admm_ctx *ctx, SoftmaxArgs a) {
     if (chunks <= 64) hipLaunchKernelGGL((k_softmax_lanes<T, 1>), grid, dim3(256), 0, ctx->stream, a);
     else if (chunks <= 128) hipLaunchKernelGGL((k_softmax_lanes<T, 2>), grid, dim3(256), 0, ctx->stream, a);
     else hipLaunchKernelGGL((k_softmax_lanes<T, 4>), grid, dim3(256), 0, ctx->stream, a);
+  } else if (a.rows < kFewRows && chunks > kPiece) {
+    const dim3 grid((unsigned)piece_count(a.cols, K), (unsigned)a.rows);
+    float *label_logits = static_cast<float *>(workspace);
+    Piece *pieces = reinterpret_cast<Piece *>(label_logits + kFewRows);
+    hipLaunchKernelGGL(k_softmax_pieces<T>, grid, dim3(256), 0, ctx->stream, a, pieces, label_logits);
+    hipLaunchKernelGGL(k_softmax_pieces_grad<T>, a.grad ? grid : dim3(1, grid.y), dim3(256), 0, ctx->stream, a, pieces, label_logits, grid.x);
   } else {
     const dim3 grid(blocks_for(a.rows, 1));
     if (chunks <= 1024) hipLaunchKernelGGL((k_softmax_block<T, 256, 4>), grid, dim3(256), 0, ctx->stream, a);
+    else if (chunks <= 2048) hipLaunchKernelGGL((k_softmax_block<T, 256, 8>), grid, dim3(256), 0, ctx->stream, a);
     else if (chunks <= 4096) hipLaunchKernelGGL((k_softmax_block<T, 512, 8>), grid, dim3(512), 0, ctx->stream, a);
     else if (chunks <= 8192) hipLaunchKernelGGL((k_softmax_block<T, 512, 16>), grid, dim3(512), 0, ctx->stream, a);
     else if (chunks <= 16384) hipLaunchKernelGGL((k_softmax_block<T, 1024, 16>), grid, dim3(1024), 0, ctx->stream, a);
@@ -329,7 +422,8 @@ extern "C" int admm_softmax_loss_workspace(uint64_t rows, uint64_t cols, uint64_
   ADMM_REQUIRE(bytes, "admm_softmax_loss_workspace: bytes is NULL");
   ADMM_REQUIRE(rows < (1ull << 40) && cols <= kMaxClasses, "admm_softmax_loss_workspace: %llu x %llu logits", (unsigned long long)rows,
                (unsigned long long)cols);
-  *bytes = 0;
+  // of the narrowest granules, for logits of any type
+  *bytes = rows && rows < kFewRows && (cols + 3) / 4 + 1 > kPiece ? kFewRows * sizeof(float) + rows * piece_count(cols, 4) * sizeof(Piece) : 0;
   return ADMM_OK;
 }
 
@@ -370,5 +464,5 @@ extern "C" int admm_softmax_loss(admm_ctx *ctx, const admm_mat *logits, const vo
   a.grad_scale = grad_scale;
   a.loss = loss;
   a.lse = lse;
-  return logits->type == ADMM_F32 ? softmax_loss<float>(ctx, a) : logits->type == ADMM_BF16 ? softmax_loss<bf16_t>(ctx, a) : softmax_loss<f16_t>(ctx, a);
+  return logits->type == ADMM_F32 ? softmax_loss<float>(ctx, a, workspace) : logits->type == ADMM_BF16 ? softmax_loss<bf16_t>(ctx, a, workspace) : softmax_loss<f16_t>(ctx, a, workspace);
 }

@@ -298,6 +298,31 @@ def test_softmax_loss(ctx, kind, rows, cols):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("cols", [4099, 9000, 16385, 33001, 65600, 131089])
+def test_softmax_loss_many_long_rows(ctx, kind, cols):
+    """rows enough that each has a workgroup of its own: in registers of several sizes, and read twice"""
+    g = rng(18, cols)
+    rows = 131
+    x = make_logits(rows, cols, kind, g)
+    labels = torch.randint(0, cols, (rows,), generator=g, device="cuda")
+    labels[::9] = -1
+    labels[1], labels[2] = 0, cols - 1
+    x[3, ::2] = -math.inf
+    x[4, :] = -math.inf
+    x[5, : cols - 1] = torch.finfo(x.dtype).min
+    x[6, cols // 3] = math.nan
+    x[7, 1] = math.inf
+    loss, grad = torch.empty(rows, device="cuda"), torch.empty_like(x)
+    ctx.softmax_loss(x, labels, loss, grad=grad)
+    assert loss[4] == math.inf and torch.all(grad[4] == 0)
+    for r in (6, 7):
+        assert torch.isnan(loss[r]) and torch.isnan(grad[r]).all()
+    x[6:8] = 0
+    check_softmax(ctx, x, labels)
+    check_softmax(ctx, x, labels, grad=x)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("cols", [5, 16, 300, 5000, 9001, 70000])
 def test_softmax_loss_rows_without_classes_or_with_nan(ctx, kind, cols):
     g = rng(9, cols)
