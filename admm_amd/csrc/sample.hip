@@ -816,12 +816,183 @@ __global__ void __launch_bounds__(kThreads) k_sample_rest(SampleArgs a, uint64_t
   draw_row(a, r, q, weight, (unsigned long long)key_of(top) << a.index_bits | first, RowSource<T>{row.base + row.lead, row.cols}, s.sh);
 }
 
+constexpr uint64_t kSmallCols = 1024;
+
+// ---- rows of up to 1024 classes ------------------------------------------------------------------------
+//
+// In one launch: LANES lanes hold a row, EACH consecutive classes a lane, and sort its keys in their registers (bitonic: the
+// partner of position p is p ^ j, in the same lane for j < EACH).  The sums over the sorted classes say which is the last that
+// is kept, those over the classes where they are give the token.  No row is left to anyone else.
+template <class T, int LANES, int EACH>
+__global__ void __launch_bounds__(256) k_sample_small(SampleArgs a) {
+  const int lane = (int)threadIdx.x & (LANES - 1);
+  auto sum = [&](unsigned long long v) {
+#pragma unroll
+    for (int off = 1; off < LANES; off <<= 1) v += __shfl_xor(v, off, 64);
+    return v;
+  };
+  auto sum_before = [&](unsigned long long v) {  // of the lanes before this one
+    unsigned long long up = v;
+#pragma unroll
+    for (int off = 1; off < LANES; off <<= 1) {
+      const unsigned long long y = __shfl_up(up, off, LANES);
+      if (lane >= off) up += y;
+    }
+    return up - v;
+  };
+  for (uint64_t r = (uint64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES; r < a.rows; r += (uint64_t)gridDim.x * (256 / LANES)) {
+    const T *row = static_cast<const T *>(a.logits) + r * a.stride;
+    const Params q = params_of(a, r);
+    float x[EACH];
+    unsigned long long mine[EACH], o[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int j = lane * EACH + e;
+      x[e] = j < (int)a.cols ? (float)row[j] : -INFINITY;
+      mine[e] = o[e] = j < (int)a.cols ? (unsigned long long)key_of(x[e]) << a.index_bits | (unsigned)j : ~0ull;
+    }
+    // sorted: position lane * EACH + e (without top-k and top-p the first class is all that is wanted of it)
+    const bool sorts = (q.k > 0 || q.p < 1.0f) && !is_greedy(q);
+    for (int k = 2; sorts && k <= LANES * EACH; k <<= 1) {
+      for (int j = k >> 1; j >= EACH; j >>= 1) {
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+          const unsigned long long other = __shfl_xor(o[e], j / EACH, 64);
+          const int p = lane * EACH + e;
+          const bool low = ((p & j) == 0) == ((p & k) == 0);
+          o[e] = (other < o[e]) == low ? other : o[e];
+        }
+      }
+#pragma unroll
+      for (int j = EACH >> 1; j >= 1; j >>= 1) {
+        if (j >= k) continue;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+          if (e & j) continue;
+          const bool up = ((lane * EACH + e) & k) == 0;
+          const unsigned long long lo = o[e] < o[e ^ j] ? o[e] : o[e ^ j], hi = o[e] < o[e ^ j] ? o[e ^ j] : o[e];
+          o[e] = up ? lo : hi;
+          o[e ^ j] = up ? hi : lo;
+        }
+      }
+    }
+    unsigned long long first = o[0];
+    if (!sorts) {
+#pragma unroll
+      for (int e = 1; e < EACH; ++e) first = o[e] < first ? o[e] : first;
+#pragma unroll
+      for (int off = 1; off < LANES; off <<= 1) {
+        const unsigned long long y = __shfl_xor(first, off, 64);
+        first = y < first ? y : first;
+      }
+    }
+    first = __shfl(first, 0, LANES);
+    const float top = logit_of((uint32_t)(first >> a.index_bits));
+    const uint32_t mask = (1u << a.index_bits) - 1;
+    if (top == -INFINITY || is_greedy(q)) {
+      if (lane == 0) {
+        a.token[r] = top == -INFINITY ? -1 : (int32_t)(first & mask);
+        if (a.logprob) a.logprob[r] = top == -INFINITY ? -INFINITY : 0.0f;
+      }
+      continue;
+    }
+    const Weights weight(top, q.t, q.m, a.shift);
+    // (a top of +inf has all the weight)
+    auto scaled = [&](float v) { return top == INFINITY ? (v == top ? ldexp(1.0, a.shift) : 0.0) : weight.scaled(v); };
+    unsigned long long last = ~0ull;
+    if (q.k > 0 || q.p < 1.0f) {
+      unsigned long long u[EACH], all = 0;
+      int kept = 0;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int at = lane * EACH + e;
+        const bool in = at < (int)a.cols && (q.k <= 0 || at < q.k);
+        u[e] = in && q.p < 1.0f ? weight.units(scaled(logit_of((uint32_t)(o[e] >> a.index_bits)))) : 0;
+        all += u[e];
+        kept += in;
+      }
+      if (q.p < 1.0f) {
+        const unsigned long long target = mass_target(q.p, sum(all));
+        unsigned long long before = sum_before(all);
+        int count = 0;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+          const int at = lane * EACH + e;
+          count += at < (int)a.cols && (q.k <= 0 || at < q.k) && before < target;
+          before += u[e];
+        }
+        kept = count;
+      }
+      // the kept ones are the first in order: the last of them is the largest key
+      last = 0;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e)
+        if (e < kept) last = o[e];
+#pragma unroll
+      for (int off = 1; off < LANES; off <<= 1) {
+        const unsigned long long y = __shfl_xor(last, off, 64);
+        last = y > last ? y : last;
+      }
+    }
+    unsigned long long amount[EACH], all = 0;
+    int lowest = 0x7FFFFFFF;  // class of any weight, however small: the token for u <= 0
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const double w = scaled(x[e]);
+      const bool in = mine[e] <= last && mine[e] != ~0ull && (w >= weight.least || mine[e] == first);
+      amount[e] = in ? weight.units(w) : 0;
+      all += amount[e];
+      const bool any = x[e] == top || ((double)x[e] - (double)top) * weight.per > -1075.0;
+      if (in && any && lane * EACH + e < lowest) lowest = lane * EACH + e;
+    }
+    const unsigned long long total = sum(all);
+    int token = -1;
+    float value = 0.0f;
+    if (q.u > 0.0f) {
+      const unsigned long long target = draw_target(q.u, total);
+      unsigned long long before = sum_before(all);
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        if (before < target && target <= before + amount[e]) {
+          token = lane * EACH + e;
+          value = x[e];
+        }
+        before += amount[e];
+      }
+    } else {
+      int at = lowest;
+#pragma unroll
+      for (int off = 1; off < LANES; off <<= 1) at = min(at, __shfl_xor(at, off, 64));
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        if (lane * EACH + e == at) {
+          token = at;
+          value = x[e];
+        }
+      }
+    }
+    if (token >= 0) write_token(a, r, (uint32_t)token, value, weight, q.t, total);
+  }
+}
+
 static uint64_t tops_groups(uint64_t cols, uint64_t per) { return ((cols + per - 1) / per + 1 + kGroup - 1) / kGroup; }
 
 static uint64_t tops_bytes(uint64_t rows, uint64_t groups) { return round_up(rows * groups * sizeof(float), 256); }
 
 template <class T>
 static int sample(admm_ctx *ctx, SampleArgs a, void *workspace) {
+  if (a.cols <= kSmallCols) {
+#define ADMM_SMALL(LANES, EACH) hipLaunchKernelGGL((k_sample_small<T, LANES, EACH>), dim3(blocks_for(a.rows, 256 / LANES)), dim3(256), 0, ctx->stream, a)
+    if (a.cols <= 16) ADMM_SMALL(16, 1);
+    else if (a.cols <= 64) ADMM_SMALL(64, 1);
+    else if (a.cols <= 128) ADMM_SMALL(64, 2);
+    else if (a.cols <= 256) ADMM_SMALL(64, 4);
+    else if (a.cols <= 512) ADMM_SMALL(64, 8);
+    else ADMM_SMALL(64, 16);
+#undef ADMM_SMALL
+    ADMM_HIP_CHECK(hipGetLastError());
+    return ADMM_OK;
+  }
   a.groups = (int64_t)tops_groups(a.cols, 16 / sizeof(T));
   a.tops = static_cast<float *>(workspace);
   a.sums = reinterpret_cast<unsigned long long *>(static_cast<char *>(workspace) + tops_bytes(a.rows, a.groups));
@@ -852,6 +1023,8 @@ extern "C" int admm_sample_workspace(uint64_t rows, uint64_t cols, uint64_t *byt
   ADMM_REQUIRE(bytes, "admm_sample_workspace: bytes is NULL");
   ADMM_REQUIRE(rows < (1ull << 40) && cols <= kMaxClasses, "admm_sample_workspace: %llu x %llu logits", (unsigned long long)rows,
                (unsigned long long)cols);
+  *bytes = 0;
+  if (cols <= kSmallCols) return ADMM_OK;
   // enough for logits of any type: granules of four floats are the most
   *bytes = tops_bytes(rows, tops_groups(cols, 4)) + (rows < kBatch ? rows : kBatch) * (kParts * kSums * sizeof(unsigned long long));
   return ADMM_OK;

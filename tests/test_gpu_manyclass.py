@@ -451,6 +451,44 @@ def test_sample(ctx, kind, rows, cols):
         check_sample(ctx, x, u, np.where(some, 0, t), k=np.where(rs.rand(rows) < 0.5, 0, k), p=np.where(some, 1.5, p), m=np.where(rs.rand(rows) < 0.3, 0, m))
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("cols", [15, 16, 64, 65, 128, 129, 256, 257, 512, 513, 1024, 1025])
+def test_sample_where_the_form_changes(ctx, kind, cols):
+    """numbers of classes around those where a row takes more lanes, or more registers, or another kernel"""
+    g, rows = rng(19, cols), 37
+    rs = np.random.RandomState(cols)
+    x = make_logits(rows, cols, kind, g, 2.0)
+    x[1] = x[1, 0]
+    x[2, ::2] = -math.inf
+    x[3, cols // 3:] = math.nan
+    x[4, [cols // 2, cols - 1]] = math.inf
+    x[5] = -math.inf
+    u = rs.rand(rows).astype(np.float32)
+    u[6:9] = [0.0, -1.0, 1.0]
+    for i in range(4):
+        pick = lambda v, off: np.where(rs.rand(rows) < 0.5, off, v)  # noqa: E731
+        t, k = pick(rs.uniform(0.3, 2, rows), 1.0), pick(rs.randint(1, cols + 1, rows), 0)
+        p, m = pick(rs.uniform(0.05, 1, rows), 1.0), pick(rs.uniform(0.001, 0.9, rows), 0.0)
+        t[rs.rand(rows) < 0.1] = 0
+        check_sample(ctx, x, u, t, k=k, p=p, m=m)
+    check_sample(ctx, x, u)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", [3000, 50000])
+def test_sample_of_many_candidates(ctx, kind, cols):
+    """a k beyond what fits LDS, nuclei of most of the classes, flat rows, classes that tie by the thousand"""
+    g, rows = rng(20, cols), 12
+    rs = np.random.RandomState(cols)
+    u, t = rs.rand(rows).astype(np.float32), rs.uniform(0.5, 2, rows)
+    for spread in (0.0, 0.01, 1.0):
+        x = make_logits(rows, cols, kind, g, spread)
+        check_sample(ctx, x, u, t, k=rs.randint(cols // 20, cols, rows))
+        check_sample(ctx, x, u, t, p=rs.uniform(0.9, 0.9999, rows))
+        check_sample(ctx, x, u, t, k=rs.randint(100, 500, rows), p=rs.uniform(0.5, 0.99, rows))
+        check_sample(ctx, x, u, t, p=rs.uniform(0.5, 0.99, rows), m=rs.uniform(0.01, 0.9, rows))
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_sample_ties_and_borders(ctx, kind):
     """equal logits: weights of exactly one, so the numbers of classes and the draws fall on exact borders"""
