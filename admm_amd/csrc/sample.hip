@@ -27,6 +27,7 @@ struct SampleArgs {
   float *tops;            // [rows][groups] largest logits of kGroup granules each
   int64_t groups;
   unsigned long long *sums;  // [rows of a batch][kParts][kSums]
+  int split;                 // workgroups per part that add to its sums; more than one where there are few rows
 };
 
 // larger logits have smaller keys; -0 counts as 0 and NaN as -inf
@@ -300,7 +301,7 @@ __device__ inline void draw_row(const SampleArgs &a, uint64_t r, const Params &q
 //    granules.  What follows knows from those the row's largest logit and reads the row again from the caches.
 //  * k_sample_list (where top-k is given), a workgroup per row: the k-th largest logit is not below the k-th largest of the
 //    groups'.  The classes from that bound on are few; everything else happens among them in LDS.
-//  * k_sample_sums (the rows without top-k), kParts workgroups per row: for top-p the weights are summed by kBuckets buckets of
+//  * k_sample_sums (the rows without top-k), kParts workgroups per row, or up to eight times as many for few rows: for top-p the weights are summed by kBuckets buckets of
 //    the logit.  Weights below (1 - p) / cols of the largest take no part in the buckets: together they are less than 1 - p of
 //    the whole.  Without top-p there is one sum; min-p is a bound on the weight.
 //  * k_sample_rest, a workgroup per row: the target of top-p falls into one bucket, whose classes are put in order; what is kept
@@ -376,6 +377,8 @@ template <class T>
 __global__ void __launch_bounds__(256) k_sample_tops(SampleArgs a) {
   constexpr int K = 16 / sizeof(T);
   const Chunks<T> row(static_cast<const T *>(a.logits) + (uint64_t)blockIdx.y * a.stride, (int)a.cols);
+  if (a.split > 1)  // the sums are added to by several workgroups of the next launch
+    for (unsigned i = blockIdx.x * 256 + threadIdx.x; i < kParts * kSums; i += gridDim.x * 256) a.sums[blockIdx.y * (uint64_t)(kParts * kSums) + i] = 0;
   const int c0 = (int)(blockIdx.x * kTopsPer + threadIdx.x);
   vec_t<T, K> x[kTopsPer / 256];
 #pragma unroll
@@ -541,12 +544,17 @@ __global__ void __launch_bounds__(256) k_sample_sums(SampleArgs a, uint64_t r0) 
   if (!by_sums(q, top)) return;
   const Weights weight(top, q.t, q.m, a.shift);
   const Chunks<T, 8> row(static_cast<const T *>(a.logits) + r * a.stride, (int)a.cols);
-  const Part part(row.count, (int)blockIdx.x);
+  const Part part(row.count, (int)blockIdx.x / a.split);
+  const int step = 256 * a.split, start = part.first + (int)blockIdx.x % a.split * 256 + (int)threadIdx.x;
   const T none = (T)-INFINITY;
-  unsigned long long *to = a.sums + (blockIdx.y * kParts + blockIdx.x) * (uint64_t)kSums;
+  unsigned long long *to = a.sums + (blockIdx.y * kParts + blockIdx.x / a.split) * (uint64_t)kSums;
+  auto put_sum = [&](int i, unsigned long long v) {
+    if (a.split == 1) to[i] = v;
+    else if (v) atomicAdd(to + i, v);  // integers: in any order
+  };
   unsigned long long rest = 0, above = 0;  // below the buckets; passing min-p
   auto each = [&](auto f) {
-    for (int c = part.first + (int)threadIdx.x; c < part.last; c += 256) {
+    for (int c = start; c < part.last; c += step) {
       const vec_t<T, K> x = row.load(c, none);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
@@ -573,15 +581,15 @@ __global__ void __launch_bounds__(256) k_sample_sums(SampleArgs a, uint64_t r0) 
       each([&](double y, double, unsigned long long u) { put(y, u); });
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < kBuckets; i += 256) to[i] = hist[i];
+    for (int i = threadIdx.x; i < kBuckets; i += 256) put_sum(i, hist[i]);
     rest = block_sum<256>(rest, sh);
   } else {
     each([&](double, double w, unsigned long long u) { above += w >= weight.least ? u : 0; });
   }
   above = block_sum<256>(above, sh);
   if (threadIdx.x == 0) {
-    to[kBuckets] = rest;
-    to[kBuckets + 1] = above;
+    put_sum(kBuckets, rest);
+    put_sum(kBuckets + 1, above);
   }
 }
 
@@ -997,6 +1005,7 @@ static int sample(admm_ctx *ctx, SampleArgs a, void *workspace) {
   a.tops = static_cast<float *>(workspace);
   a.sums = reinterpret_cast<unsigned long long *>(static_cast<char *>(workspace) + tops_bytes(a.rows, a.groups));
   const dim3 block(kThreads);
+  a.split = a.rows * kParts >= 512 ? 1 : (int)(512 / (a.rows * kParts) < 8 ? 512 / (a.rows * kParts) : 8);
   const unsigned per_row = (unsigned)((a.groups * kGroup + kTopsPer - 1) / kTopsPer);
   for (uint64_t r = 0; r < a.rows; r += 65535) {  // rows are the second dimension of the grid
     SampleArgs b = a;
@@ -1008,7 +1017,7 @@ static int sample(admm_ctx *ctx, SampleArgs a, void *workspace) {
   if (a.top_k) hipLaunchKernelGGL(k_sample_list<T>, dim3(blocks_for(a.rows, 1)), block, 0, ctx->stream, a);
   for (uint64_t r = 0; r < a.rows; r += kBatch) {
     const uint64_t end = r + kBatch < a.rows ? r + kBatch : a.rows;
-    hipLaunchKernelGGL(k_sample_sums<T>, dim3(kParts, (unsigned)(end - r)), dim3(256), 0, ctx->stream, a, r);
+    hipLaunchKernelGGL(k_sample_sums<T>, dim3(kParts * a.split, (unsigned)(end - r)), dim3(256), 0, ctx->stream, a, r);
     hipLaunchKernelGGL(k_sample_rest<T>, dim3((unsigned)(end - r)), block, 0, ctx->stream, a, r, end);
   }
   ADMM_HIP_CHECK(hipGetLastError());
