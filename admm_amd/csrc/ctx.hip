@@ -529,6 +529,12 @@ extern "C" int admm_timing_get(admm_ctx *ctx, int kernel, double *total_ms, uint
 extern "C" int admm_vec_alloc(admm_ctx *ctx, uint64_t n, float **out) {
   ADMM_REQUIRE(ctx && out && n > 0, "admm_vec_alloc: bad arguments");
   ADMM_HIP_CHECK(hipSetDevice(ctx->device));
+  hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(ctx->stream, &capturing) != hipSuccess || capturing != hipStreamCaptureStatusNone) {
+    (void)hipGetLastError();
+    set_error("admm_vec_alloc: the context's stream is being captured: allocate before the capture");
+    return ADMM_ERR_STATE;
+  }
   float *p = nullptr;
   ADMM_HIP_CHECK(hipMalloc(&p, sizeof(float) * n));
   hipError_t e = hipMemsetAsync(p, 0, sizeof(float) * n, ctx->stream);

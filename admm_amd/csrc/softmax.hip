@@ -2,8 +2,9 @@
 //
 // With L = log2(e) and m the row's largest logit, the exponentials are 2^(x L - m L) (one fused multiply-add and one
 // hardware exp2 each), s their sum, and
-//   loss = ln 2 (log2 s - (x_t L - m L)),  grad = exp2(x L - (m L + log2 s)) w - [j = t] w.
-// Both read x L - m L through the same rounded m L, so its rounding cancels.  Where m L would overflow (a mask of the type's
+//   loss = ln 2 (log2 s - (x_t L - m L)),  grad = 2^(x L - m L) w / s - [j = t] w.
+// Both read x L - m L through the same rounded m L, so its rounding cancels (log2 s in the exponent instead of the division
+// would add half a step of m L to it, 2e-6 of a probability where m is 30).  Where m L would overflow (a mask of the type's
 // lowest value over a whole row), 1 takes the place of L: logits of that size are equal or more than 2^100 apart.
 #include "rows_common.h"
 
@@ -77,11 +78,11 @@ __device__ inline void stay_packed(V &x) {
 
 // the gradient of a chunk; `at`: which of its elements the label is, or anything else
 template <class T>
-__device__ inline vec_t<T, 16 / sizeof(T)> chunk_grad(const vec_t<T, 16 / sizeof(T)> &x, float l, float lse2, float g, int at) {
+__device__ inline vec_t<T, 16 / sizeof(T)> chunk_grad(const vec_t<T, 16 / sizeof(T)> &x, Shift b, float share, float g, int at) {
   constexpr int K = 16 / sizeof(T);
   float v[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) v[k] = g * exp2_fast(__fmaf_rn((float)x[k], l, -lse2));
+  for (int k = 0; k < K; ++k) v[k] = share * exp2_fast(__fmaf_rn((float)x[k], b.l, -b.m2));
   if (at >= 0 && at < K) {
 #pragma unroll
     for (int k = 0; k < K; ++k) v[k] -= at == k ? g : 0.0f;
@@ -92,11 +93,9 @@ __device__ inline vec_t<T, 16 / sizeof(T)> chunk_grad(const vec_t<T, 16 / sizeof
   return y;
 }
 
-// loss and lse of a row with the label t, and what its gradient takes: lse2 (so that p = 2^(x l - lse2))
-__device__ inline void finish_row(const SoftmaxArgs &a, uint64_t r, Shift b, float s, int64_t t, float w, float xt, bool writes, float &lse2) {
+// loss and lse of a row with the label t
+__device__ inline void finish_row(const SoftmaxArgs &a, uint64_t r, Shift b, float s, int64_t t, float w, float xt) {
   const float log2s = __log2f(s);  // -inf where no class is left
-  lse2 = b.m2 + log2s;
-  if (!writes) return;
   const float nats = b.l == 1.0f ? 1.0f : kLn2;
   if (a.lse) a.lse[r] = s == 0.0f ? -INFINITY : b.m2 * nats + log2s * kLn2;
   // (a label masked by the type's lowest value: x_t L would overflow)
@@ -133,10 +132,9 @@ __global__ void __launch_bounds__(256) k_softmax_lanes(SoftmaxArgs a) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) s += chunk_sum<T>(x[c], b);
     for (unsigned off = 1; off < lanes; off <<= 1) s += __shfl_xor(s, off, 64);
-    float lse2;
-    finish_row(a, r, b, s, t, w, xt, lane == 0, lse2);
+    if (lane == 0) finish_row(a, r, b, s, t, w, xt);
     if (!to) continue;
-    const float g = t < 0 ? 0.0f : w * a.grad_scale;
+    const float g = t < 0 ? 0.0f : w * a.grad_scale, share = g / s;
     const int tc = t < 0 ? -1 : (int)t + row.lead;
 #pragma unroll
     for (int c = 0; c < CH; ++c) stay_packed(x[c]);
@@ -145,7 +143,7 @@ __global__ void __launch_bounds__(256) k_softmax_lanes(SoftmaxArgs a) {
       const int at = c * (int)lanes + (int)lane;
       if (at >= row.count) continue;
       const vec_t<T, K> zero = (T)0.0f;
-      row.store(to, a.apart, at, t < 0 || s == 0.0f ? zero : chunk_grad<T>(x[c], b.l, lse2, g, tc - at * K));
+      row.store(to, a.apart, at, t < 0 || s == 0.0f ? zero : chunk_grad<T>(x[c], b, share, g, tc - at * K));
     }
   }
 }
@@ -272,25 +270,24 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 4 : 1) k_softmax_block(Softmax
       }
     }
     s = block_sum<NT>(s, sh[1]);
-    float lse2;
-    finish_row(a, r, b, s, t, w, xt, tid == 0, lse2);
+    if (tid == 0) finish_row(a, r, b, s, t, w, xt);
     if (to) {
-      const float g = t < 0 ? 0.0f : w * a.grad_scale;
+      const float g = t < 0 ? 0.0f : w * a.grad_scale, share = g / s;
       const int tc = t < 0 ? -1 : (int)t + row.lead - row.whole_from * K;
       const bool no = t < 0 || s == 0.0f;
       if (tid < edges.count) {
         const int j = edges.column(tid);
-        to[j] = no ? (T)0.0f : (T)(g * exp2_fast(__fmaf_rn(edge, b.l, -lse2)) - (j == (int)t ? g : 0.0f));
+        to[j] = no ? (T)0.0f : (T)(share * exp2_fast(__fmaf_rn(edge, b.l, -b.m2)) - (j == (int)t ? g : 0.0f));
       }
       if (CH) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
           const int at = c * NT + tid;
           stay_packed(x[c]);
-          if (at < count) put(at, no ? zero : chunk_grad<T>(x[c], b.l, lse2, g, tc - at * K));
+          if (at < count) put(at, no ? zero : chunk_grad<T>(x[c], b, share, g, tc - at * K));
         }
       } else {
-        for (int c = tid; c < count; c += NT) put(c, no ? zero : chunk_grad<T>(in[c], b.l, lse2, g, tc - c * K));
+        for (int c = tid; c < count; c += NT) put(c, no ? zero : chunk_grad<T>(in[c], b, share, g, tc - c * K));
       }
     }
     __syncthreads();  // sh is free again
@@ -349,7 +346,7 @@ __global__ void __launch_bounds__(256) k_softmax_pieces_grad(SoftmaxArgs a, cons
   const int64_t t = label_of(a, r, w);
   const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int)a.cols);
   const vec_t<T, K> zero = (T)0.0f;
-  float s = 0.0f, lse2 = 0.0f;
+  float s = 0.0f;
   Shift b(0.0f);
   if (t >= 0 || a.lse) {
     // every wave for itself: its lanes take pieces in turn
@@ -362,19 +359,19 @@ __global__ void __launch_bounds__(256) k_softmax_pieces_grad(SoftmaxArgs a, cons
       s += p.m == -INFINITY ? p.s : p.s * exp2_fast(Shift(p.m).m2 - b.m2);  // s of a piece without classes: 0, or NaN
     }
     for (int off = 1; off < 64; off <<= 1) s += __shfl_xor(s, off, 64);
-    finish_row(a, r, b, s, t, w, label_logits[r], blockIdx.x == 0 && threadIdx.x == 0, lse2);
+    if (blockIdx.x == 0 && threadIdx.x == 0) finish_row(a, r, b, s, t, w, label_logits[r]);
   } else if (blockIdx.x == 0 && threadIdx.x == 0) {
     a.loss[r] = 0.0f;
   }
   if (!a.grad) return;
   T *const to = static_cast<T *>(a.grad) + r * a.gstride;
-  const float g = t < 0 ? 0.0f : w * a.grad_scale;
+  const float g = t < 0 ? 0.0f : w * a.grad_scale, share = g / s;
   const int tc = t < 0 ? -1 : (int)t + row.lead;
 #pragma unroll
   for (int i = 0; i < kPiece / 256; ++i) {
     const int at = (int)blockIdx.x * kPiece + (int)threadIdx.x + i * 256;
     if (at >= row.count) break;
-    row.store(to, a.apart, at, t < 0 || s == 0.0f ? zero : chunk_grad<T>(row.load(at, (T)-INFINITY), b.l, lse2, g, tc - at * K));
+    row.store(to, a.apart, at, t < 0 || s == 0.0f ? zero : chunk_grad<T>(row.load(at, (T)-INFINITY), b, share, g, tc - at * K));
   }
 }
 

@@ -660,6 +660,99 @@ def test_the_context_keeps_a_workspace(ctx):
         check_grad(ctx, ids, None, None, torch.arange(rows, device="cuda"), rows, 50, 64, "f32", "f32", False, g)
 
 
+def test_a_workspace_does_not_grow_under_capture(ctx):
+    """a call that needs a larger workspace than its context has is refused while its stream is captured, and captured once
+    the context has it"""
+    from admm_amd import capi
+    side = torch.cuda.Stream()
+    other = capi.Context(0, stream=side.cuda_stream)
+    g = rng(21, 1)
+    x, u = make_logits(3, 5000, "f32", g), torch.rand(3, generator=g, device="cuda")
+    want, token = torch.empty(3, dtype=torch.int32, device="cuda"), torch.empty(3, dtype=torch.int32, device="cuda")
+    ctx.sample(x, u, want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        token.zero_()
+        with pytest.raises(capi.AdmmError, match="captured"):
+            other.sample(x, u, token)
+    with torch.cuda.stream(side):
+        other.sample(x, u, token)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        other.sample(x, u, token)
+    for _ in range(3):
+        token.fill_(9)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(token, want)
+    del graph
+    other.close()
+
+
+def test_nothing_to_do(ctx):
+    """shapes without elements"""
+    f = lambda *shape, **kw: torch.zeros(*shape, device="cuda", **kw)  # noqa: E731
+    none = ctx.bags(f(0, dtype=torch.int64))
+    ctx.embed(none, f(5, 3), f(0, 3))
+    ctx.embed(ctx.bags(f(4, dtype=torch.int64)), f(5, 0), f(4, 0))
+    out, grad = torch.ones(4, 3, device="cuda"), torch.ones(5, 3, device="cuda")
+    ctx.embed(none, f(5, 3), out)
+    assert torch.all(out == 1)
+    order = ctx.embed_order(none, 5)
+    ctx.embed_grad(none, order, f(0, 3), grad, accumulate=True)
+    assert torch.all(grad == 1)
+    ctx.embed_grad(none, order, f(0, 3), grad)
+    assert torch.all(grad == 0)
+    ctx.softmax_loss(f(0, 3), f(0, dtype=torch.int64), f(0))
+    ctx.sample(f(0, 3), f(0), f(0, dtype=torch.int32))
+    empty_rows = ctx.bags(f(0, dtype=torch.int32), f(4, dtype=torch.int64))
+    out = torch.ones(3, 3, device="cuda")
+    ctx.embed(empty_rows, f(5, 3), out)
+    assert torch.all(out == 0)
+
+
+def test_more_elements_than_32_bits_count(ctx):
+    """a table and logits of more than 2^32 elements: rows at both ends"""
+    vocab, cols = 1 << 20, 4104
+    table = torch.zeros(vocab, cols, dtype=torch.bfloat16, device="cuda")
+    ids = torch.tensor([0, 1, vocab - 1, vocab - 2, vocab // 2], device="cuda")
+    g = rng(22, 1)
+    rows = torch.randn(5, cols, generator=g, device="cuda").bfloat16()
+    table[ids] = rows
+    out = torch.empty(5, cols, dtype=torch.bfloat16, device="cuda")
+    bags = ctx.bags(ids)
+    ctx.embed(bags, table, out)
+    assert torch.equal(out, rows)
+    ctx.embed_grad(bags, ctx.embed_order(bags, vocab), rows, table, scale=-1.0, accumulate=True)
+    assert not table.any()
+    table.fill_(1)
+    ctx.embed_grad(bags, ctx.embed_order(bags, vocab), rows, table, scale=2.0)
+    assert torch.equal(table[ids], rows * 2)
+    table[ids] = 0
+    assert not table.any()
+    del table
+    x = torch.zeros(33000, 130200, dtype=torch.bfloat16, device="cuda")
+    peak = torch.arange(33000, device="cuda") % 130200
+    x[torch.arange(33000, device="cuda"), peak] = 30.0
+    token = torch.empty(33000, dtype=torch.int32, device="cuda")
+    u = torch.full((33000,), 0.5, device="cuda")
+    ctx.sample(x, u, token, top_p=u)
+    assert torch.equal(token.long(), peak)
+    ctx.sample(x, u, token, top_k=torch.full((33000,), 5, dtype=torch.int32, device="cuda"))
+    assert torch.equal(token.long(), peak)
+    loss = torch.empty(33000, device="cuda")
+    ctx.softmax_loss(x, peak, loss, grad=x)
+    assert float(loss.abs().max()) < 1e-7  # 130199 e^-30 = 1.2e-8
+    for r in (0, 16500, 32999):
+        p = math.exp(-30) / (1 + 130199 * math.exp(-30))
+        want = torch.full((130200,), p, dtype=torch.float64, device="cuda")
+        want[int(peak[r])] = -130199 * p
+        within(x[r], want, want.abs() * (2.0 ** -8 + 1e-4) + 2.0 ** -23, "grad")
+
+
 def test_python_refusals(ctx):
     from admm_amd import capi
     f = lambda *shape, **kw: torch.zeros(*shape, device="cuda", **kw)  # noqa: E731
