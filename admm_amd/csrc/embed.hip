@@ -219,6 +219,14 @@ struct Sorted {
   float *val;
   const uint32_t *row_of;  // row of every entry in the caller's order; NULL: entry e is row e
   const float *val_of;     // the caller's factors or NULL
+  const uint64_t *rowptr;
+  uint32_t nrows;
+  // the row of an entry; one that does not exist where no row holds the entry (row_of is not written there)
+  __device__ uint32_t row(uint32_t entry) const {
+    if (!row_of) return entry;
+    const uint32_t r = row_of[entry];
+    return r < nrows && rowptr[r] <= entry && entry < rowptr[r + 1] ? r : 0xFFFFFFFFu;
+  }
 };
 
 // Up to kSortSmall entries, in one launch: every workgroup looks at all keys and sorts those of its own range of them in its
@@ -302,7 +310,7 @@ __global__ void __launch_bounds__(1024) k_sort_small(const Id *__restrict__ ids,
   for (uint32_t i = threadIdx.x; i < count; i += 1024) {
     const uint32_t e = entries[i];
     to.ids[first + i] = keys[i] + (uint32_t)from;
-    to.rows[first + i] = to.row_of ? to.row_of[e] : e;
+    to.rows[first + i] = to.row(e);
     if (to.val_of) to.val[first + i] = to.val_of[e];
   }
 }
@@ -388,7 +396,7 @@ __global__ void __launch_bounds__(256) k_sort_move(const Id *__restrict__ ids, c
     if (in < count) {
       key[i] = sort_key<Id, FIRST>(ids, keys, at, trows);
       if (FIRST) {
-        load[i] = to.row_of ? to.row_of[at] : at;
+        load[i] = to.row(at);
         if (sizeof(Load) == 8) load[i] |= (Load)((unsigned long long)__float_as_uint(to.val_of[at]) << 32);
       } else {
         load[i] = loads[at];
@@ -429,18 +437,14 @@ __global__ void __launch_bounds__(256) k_sort_move(const Id *__restrict__ ids, c
   }
 }
 
-// row of every entry; entries that no row holds get a row that does not exist
+// row of every entry that a row holds, 16 lanes a row
 __global__ void __launch_bounds__(256) k_entry_rows(const uint64_t *__restrict__ rowptr, uint64_t nrows, uint64_t nnz,
                                                     uint32_t *__restrict__ row_of) {
-  const unsigned lane = threadIdx.x & 63;
-  for (uint64_t r = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < nrows; r += (uint64_t)gridDim.x * 4) {
+  const unsigned lane = threadIdx.x & 15;
+  for (uint64_t r = (uint64_t)blockIdx.x * 16 + (threadIdx.x >> 4); r < nrows; r += (uint64_t)gridDim.x * 16) {
     const uint64_t b = rowptr[r], e1 = rowptr[r + 1], end = e1 < nnz ? e1 : nnz;
-    for (uint64_t e = b + lane; e < end; e += 64) row_of[e] = (uint32_t)r;
+    for (uint64_t e = b + lane; e < end; e += 16) row_of[e] = (uint32_t)r;
   }
-}
-
-__global__ void __launch_bounds__(256) k_fill_u32(uint32_t *p, uint64_t n, uint32_t v) {
-  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256) p[i] = v;
 }
 
 // ---- gradient ---------------------------------------------------------------------------------
@@ -836,11 +840,9 @@ static int sort_entries(admm_ctx *ctx, const admm_bags *b, uint32_t trows, char 
   const uint32_t n = (uint32_t)b->nnz;
   const Id *ids = static_cast<const Id *>(b->ids);
   auto u32 = [&](uint64_t off) { return reinterpret_cast<uint32_t *>(order + off); };
-  Sorted to{u32(at.ids), u32(at.rows), reinterpret_cast<float *>(order + at.val), b->rowptr ? u32(at.row_of) : nullptr, b->val};
-  if (b->rowptr) {
-    hipLaunchKernelGGL(k_fill_u32, dim3(blocks_for(n, 2048, 4096)), dim3(256), 0, ctx->stream, u32(at.row_of), (uint64_t)n, 0xFFFFFFFFu);
-    hipLaunchKernelGGL(k_entry_rows, dim3(blocks_for(b->nrows, 4)), dim3(256), 0, ctx->stream, b->rowptr, b->nrows, b->nnz, u32(at.row_of));
-  }
+  Sorted to{u32(at.ids), u32(at.rows), reinterpret_cast<float *>(order + at.val), b->rowptr ? u32(at.row_of) : nullptr, b->val, b->rowptr, (uint32_t)b->nrows};
+  if (b->rowptr)
+    hipLaunchKernelGGL(k_entry_rows, dim3(blocks_for(b->nrows, 16)), dim3(256), 0, ctx->stream, b->rowptr, b->nrows, b->nnz, u32(at.row_of));
   if (n <= kSortSmall) {
     const size_t lds = 4 * (17 * 256 + 32 + 2 * (size_t)n);
     ADMM_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&k_sort_small<Id>), hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -891,7 +893,7 @@ static int embed(admm_ctx *ctx, const admm_bags *b, const admm_mat *table, float
 
 // Entries per chunk: short chunks keep the GPU busy where there are few entries; every chunk may write two rows of floats, so
 // they are longer where there are enough.
-static uint64_t grad_chunk(uint64_t nnz) { return nnz <= (1u << 15) ? 8 : nnz <= (1u << 18) ? 16 : 32; }
+static uint64_t grad_chunk(uint64_t nnz) { return nnz <= 16 ? 16 : nnz <= (1u << 13) ? 8 : nnz <= (1u << 18) ? 16 : 32; }
 
 static uint64_t grad_parts_bytes(uint64_t nnz, uint64_t cols) {
   return (nnz + grad_chunk(nnz) - 1) / grad_chunk(nnz) * 2 * round_up(cols, 8) * sizeof(float);
