@@ -495,10 +495,14 @@ __device__ inline void draw_held(const SampleArgs &a, uint64_t r, const Params &
 template <class T, class Amount, class Hit>
 __device__ inline void find_class(const Chunks<T, 8> &row, int c0, int c1, unsigned long long target, Shared &sh, Amount amount, Hit hit) {
   constexpr int K = 8 / sizeof(T);
+  const T none = (T)-INFINITY;
+  vec_t<T, K> x = none, next = none;
+  if (c0 + (int)threadIdx.x < c1) next = row.load(c0 + (int)threadIdx.x, none);
   for (int b = c0; b < c1; b += kThreads) {
     const int c = b + (int)threadIdx.x;
-    vec_t<T, K> x = (T)-INFINITY;
-    if (c < c1) x = row.load(c, (T)-INFINITY);
+    x = next;
+    next = none;
+    if (c + kThreads < c1) next = row.load(c + kThreads, none);
     unsigned long long u[K], mine = 0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -626,7 +630,13 @@ __device__ inline bool draw_sums(const SampleArgs &a, uint64_t r, const unsigned
       const unsigned long long within = target - s.sh.before;
       // the classes of the bucket that the target falls into
       const Chunks<T> wide(static_cast<const T *>(a.logits) + r * a.stride, (int)a.cols);
-      constexpr int K = 16 / sizeof(T), kAhead = 4;
+      constexpr int K = 16 / sizeof(T), kAhead = 8;
+      // The logits of the bucket lie between two floats; these are a little farther apart.  What lies outside is left out by
+      // them, the rest is asked for its bucket (asked all: 16 instructions a class, 62 us instead of 58 at 512 x 128000 bf16,
+      // where the rows come at 12 bytes a clock per CU).  Classes whose exponent is held at -64 weigh nothing and may be left out.
+      const double high = weight.top + (border - 0.5) / buckets.per / weight.per, low = weight.top + (border + 0.5) / buckets.per / weight.per;
+      const float from = (float)(low - fabs(low) * 0x1p-22 - fabs((double)weight.top) * 0x1p-48 - 0x1p-140);
+      const float to = (float)(high + fabs(high) * 0x1p-22 + fabs((double)weight.top) * 0x1p-48 + 0x1p-140);
       for (int c0 = threadIdx.x; c0 < wide.count; c0 += kAhead * kThreads) {
         vec_t<T, K> x[kAhead];
 #pragma unroll
@@ -638,7 +648,7 @@ __device__ inline bool draw_sums(const SampleArgs &a, uint64_t r, const unsigned
         for (int u = 0; u < kAhead; ++u) {
 #pragma unroll
           for (int k = 0; k < K; ++k) {
-            if (buckets.of(weight.exponent((float)x[u][k])) != border) continue;
+            if (!((float)x[u][k] >= from && (float)x[u][k] <= to) || buckets.of(weight.exponent((float)x[u][k])) != border) continue;
             const int j = wide.column(c0 + u * kThreads, k);
             if (j < 0 || j >= wide.cols) continue;
             const unsigned at = atomicAdd(&s.count, 1u);

@@ -533,6 +533,19 @@ def test_sample_odd_logits_and_parameters(ctx, kind, cols):
                  p=[1, 1, 1, 1, 1, 0.0, -1.0, np.nan], m=[0, 0, 0, 0, 1.0, 2.0, -1.0, np.nan])
 
 
+@pytest.mark.parametrize("offset,spread,t", [(0.0, 1.0, 1.0), (1e3, 1.0, 0.7), (-1e3, 1.0, 0.7), (1e5, 1.0, 0.01), (-3e38, 1e36, 1e36),
+                                             (3e37, 3e36, 1e36), (0.0, 1e-37, 1e-37), (1e-36, 1e-38, 1e-38), (0.0, 1e-3, 1e30)])
+def test_sample_top_p_at_any_scale(ctx, offset, spread, t):
+    """the kept classes' border far from zero, close to it and at scales where a logit's step is a large part of a bucket"""
+    g = rng(31, 7)
+    for rows, cols in ((12, 1500), (4, 30000)):
+        x = (torch.randn(rows, cols, generator=g, dtype=torch.float64, device="cuda") * spread * 2 + offset).float()
+        x[0, 1::2] = -math.inf
+        u = np.linspace(0.03, 0.97, rows).astype(np.float32)
+        for p in (0.02, 0.5, 0.93, 0.9999):
+            check_sample(ctx, x, u, t, p=p)
+
+
 def test_sample_does_not_depend_on_the_batch(ctx):
     """a row's token and log-probability are the same alone, in a batch, and at other strides and alignments"""
     g = rng(14, 1)
