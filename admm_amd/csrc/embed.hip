@@ -8,7 +8,8 @@ constexpr int kSortSmall = 16384;  // entries that one workgroup can sort in its
 
 // ---- lookup -----------------------------------------------------------------------------------
 
-// One id per row: a copy with a factor, bound by memory.  2^lanes_log2 lanes share a row, N elements each at a time.
+// One id per row: a copy with a factor, bound by memory.  2^lanes_log2 lanes share a row, N elements each at a time, four of
+// those on the way.  16384 rows of 4096 in 16 bits: 36 us, 134 MB written and the distinct rows (56 MB) read, 5.3 TB/s; 8 rows: 2.3 us.
 template <class T, class TO, int N, class Id>
 __global__ void __launch_bounds__(256) k_embed_rows(const Id *__restrict__ ids, uint64_t nrows, const T *__restrict__ table,
                                                     uint64_t tstride, uint64_t trows, TO *__restrict__ out, uint64_t ostride,
@@ -74,7 +75,8 @@ __device__ inline void add_groups(int lanes_log2, float (&acc)[N]) {
 }
 
 // Rows of several ids.  WAVES waves share a row (1 for short ones, 16 for rows of hundreds of entries), each of them as 64 /
-// 2^lanes_log2 groups of lanes that take entries in turn.
+// 2^lanes_log2 groups of lanes that take entries in turn.  65536 rows of 40 entries over 16 floats: 36 us, bound by the units
+// that form the addresses (2 clocks for the 16 bytes of a lane: 2.6 million entries of 4 lanes), not by the 75 MB that come.
 template <class T, class TO, int N, class Id, int WAVES>
 __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
     k_embed_bags(const Id *__restrict__ ids, const uint64_t *__restrict__ rowptr, const float *__restrict__ val, uint64_t nrows,
@@ -231,7 +233,7 @@ struct Sorted {
 
 // Up to kSortSmall entries, in one launch: every workgroup looks at all keys and sorts those of its own range of them in its
 // LDS; how many are below its range says where they go.  (All passes over all keys in one workgroup: 17.5 us for 4001 keys of
-// 15 bits; this: 9.)
+// 15 bits; this: 10, and 17 for 16384 keys of 17 bits.)
 template <class Id>
 __global__ void __launch_bounds__(1024) k_sort_small(const Id *__restrict__ ids, uint32_t n, uint32_t trows, Sorted to) {
   constexpr int kItems = kSortSmall / 1024;
@@ -330,8 +332,10 @@ __global__ void __launch_bounds__(256) k_entry_rows(const uint64_t *__restrict__
 
 // More entries: one pass per digit, least significant first: counts per tile, their sums, the move.  What is moved with the key
 // is the entry's row, and its factor in the upper half where there are factors.  Up to kFewTiles tiles the move sums their
-// counts itself (counts by tile, then digit), which saves a launch a pass (32000 entries: 47 us instead of 53 with the gradient; 98 tiles: 59 instead of 56); from more of them the sums are made by a launch of
-// their own (counts by digit, then tile).  The first count also finds the entries' rows, with workgroups of its own.
+// counts itself (counts by tile, then digit), which saves a launch a pass (32000 entries: 47 us instead of 53 with the
+// gradient; 98 tiles: 59 instead of 56); from more of them the sums are made by a launch of their own (counts by digit, then
+// tile).  The first count also finds the entries' rows, with workgroups of its own.  2.6 million entries with factors over 2^20
+// ids: 3 passes, 102 us in all, of which the moves 58 and the counts 28; what they read and write would take 25.
 constexpr uint32_t kFewTiles = 48;
 
 template <class Id, bool FIRST>
@@ -539,6 +543,8 @@ __device__ inline void put_part(const GradArgs<T, TO> &a, uint32_t chunk, int sl
 //    of one that begins here and goes on to slot 1.  So every group has the same work, every row is written by one group, in a
 //    fixed order and without atomics, whatever the ids.
 //  * zeros (only where every row has to be written): rows of the table that no entry names.
+// 16384 entries of 2048 columns, bf16 added to f32: 43 us at 128 MB (reads and writes of touched rows, in no order).  2.6 million
+// entries of 16 floats: 49 us, half of it address work as in the lookup; 71 MB are written, 78 read.
 template <class T, class TO, int N>
 __global__ void __launch_bounds__(256) k_grad(GradArgs<T, TO> a) {
   const Place<N> p(a.lanes_log2, a.cols);
@@ -667,7 +673,7 @@ __global__ void __launch_bounds__(256) k_grad(GradArgs<T, TO> a) {
 
 // Runs that go over the end of the chunk they begin in: the sums of their parts, in the order of the chunks.  Runs of up to
 // kShort chunks after the first are summed by a group of lanes each; longer ones by a workgroup, which looks for them in
-// kSet chunks at a time.
+// kSet chunks at a time.  Bound by latency: 29 us for 82000 chunks of which most end inside a run, and 7 for 501.
 constexpr int kShort = 7, kSet = 16;
 
 template <class T, class TO>
@@ -921,12 +927,17 @@ static int embed(admm_ctx *ctx, const admm_bags *b, const admm_mat *table, float
   });
 }
 
-// Entries per chunk: short chunks keep the GPU busy where there are few entries; every chunk may write two rows of floats, so
-// they are longer where there are enough.
-static uint64_t grad_chunk(uint64_t nnz) { return nnz <= 16 ? 16 : nnz <= (1u << 13) ? 8 : nnz <= (1u << 18) ? 16 : 32; }
+// Entries per chunk: short chunks keep the GPU busy where there is little to add; every chunk may write two rows of floats, so
+// they are longer where there is more.  With 8 / 16 / 32 entries a chunk (us, sort included): 4001 entries of 1024 columns 24 /
+// 27 / 37, 262144 of 16 64 / 67 / 79, 16384 of 1024 54 / 46 / 52, 640000 of 16 100 / 95 / 104, 65536 of 1024 177 / 151 / 129,
+// 2.6 million of 16 234 / 194 / 163.  One chunk has nothing to join: 16 entries of 1024 in one 17.4, in two 20.4.
+static uint64_t grad_chunk(uint64_t nnz, uint64_t cols) {
+  const double sums = (double)nnz * (double)cols;
+  return nnz <= 16 ? 16 : sums <= 0x1p23 ? 8 : sums <= 0x1p25 ? 16 : 32;
+}
 
 static uint64_t grad_parts_bytes(uint64_t nnz, uint64_t cols) {
-  return (nnz + grad_chunk(nnz) - 1) / grad_chunk(nnz) * 2 * round_up(cols, 8) * sizeof(float);
+  return (nnz + grad_chunk(nnz, cols) - 1) / grad_chunk(nnz, cols) * 2 * round_up(cols, 8) * sizeof(float);
 }
 
 static int embed_grad(admm_ctx *ctx, const admm_bags *b, const char *order, const admm_mat *from, float scale, int accumulate,
@@ -956,7 +967,7 @@ static int embed_grad(admm_ctx *ctx, const admm_bags *b, const char *order, cons
     a.scale = scale;
     a.accumulate = accumulate != 0;
     a.lanes_log2 = lanes;
-    a.chunk = (uint32_t)grad_chunk(b->nnz);
+    a.chunk = (uint32_t)grad_chunk(b->nnz, from->cols);
     a.nchunks = (uint32_t)((b->nnz + a.chunk - 1) / a.chunk);
     a.parts = parts;
     a.pitch = round_up(from->cols, 8);
@@ -1043,7 +1054,7 @@ extern "C" int admm_embed_grad_workspace(const admm_bags *bags, uint64_t cols, u
   ADMM_REQUIRE(bytes, "admm_embed_grad_workspace: bytes is NULL");
   ADMM_TRY(check_bags(bags, "admm_embed_grad_workspace"));
   ADMM_REQUIRE(cols < (1ull << 40), "admm_embed_grad_workspace: %llu columns", (unsigned long long)cols);
-  *bytes = bags->nnz > grad_chunk(bags->nnz) ? grad_parts_bytes(bags->nnz, cols) : 0;
+  *bytes = bags->nnz > grad_chunk(bags->nnz, cols) ? grad_parts_bytes(bags->nnz, cols) : 0;
   return ADMM_OK;
 }
 
