@@ -50,14 +50,20 @@ __device__ inline float chunk_max(const vec_t<T, 16 / sizeof(T)> &x, float m) {
   return m;
 }
 
-// what is taken off a row's exponents: x l - m2
+// What is taken off a row's exponents: x l - m2, rounded once.  m2 is m L rounded, by up to 2^-24 of itself; that is in every
+// power of the row and cancels, so long as it stays far from the ends of the exponents: by up to 64 at |m| = 2^30.  Larger logits
+// that differ are at least 64 apart, so their factor may as well be 1, with which m2 is exact (and does not overflow).
 struct Shift {
   float l, m2;
   explicit __device__ Shift(float m) {
-    l = fabsf(m) < 0x1p126f || m == -INFINITY ? kLog2e : 1.0f;
+    l = fabsf(m) < 0x1p30f || m == -INFINITY ? kLog2e : 1.0f;
     m2 = m == -INFINITY ? 0.0f : m * l;  // without a class every power is 2^(-inf - 0) = 0
   }
 };
+
+// What a sum relative to `from` is multiplied by to be relative to `to`, a larger logit's.  Where their factors differ, so do the
+// logits, by 64 or more (and m2 is not in their order).
+__device__ inline float moved(Shift from, Shift to) { return from.l == to.l ? exp2_fast(from.m2 - to.m2) : 0.0f; }
 
 template <class T>
 __device__ inline float chunk_sum(const vec_t<T, 16 / sizeof(T)> &x, Shift b) {
@@ -237,7 +243,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 4 : 1) k_softmax_block(Softmax
       const float mc = chunk_max<T>(y, m);
       if (mc > m) {
         const Shift next(mc);
-        s *= m == -INFINITY ? 1.0f : exp2_fast(b.m2 - next.m2);  // s is 0 (or NaN) while no class was seen
+        s *= m == -INFINITY ? 1.0f : moved(b, next);  // s is 0 (or NaN) while no class was seen
         m = mc;
         b = next;
       }
@@ -259,11 +265,12 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 4 : 1) k_softmax_block(Softmax
     } else {
       for (int c = tid; c < count; c += NT) take(in[c]);
     }
-    const float mine = m, was = b.m2;
+    const float mine = m;
+    const Shift was = b;
     m = block_max<NT>(m, sh[0]);
     b = Shift(m);
     if (kOnePass) {
-      if (mine != -INFINITY) s *= exp2_fast(was - b.m2);
+      if (mine != -INFINITY) s *= moved(was, b);
     } else {
       s = exp2_fast(__fmaf_rn(edge, b.l, -b.m2));
 #pragma unroll
@@ -359,7 +366,7 @@ __global__ void __launch_bounds__(256) k_softmax_pieces_grad(SoftmaxArgs a, cons
     b = Shift(m);
     for (unsigned i = threadIdx.x & 63; i < count; i += 64) {
       const Piece p = pieces[r * count + i];
-      s += p.m == -INFINITY ? p.s : p.s * exp2_fast(Shift(p.m).m2 - b.m2);  // s of a piece without classes: 0, or NaN
+      s += p.m == -INFINITY ? p.s : p.s * moved(Shift(p.m), b);  // s of a piece without classes: 0, or NaN
     }
     for (int off = 1; off < 64; off <<= 1) s += __shfl_xor(s, off, 64);
     if (blockIdx.x == 0 && threadIdx.x == 0) finish_row(a, r, b, s, t, w, label_logits[r]);

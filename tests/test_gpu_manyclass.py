@@ -345,6 +345,54 @@ def test_softmax_loss_rows_without_classes_or_with_nan(ctx, kind, cols):
     check_softmax(ctx, x[[0, 5]].contiguous(), torch.zeros(2, dtype=torch.int64, device="cuda"))
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(2, 300), (131, 3000), (131, 9000), (131, 33001), (131, 131089), (3, 40000)])
+def test_softmax_loss_where_the_shift_of_huge_logits_changes(ctx, kind, rows, cols):
+    """logits to both sides of 2^126 within a row, a larger one behind a smaller one; the loss is within the logits' own steps"""
+    g = rng(41, rows, cols)
+    x = make_logits(rows, cols, kind, g)
+    near, far = torch.tensor(0.9 * 2.0 ** 126, dtype=TYPES[kind]), torch.tensor(1.1 * 2.0 ** 126, dtype=TYPES[kind])
+    x[0, : cols // 2], x[0, cols // 2:] = near, far
+    x[1, : cols // 2], x[1, cols // 2:] = -far, -near
+    x[rows - 1], x[rows - 1, cols - 2] = near, far
+    labels = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    labels[rows - 1] = cols - 2
+    loss, grad = torch.empty(rows, device="cuda"), torch.empty_like(x)
+    ctx.softmax_loss(x, labels, loss, grad=grad)
+    step = float(far) - float(near)
+    many = cols - cols // 2
+    U32 = torch.finfo(torch.float32).eps / 2
+    for r in {0, 1} - {rows - 1}:  # the label is one of the smaller: the rest share the probability
+        # both logits' products with L and their difference are rounded: 2^-24 each of at most 2^127 L
+        assert abs(float(loss[r]) - step) <= 8 * U32 * 2.0 ** 127.6, (r, float(loss[r]), step)
+        want = torch.zeros(cols, device="cuda", dtype=torch.float64)
+        want[cols // 2:] = 1.0 / many
+        want[0] -= 1
+        # a sum of equal powers: a rounding per addition, of a thread's, the wave's and the block's
+        bound = want.abs() * (U32 * (64 + many / 256) + torch.finfo(x.dtype).eps) + (2.0 ** -133 if kind == "bf16" else 0.0)
+        within(grad[r], want, bound, "grad")
+    assert abs(float(loss[rows - 1])) <= 8 * U32 * 2.0 ** 127.6 and torch.all(grad[rows - 1] == 0)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(13, 7), (13, 300), (131, 3000), (131, 9000), (131, 33001), (131, 131089), (13, 40000)])
+def test_softmax_loss_of_one_huge_value(ctx, kind, rows, cols):
+    """rows whose logits are all the same (every class masked by the same finite value): an even distribution at any magnitude"""
+    values = [-1e4, 1e6, -1e9, 1.07e9, -1.08e9, 1e10, -1e10, 1e15, -1e20, 1e30, -8.4e37, 8.6e37, -3e38]
+    x = torch.tensor([values[r % 13] for r in range(rows)], device="cuda").to(TYPES[kind])[:, None].expand(rows, cols).contiguous()
+    labels = torch.arange(rows, device="cuda") % cols
+    loss, lse, grad = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda"), torch.empty_like(x)
+    ctx.softmax_loss(x, labels, loss, grad=grad, lse=lse)
+    U32 = torch.finfo(torch.float32).eps / 2
+    # a power's exponent is at most 64, rounded by 2^-24 of that, and the same for all; a rounding per addition
+    sums = U32 * (64 + cols / 256)
+    within(loss, torch.full((rows,), math.log(cols), dtype=torch.float64, device="cuda"), sums + U32 * (4 * 64 + 8), "loss")
+    within(lse, x[:, 0].double() + math.log(cols), sums + U32 * (4 * x[:, 0].double().abs() + 8 * math.log(cols) + 64), "lse")
+    want = torch.full((rows, cols), 1.0 / cols, dtype=torch.float64, device="cuda")
+    want[torch.arange(rows, device="cuda"), labels] -= 1
+    within(grad, want, want.abs() * (4 * U32 + torch.finfo(x.dtype).eps / 2 * 1.01) + (sums + 4 * U32) / cols, "grad")
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("rows,cols,pad,shift", [(9, 30, 3, 1), (9, 64, 64, 0), (5, 1001, 0, 5), (4, 6000, 8, 2), (3, 40001, 1, 3)])
 def test_softmax_loss_strides_and_in_place(ctx, kind, rows, cols, pad, shift):
