@@ -443,6 +443,8 @@ class Context:
     def _bytes(self, buf, name):
         if isinstance(buf, DeviceBuf):
             return buf.ptr, buf.nbytes
+        if not hasattr(buf, "data_ptr"):
+            raise AdmmError("%s: a DeviceBuf or a torch tensor is needed, not %s" % (name, buf.__class__.__name__))
         if buf.get_device() != self.device:
             raise self._elsewhere(buf, name)
         if not buf.is_contiguous():

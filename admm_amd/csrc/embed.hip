@@ -74,7 +74,7 @@ __device__ inline void add_groups(int lanes_log2, float (&acc)[N]) {
   }
 }
 
-// Rows of several ids.  WAVES waves share a row (1 for short ones, 16 for rows of hundreds of entries), each of them as 64 /
+// Rows of several ids.  WAVES waves share a row (1, or 16 for few long ones), each of them as 64 /
 // 2^lanes_log2 groups of lanes that take entries in turn.  65536 rows of 40 entries over 16 floats: 36 us, bound by the units
 // that form the addresses (2 clocks for the 16 bytes of a lane: 2.6 million entries of 4 lanes), not by the 75 MB that come.
 template <class T, class TO, int N, class Id, int WAVES>
@@ -734,10 +734,25 @@ __global__ void __launch_bounds__(256) k_grad_join(GradArgs<T, TO> a, unsigned s
       }
 #pragma unroll
       for (int k = 0; k < N; ++k) acc[k] = 0.0f;
-      const uint32_t step = 4 * p.groups;
-      if (p.here)
-#pragma unroll 4
-        for (uint32_t q = c + p.wave * p.groups + p.group; q <= lo; q += step) add(acc, q, q == c ? 1 : 0);
+      if (p.here) {
+        constexpr int kAhead = 8;
+        const uint32_t step = 4 * p.groups;
+        uint64_t q = c + p.wave * p.groups + p.group;
+        if (q == c) {
+          add(acc, c, 1);
+          q += step;
+        }
+        for (; q + (kAhead - 1) * step <= lo; q += kAhead * step) {
+          float v[kAhead][N];
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) load_n<float, N>(a.parts + (q + u * step) * 2 * a.pitch + p.col, v[u]);
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int k = 0; k < N; ++k) acc[k] += v[u][k];
+        }
+        for (; q <= lo; q += step) add(acc, (uint32_t)q, 0);
+      }
       add_groups<N>(a.lanes_log2, acc);
       __syncthreads();
 #pragma unroll
@@ -807,8 +822,10 @@ static int check_tiles(uint64_t tiles, const char *who, uint64_t cols) {
   return ADMM_OK;
 }
 
-// Entries per tile of the sort's passes: large tiles write longer pieces side by side, small ones keep more of the GPU busy.
-static uint64_t sort_tile(uint64_t n) { return n <= (1u << 19) ? 1024 : 2048; }
+// Entries per tile of the sort's passes: large tiles write longer pieces side by side, small ones keep more of the GPU busy (us
+// with 1024 and 2048: 100000 entries 32 and 40, 400000 36 and 42, 800000 45 and 49, 1600000 54 and 57 or, of more ids, 63 and
+// 61, 2600000 91 and 74, 20000000 594 and 469).
+static uint64_t sort_tile(uint64_t n) { return n <= (1u << 20) ? 1024 : 2048; }
 
 struct OrderLayout {
   uint64_t ids, rows, val, row_of, keys_a, loads_a, keys_b, loads_b, counts, totals, bytes;
@@ -911,8 +928,11 @@ static int embed(admm_ctx *ctx, const admm_bags *b, const admm_mat *table, float
       if (lanes > 6) lanes = 6;
       const uint64_t tiles = (per_row + (1u << lanes) - 1) >> lanes;
       ADMM_TRY(check_tiles(tiles, "admm_embed", table->cols));
-      // a wave takes a row of 40 entries in a few steps; one of many hundreds would keep it alone on its CU
-      const bool longrows = b->nnz / b->nrows >= 512;
+      // 16 waves a row where the rows are too few to fill the GPU and each would keep its wave for many steps (us with 1 and 16:
+      // 300 rows of 40 entries of 256 floats 11 and 5, 1000 of 40 20 and 13, 2000 of 40 23 and 24, of 80 44 and 37, 4000 of 600
+      // 529 and 537, 6000 of 600 595 and 803; of 16 floats 1000 rows of 130 6 and 9, of 600 22 and 18)
+      const uint64_t steps = b->nnz / b->nrows >> (6 - lanes), waves = b->nrows * tiles;
+      const bool longrows = waves <= 2048 && steps >= 8 && steps * 32 >= waves;
       if (longrows)
         hipLaunchKernelGGL((k_embed_bags<T, TO, N, Id, 16>), dim3(blocks_for(b->nrows, 1), (unsigned)tiles), dim3(1024), 0, ctx->stream, ids, b->rowptr,
                            b->val, b->nrows, b->nnz, static_cast<const T *>(table->data), table->stride, table->rows,

@@ -309,8 +309,11 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 4 : 1) k_softmax_block(Softmax
 // A row is cut into pieces of kPiece granules.  The first launch leaves every piece's largest logit and its sum relative to
 // that; the second puts a row's pieces together (every workgroup for itself, in the same order) and writes the gradient of
 // its own, which it reads again from the cache.
-constexpr int kPiece = 2048;
-constexpr uint64_t kFewRows = 128;  // from here on the rows fill the GPU by themselves
+// For fewer than kFewRows rows of more than kLong granules (us for 8 rows in 16 bits, this and a workgroup a row: 48000 classes
+// 10.4 and 9.3, 65000 10.2 and 10.4, 80000 10.4 and 13.9, 131000 10.1 and 16.8; 127 rows of 80000 15.2 and 16.9, of 131000 19.9
+// and 21.9, but 256 of 128000 35.5 and 28).
+constexpr int kPiece = 2048, kLong = 8192;
+constexpr uint64_t kFewRows = 128;
 
 struct Piece {
   float m, s;
@@ -395,6 +398,10 @@ static int softmax_loss(admm_ctx *ctx, SoftmaxArgs a, void *workspace) {
   a.apart = a.grad && (offset(a.grad) != offset(a.logits) || (a.rows > 1 && (a.gstride - a.stride) * sizeof(T) % 16 != 0));
   const bool even = offset(a.logits) == 0 && (a.rows == 1 || a.stride * sizeof(T) % 16 == 0);
   const uint64_t chunks = (a.cols + K - 1) / K + (even ? 0 : 1);  // a row between granules touches one more
+  // The fewest registers and threads that hold a row.  Up to 256 granules a wave holds rows without barriers (8192 rows of 1000
+  // in 16 bits: 9 us, by the next form 22; of 2000: 15 and 24).  Each of the others against the one after it, in 16 bits: 8192
+  // rows of 8000 42 and 50 us, of 16000 101 and 128, 4096 of 32000 100 and 116, 2048 of 64000 108 and 153, 1024 of 128000 123
+  // and 143.
   if (chunks <= 256) {
     a.lanes_log2 = 0;
     while (a.lanes_log2 < 6 && (1ull << a.lanes_log2) < chunks) ++a.lanes_log2;
@@ -402,7 +409,7 @@ static int softmax_loss(admm_ctx *ctx, SoftmaxArgs a, void *workspace) {
     if (chunks <= 64) hipLaunchKernelGGL((k_softmax_lanes<T, 1>), grid, dim3(256), 0, ctx->stream, a);
     else if (chunks <= 128) hipLaunchKernelGGL((k_softmax_lanes<T, 2>), grid, dim3(256), 0, ctx->stream, a);
     else hipLaunchKernelGGL((k_softmax_lanes<T, 4>), grid, dim3(256), 0, ctx->stream, a);
-  } else if (a.rows < kFewRows && chunks > kPiece) {
+  } else if (a.rows < kFewRows && chunks > kLong) {
     const dim3 grid((unsigned)piece_count(a.cols, K), (unsigned)a.rows);
     float *label_logits = static_cast<float *>(workspace);
     Piece *pieces = reinterpret_cast<Piece *>(label_logits + kFewRows);
@@ -430,7 +437,7 @@ extern "C" int admm_softmax_loss_workspace(uint64_t rows, uint64_t cols, uint64_
   ADMM_REQUIRE(rows < (1ull << 40) && cols <= kMaxClasses, "admm_softmax_loss_workspace: %llu x %llu logits", (unsigned long long)rows,
                (unsigned long long)cols);
   // of the narrowest granules, for logits of any type
-  *bytes = rows && rows < kFewRows && (cols + 3) / 4 + 1 > kPiece ? kFewRows * sizeof(float) + rows * piece_count(cols, 4) * sizeof(Piece) : 0;
+  *bytes = rows && rows < kFewRows && (cols + 3) / 4 + 1 > kLong ? kFewRows * sizeof(float) + rows * piece_count(cols, 4) * sizeof(Piece) : 0;
   return ADMM_OK;
 }
 

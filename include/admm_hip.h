@@ -328,7 +328,8 @@ typedef struct admm_mat {
 
 /* Rows of ids in DEVICE memory.  rowptr == NULL: one id per row (tokens), nnz == nrows.  Else row r holds the entries
  * [rowptr[r], rowptr[r+1]) (a sample set's rows; a row may be empty; what lies beyond nnz is not read).  An id outside
- * the table (-1 in a padded batch) stands for nothing: it adds zero and receives no gradient.
+ * the table (-1 in a padded batch) stands for nothing: it adds zero and receives no gradient.  So does an entry whose
+ * factor is 0, whatever its row holds.
  * Limits: nrows, nnz and the table's rows at most 2^32 - 256. */
 typedef struct admm_bags {
   const void *ids;
@@ -369,8 +370,8 @@ int admm_embed_grad(admm_ctx *ctx, const admm_bags *bags, const void *order, uin
  * is outside [0, cols) or whose weight is 0 is not trained on: loss 0, gradient 0.  Logits of -inf are classes that are
  * masked out: probability 0, gradient 0.  A row whose label is masked has loss +inf; one with no class left has loss +inf
  * and gradient 0 (lse -inf).  A NaN, or a logit of +inf, makes its row NaN.
- * cols <= 2^31 - 256.  lse and grad may be NULL (not wanted); grad has the logits' shape and type and may be the logits' own memory (same data
- * and stride), else it may not overlap them. */
+ * lse and grad may be NULL (not wanted); grad has the logits' shape and type and may be the logits' own memory (same data
+ * and stride), else it may not overlap them.  cols <= 2^31 - 256. */
 int admm_softmax_loss_workspace(uint64_t rows, uint64_t cols, uint64_t *bytes);
 int admm_softmax_loss(admm_ctx *ctx, const admm_mat *logits, const void *labels, int label_type, const float *weight,
                       float grad_scale, float *loss, float *lse, const admm_mat *grad, void *workspace,
@@ -385,8 +386,9 @@ int admm_softmax_loss(admm_ctx *ctx, const admm_mat *logits, const void *labels,
  * The token is the first class, in the order of the indexes, at which the cumulative mass of the kept classes exceeds
  * uniform[r] times their total; logprob (may be NULL) is the log of its share of that total.  temperature[r] <= 0 (or
  * NaN) takes the first class, logprob 0.  temperature, top_k, top_p and min_p are DEVICE arrays of one number per row;
- * NULL: 1, and no filter.  uniform is in [0, 1); what is outside counts as the nearest end.  NaN logits count as -inf; a
- * row without any logit above -inf gives token -1 and logprob -inf; logits of +inf share all the mass.
+ * NULL: 1, and no filter; a NaN among the filters filters nothing.  uniform is in [0, 1); what is outside counts as the
+ * nearest end, NaN as 0.  NaN logits count as -inf; a row without any logit above -inf gives token -1 and logprob -inf;
+ * logits of +inf share all the mass.
  * Weights are rounded to multiples of 2^-51 of the row's largest (for more than 2^11 classes of 2^-(62 - ceil(log2 cols)))
  * and summed as integers, so a draw does not depend on the batch it is in.  cols <= 2^31 - 256. */
 typedef struct admm_sample_params {
