@@ -311,8 +311,8 @@ __device__ inline void draw_row(const SampleArgs &a, uint64_t r, const Params &q
 // A row that is left to a later kernel has the token kLeft.  One kernel for all of it took 43 us for a row of 128000 classes
 // with top-k, where k_sample_list takes 18, and 290 for 512 rows with top-p.  512 rows of 128000 in 16 bits with top-p: tops 21
 // us (131 MB at 6.2 TB/s), sums 75 (bound by arithmetic: 33 instructions a class, most of them in 64 bits, issued three quarters
-// of the time), rest 58 (17 for the border's bucket, 9 for the draw, 12 of steps of one row behind another; rows that share a CU
-// with a slower one end last).
+// of the time), rest 58 (17 for the border's bucket, 7 for the draw, 12 of steps that wait for each other; rows that share a CU with
+// a slower one end last).
 
 constexpr int kGroup = 32;       // granules
 constexpr int kTopsPer = 512;    // granules per workgroup of k_sample_tops
@@ -493,39 +493,67 @@ __device__ inline void draw_held(const SampleArgs &a, uint64_t r, const Params &
     if (amount[i] && index[i] == token) write_token(a, r, (uint32_t)token, logit_of((uint32_t)(h.o[i] >> a.index_bits)), weight, q.t, total);
 }
 
-// The first class, in the order of the indexes, at which the amounts of the granules [c0, c1) reach `target`; visit(x, j) is
-// a class's amount, hit(x, j) gets the class.
+// The first class, in the order of the indexes, at which the amounts of the granules [c0, c1) reach `target`; amount(x, j) is a
+// class's, hit(x, j) gets the class.  Every wave leaves the sums of eight of its steps of 64 granules, then all look among the 64
+// sums, and the wave that has the class goes through that step again.  (With all waves looking after every step: 512 rows of
+// 128000 floats 131 us instead of 122, but 512 of 5000 20 instead of 21.)
 template <class T, class Amount, class Hit>
 __device__ inline void find_class(const Chunks<T, 8> &row, int c0, int c1, unsigned long long target, Shared &sh, Amount amount, Hit hit) {
-  constexpr int K = 8 / sizeof(T);
+  constexpr int K = 8 / sizeof(T), kWaves = kThreads / 64, kSteps = 64 / kWaves;
   const T none = (T)-INFINITY;
-  vec_t<T, K> x = none, next = none;
-  if (c0 + (int)threadIdx.x < c1) next = row.load(c0 + (int)threadIdx.x, none);
-  for (int b = c0; b < c1; b += kThreads) {
-    const int c = b + (int)threadIdx.x;
-    x = next;
-    next = none;
-    if (c + kThreads < c1) next = row.load(c + kThreads, none);
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  auto load = [&](int c) {
+    vec_t<T, K> x = none;
+    if (c < c1) x = row.load(c, none);
+    return x;
+  };
+  auto scan = [&](unsigned long long v) {
+    for (int off = 1; off < 64; off <<= 1) {
+      const unsigned long long y = __shfl_up(v, off, 64);
+      if (lane >= off) v += y;
+    }
+    return v;
+  };
+  for (int b = c0; b < c1; b += kSteps * kThreads) {
+    __syncthreads();
+    vec_t<T, K> x[kSteps];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) x[i] = load(b + i * kThreads + (int)threadIdx.x);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int c = b + i * kThreads + (int)threadIdx.x;
+      unsigned long long mine = 0;
+      if (b + i * kThreads < c1) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) mine += amount((float)x[i][k], row.column(c, k));
+        for (int off = 1; off < 64; off <<= 1) mine += __shfl_xor(mine, off, 64);
+      }
+      if (lane == 0) sh.hist[i * kWaves + wave] = mine;
+    }
+    __syncthreads();
+    const unsigned long long sum = sh.hist[lane], up = scan(sum), all = __shfl(up, 63, 64);
+    if (all < target) {  // uniform
+      target -= all;
+      continue;
+    }
+    const int at = __ffsll((unsigned long long)__ballot(up >= target)) - 1;
+    if (wave != at % kWaves) return;
+    unsigned long long before = __shfl(up - sum, at, 64);
+    const int c = b + at / kWaves * kThreads + (int)threadIdx.x;
+    const vec_t<T, K> y = load(c);
     unsigned long long u[K], mine = 0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      u[k] = amount((float)x[k], row.column(c, k));
+      u[k] = amount((float)y[k], row.column(c, k));
       mine += u[k];
     }
-    __syncthreads();
-    const unsigned long long all = find_value(sh, mine, target);
-    if (all >= target) {  // uniform
-      if (sh.found == threadIdx.x) {
-        unsigned long long sum = sh.before;
+    before += scan(mine) - mine;
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          if (sum < target && target <= sum + u[k]) hit((float)x[k], row.column(c, k));
-          sum += u[k];
-        }
-      }
-      return;
+    for (int k = 0; k < K; ++k) {
+      if (before < target && target <= before + u[k]) hit((float)y[k], row.column(c, k));
+      before += u[k];
     }
-    target -= all;
+    return;
   }
 }
 
