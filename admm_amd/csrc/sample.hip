@@ -495,8 +495,8 @@ __device__ inline void draw_held(const SampleArgs &a, uint64_t r, const Params &
 
 // The first class, in the order of the indexes, at which the amounts of the granules [c0, c1) reach `target`; amount(x, j) is a
 // class's, hit(x, j) gets the class.  Every wave leaves the sums of eight of its steps of 64 granules, then all look among the 64
-// sums, and the wave that has the class goes through that step again.  (With all waves looking after every step: 512 rows of
-// 128000 floats 131 us instead of 122, but 512 of 5000 20 instead of 21.)
+// sums, and the wave that has the class goes through that step again; a single step is looked at by all.  (All looking after
+// every step: 512 rows of 128000 floats 131 us instead of 122; the sums for a single step too: 4096 rows of 5000 144, not 134.)
 template <class T, class Amount, class Hit>
 __device__ inline void find_class(const Chunks<T, 8> &row, int c0, int c1, unsigned long long target, Shared &sh, Amount amount, Hit hit) {
   constexpr int K = 8 / sizeof(T), kWaves = kThreads / 64, kSteps = 64 / kWaves;
@@ -514,6 +514,32 @@ __device__ inline void find_class(const Chunks<T, 8> &row, int c0, int c1, unsig
     }
     return v;
   };
+  unsigned long long u[K];
+  auto amounts = [&](const vec_t<T, K> &x, int c) {
+    unsigned long long sum = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      u[k] = amount((float)x[k], row.column(c, k));
+      sum += u[k];
+    }
+    return sum;
+  };
+  auto hit_among = [&](const vec_t<T, K> &x, int c, unsigned long long before) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (before < target && target <= before + u[k]) hit((float)x[k], row.column(c, k));
+      before += u[k];
+    }
+  };
+  if (c1 - c0 <= kThreads) {
+    const int c = c0 + (int)threadIdx.x;
+    const vec_t<T, K> x = load(c);
+    const unsigned long long mine = amounts(x, c);
+    __syncthreads();
+    find_value(sh, mine, target);
+    if (sh.found == threadIdx.x) hit_among(x, c, sh.before);
+    return;
+  }
   for (int b = c0; b < c1; b += kSteps * kThreads) {
     __syncthreads();
     vec_t<T, K> x[kSteps];
@@ -538,21 +564,13 @@ __device__ inline void find_class(const Chunks<T, 8> &row, int c0, int c1, unsig
     }
     const int at = __ffsll((unsigned long long)__ballot(up >= target)) - 1;
     if (wave != at % kWaves) return;
-    unsigned long long before = __shfl(up - sum, at, 64);
+    const unsigned long long before = __shfl(up - sum, at, 64);
     const int c = b + at / kWaves * kThreads + (int)threadIdx.x;
-    const vec_t<T, K> y = load(c);
-    unsigned long long u[K], mine = 0;
+    vec_t<T, K> y = x[0];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      u[k] = amount((float)y[k], row.column(c, k));
-      mine += u[k];
-    }
-    before += scan(mine) - mine;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if (before < target && target <= before + u[k]) hit((float)y[k], row.column(c, k));
-      before += u[k];
-    }
+    for (int i = 1; i < kSteps; ++i) y = i == at / kWaves ? x[i] : y;
+    const unsigned long long mine = amounts(y, c);
+    hit_among(y, c, before + scan(mine) - mine);
     return;
   }
 }
@@ -865,13 +883,16 @@ __global__ void __launch_bounds__(kThreads) k_sample_rest(SampleArgs a, uint64_t
   draw_row(a, r, q, weight, (unsigned long long)key_of(top) << a.index_bits | first, RowSource<T>{row.base + row.lead, row.cols}, s.sh);
 }
 
-constexpr uint64_t kSmallCols = 1024;
-
 // ---- rows of up to 1024 classes ------------------------------------------------------------------------
 //
 // In one launch: LANES lanes hold a row, EACH consecutive classes a lane, and sort its keys in their registers (bitonic: the
 // partner of position p is p ^ j, in the same lane for j < EACH).  The sums over the sorted classes say which is the last that
-// is kept, those over the classes where they are give the token.  No row is left to anyone else.
+// is kept, those over the classes where they are give the token.  No row is left to anyone else.  With more than kLaneCols
+// classes the sort is long for one wave (33 us where the kernels above take 23), so that fewer than kSmallRows rows that need
+// it go there: 64 rows of 1000 with top-k 33 and 24 us, 512 35 and 32, with top-p 37 and 41, 8192 137 and 417; without either
+// filter there is no sort and this is faster, 64 rows 8 and 13.
+constexpr uint64_t kSmallCols = 1024, kLaneCols = 512, kSmallRows = 512;
+
 template <class T, int LANES, int EACH>
 __global__ void __launch_bounds__(256) k_sample_small(SampleArgs a) {
   const int lane = (int)threadIdx.x & (LANES - 1);
@@ -1030,7 +1051,7 @@ static uint64_t tops_bytes(uint64_t rows, uint64_t groups) { return round_up(row
 
 template <class T>
 static int sample(admm_ctx *ctx, SampleArgs a, void *workspace) {
-  if (a.cols <= kSmallCols) {
+  if (a.cols <= kLaneCols || (a.cols <= kSmallCols && (a.rows >= kSmallRows || !(a.top_k || a.top_p)))) {
 #define ADMM_SMALL(LANES, EACH) hipLaunchKernelGGL((k_sample_small<T, LANES, EACH>), dim3(blocks_for(a.rows, 256 / LANES)), dim3(256), 0, ctx->stream, a)
     if (a.cols <= 16) ADMM_SMALL(16, 1);
     else if (a.cols <= 64) ADMM_SMALL(64, 1);
@@ -1074,7 +1095,7 @@ extern "C" int admm_sample_workspace(uint64_t rows, uint64_t cols, uint64_t *byt
   ADMM_REQUIRE(rows < (1ull << 40) && cols <= kMaxClasses, "admm_sample_workspace: %llu x %llu logits", (unsigned long long)rows,
                (unsigned long long)cols);
   *bytes = 0;
-  if (cols <= kSmallCols) return ADMM_OK;
+  if (cols <= kLaneCols || (cols <= kSmallCols && rows >= kSmallRows)) return ADMM_OK;
   // enough for logits of any type: granules of four floats are the most
   *bytes = tops_bytes(rows, tops_groups(cols, 4)) + (rows < kBatch ? rows : kBatch) * (kParts * kSums * sizeof(unsigned long long));
   return ADMM_OK;

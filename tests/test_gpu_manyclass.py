@@ -522,6 +522,30 @@ def test_sample_where_the_form_changes(ctx, kind, cols):
     check_sample(ctx, x, u)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,cols", [(511, 513), (512, 513), (512, 1024), (530, 777)])
+def test_sample_of_many_short_rows(ctx, kind, rows, cols):
+    """rows enough that each is sorted by one wave, with every filter"""
+    g = rng(23, rows, cols)
+    rs = np.random.RandomState(rows + cols)
+    x = make_logits(rows, cols, kind, g, 2.0)
+    x[1] = x[1, 0]
+    x[2, ::2] = -math.inf
+    x[3, cols // 3:] = math.nan
+    x[4, [cols // 2, cols - 1]] = math.inf
+    x[5] = -math.inf
+    u = rs.rand(rows).astype(np.float32)
+    u[6:9] = [0.0, -1.0, 1.0]
+    pick = lambda v, off: np.where(rs.rand(rows) < 0.5, off, v)  # noqa: E731
+    t, k = pick(rs.uniform(0.3, 2, rows), 1.0), pick(rs.randint(1, cols + 1, rows), 0)
+    p, m = pick(rs.uniform(0.05, 1, rows), 1.0), pick(rs.uniform(0.001, 0.9, rows), 0.0)
+    t[rs.rand(rows) < 0.1] = 0
+    check_sample(ctx, x, u, t, k=k, p=p, m=m)
+    check_sample(ctx, x, u, t, k=k)
+    check_sample(ctx, x, u, t, p=p)
+    check_sample(ctx, x, u, m=m)
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("cols", [3000, 50000])
 def test_sample_of_many_candidates(ctx, kind, cols):
