@@ -75,8 +75,9 @@ __device__ inline void add_groups(int lanes_log2, float (&acc)[N]) {
 }
 
 // Rows of several ids.  WAVES waves share a row (1, or 16 for few long ones), each of them as 64 /
-// 2^lanes_log2 groups of lanes that take entries in turn.  65536 rows of 40 entries over 16 floats: 36 us, bound by the units
-// that form the addresses (2 clocks for the 16 bytes of a lane: 2.6 million entries of 4 lanes), not by the 75 MB that come.
+// 2^lanes_log2 groups of lanes that take entries in turn.  65536 rows of 40 entries over 16 floats: 36 us, bound by requests
+// (2.6 million rows of 64 bytes in four 16-byte lanes each; the units that form the addresses are busy for half of the time, and an
+// entry is two reads one behind the other), not by the 75 MB that come.  65536 x 40 x 256: 441 us, 6.1 TB/s.
 template <class T, class TO, int N, class Id, int WAVES>
 __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
     k_embed_bags(const Id *__restrict__ ids, const uint64_t *__restrict__ rowptr, const float *__restrict__ val, uint64_t nrows,
@@ -673,7 +674,7 @@ __global__ void __launch_bounds__(256) k_grad(GradArgs<T, TO> a) {
 
 // Runs that go over the end of the chunk they begin in: the sums of their parts, in the order of the chunks.  Runs of up to
 // kShort chunks after the first are summed by a group of lanes each; longer ones by a workgroup, which looks for them in
-// kSet chunks at a time.  Bound by latency: 29 us for 82000 chunks of which most end inside a run, and 7 for 501.
+// kSet chunks at a time.  Bound by latency: 17 us for 82000 chunks of which most end inside a run, and 6 for 501.
 constexpr int kShort = 7, kSet = 16;
 
 template <class T, class TO>
