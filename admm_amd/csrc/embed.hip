@@ -899,8 +899,9 @@ static int sort_entries(admm_ctx *ctx, const admm_bags *b, uint32_t trows, char 
     if (b->rowptr)
       hipLaunchKernelGGL(k_entry_rows, dim3(blocks_for(b->nrows, 16)), dim3(256), 0, ctx->stream, b->rowptr, b->nrows, b->nnz, u32(at.row_of));
     const size_t lds = 4 * (17 * 256 + 32 + 2 * (size_t)n);
-    ADMM_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&k_sort_small<Id>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                       4 * (17 * 256 + 32 + 2 * kSortSmall)));
+    if (lds > 64 * 1024)
+      ADMM_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&k_sort_small<Id>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                         4 * (17 * 256 + 32 + 2 * kSortSmall)));
     hipLaunchKernelGGL(k_sort_small<Id>, dim3((n + 511) / 512), dim3(1024), lds, ctx->stream, ids, n, trows, to);
     ADMM_HIP_CHECK(hipGetLastError());
     return ADMM_OK;

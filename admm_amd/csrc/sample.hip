@@ -24,8 +24,9 @@ struct SampleArgs {
   int32_t *token;
   float *logprob;
   int index_bits, shift;  // 2^index_bits >= cols; S
-  float *tops;            // [rows][groups] largest logits of kGroup granules each
+  float *tops;            // [rows][groups] largest logits of 2^group_log2 granules each
   int64_t groups;
+  int group_log2;
   unsigned long long *sums;  // [rows of a batch][kParts][kSums]
   int split;                 // workgroups per part that add to its sums; more than one where there are few rows
 };
@@ -297,8 +298,8 @@ __device__ inline void draw_row(const SampleArgs &a, uint64_t r, const Params &q
 
 // ---- rows in a few launches ----------------------------------------------------------------------------
 //
-//  * k_sample_tops reads the logits once, with as many workgroups as there are, and leaves the largest logit of every kGroup
-//    granules.  What follows knows from those the row's largest logit and reads the row again from the caches.
+//  * k_sample_tops reads the logits once, with as many workgroups as there are, and leaves the largest logit of every group
+//    of granules.  What follows knows from those the row's largest logit and reads the row again from the caches.
 //  * k_sample_list (where top-k is given), a workgroup per row: the k-th largest logit is not below the k-th largest of the
 //    groups'.  The classes from that bound on are few; everything else happens among them in LDS.
 //  * k_sample_sums (the rows without top-k), kParts workgroups per row, or up to eight times as many for few rows: for top-p
@@ -314,7 +315,6 @@ __device__ inline void draw_row(const SampleArgs &a, uint64_t r, const Params &q
 // of the time), rest 58 (17 for the border's bucket, 7 for the draw, 12 of steps that wait for each other; rows that share a CU with
 // a slower one end last).
 
-constexpr int kGroup = 32;       // granules
 constexpr int kTopsPer = 512;    // granules per workgroup of k_sample_tops
 constexpr int kMaxGroups = 4096; // groups whose largest logits fit LDS beside the rest
 constexpr int kList = kHeld * kThreads;  // classes kept in LDS
@@ -394,9 +394,9 @@ __global__ void __launch_bounds__(256) k_sample_tops(SampleArgs a) {
     float m = -INFINITY;
 #pragma unroll
     for (int k = 0; k < K; ++k) m = fmaxf(m, (float)x[i][k]);
-    for (int off = 1; off < kGroup; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-    const int g = (c0 + i * 256) / kGroup;
-    if (threadIdx.x % kGroup == 0 && g < a.groups) a.tops[(uint64_t)blockIdx.y * a.groups + g] = m;
+    for (int off = 1; off < 1 << a.group_log2; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    const int g = (c0 + i * 256) >> a.group_log2;
+    if ((threadIdx.x & ((1u << a.group_log2) - 1)) == 0 && g < a.groups) a.tops[(uint64_t)blockIdx.y * a.groups + g] = m;
   }
 }
 
@@ -759,8 +759,8 @@ __global__ void __launch_bounds__(kThreads) k_sample_list(SampleArgs a) {
     __syncthreads();
     const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int)a.cols);
     const Params q = params_of(a, r);
-    const int small = (row.count + kGroup - 1) / kGroup, size = (small + kMaxGroups - 1) / kMaxGroups;
-    const int groups = (small + size - 1) / size;  // of `size` times kGroup granules
+    const int small = (row.count + (1 << a.group_log2) - 1) >> a.group_log2, size = (small + kMaxGroups - 1) / kMaxGroups;
+    const int groups = (small + size - 1) / size;  // of `size` times 2^group_log2 granules
     // the groups' largest logits, and the row's
     float top = -INFINITY;
     for (int g = threadIdx.x; g < groups; g += kThreads) {
@@ -807,7 +807,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_list(SampleArgs a) {
     __syncthreads();
     // the classes from the bound on
     unsigned long long first = ~0ull;
-    const unsigned per = (unsigned)(size * kGroup), granules = s.nhits * per;  // at most the row's 2^31 / K and kMaxGroups' rounding
+    const unsigned per = (unsigned)(size << a.group_log2), granules = s.nhits * per;  // at most the row's 2^31 / K and kMaxGroups' rounding
     for (unsigned i = threadIdx.x; i < granules; i += 4 * kThreads) {
       vec_t<T, K> x[4];
       int c[4];
@@ -1045,7 +1045,22 @@ __global__ void __launch_bounds__(256) k_sample_small(SampleArgs a) {
   }
 }
 
-static uint64_t tops_groups(uint64_t cols, uint64_t per) { return ((cols + per - 1) / per + 1 + kGroup - 1) / kGroup; }
+// Granules per group: as many groups as a wave can hold in registers, 256 to 512, so that a large k has its groups too; rows of
+// more than 2^14 granules have more groups, of 32 granules.  (With groups of 32 whatever the row, us for k = 50 and 200: 64 rows
+// of 5000 floats 34 and 36, 64 of 32000 halves 21 and 137, 2048 of 32000 halves 149 and 912; so: 18 and 27, 19 and 31, 129 and
+// 225.)
+static int tops_group_log2(uint64_t granules) {
+  int log2 = 0;
+  while (log2 < 5 && (granules >> log2) >= 512) ++log2;
+  return log2;
+}
+
+// groups of a row, whatever its alignment
+static uint64_t tops_groups(uint64_t cols, uint64_t per) {
+  const uint64_t granules = (cols + per - 1) / per + 1;
+  const int log2 = tops_group_log2(granules);
+  return (granules + (1ull << log2) - 1) >> log2;
+}
 
 static uint64_t tops_bytes(uint64_t rows, uint64_t groups) { return round_up(rows * groups * sizeof(float), 256); }
 
@@ -1064,11 +1079,12 @@ static int sample(admm_ctx *ctx, SampleArgs a, void *workspace) {
     return ADMM_OK;
   }
   a.groups = (int64_t)tops_groups(a.cols, 16 / sizeof(T));
+  a.group_log2 = tops_group_log2((a.cols + 16 / sizeof(T) - 1) / (16 / sizeof(T)) + 1);
   a.tops = static_cast<float *>(workspace);
   a.sums = reinterpret_cast<unsigned long long *>(static_cast<char *>(workspace) + tops_bytes(a.rows, a.groups));
   const dim3 block(kThreads);
   a.split = a.rows * kParts >= 512 ? 1 : (int)(512 / (a.rows * kParts) < 8 ? 512 / (a.rows * kParts) : 8);
-  const unsigned per_row = (unsigned)((a.groups * kGroup + kTopsPer - 1) / kTopsPer);
+  const unsigned per_row = (unsigned)(((a.groups << a.group_log2) + kTopsPer - 1) / kTopsPer);
   for (uint64_t r = 0; r < a.rows; r += 65535) {  // rows are the second dimension of the grid
     SampleArgs b = a;
     b.logits = static_cast<const T *>(a.logits) + r * a.stride;
@@ -1096,8 +1112,9 @@ extern "C" int admm_sample_workspace(uint64_t rows, uint64_t cols, uint64_t *byt
                (unsigned long long)cols);
   *bytes = 0;
   if (cols <= kLaneCols || (cols <= kSmallCols && rows >= kSmallRows)) return ADMM_OK;
-  // enough for logits of any type: granules of four floats are the most
-  *bytes = tops_bytes(rows, tops_groups(cols, 4)) + (rows < kBatch ? rows : kBatch) * (kParts * kSums * sizeof(unsigned long long));
+  // enough for logits of any type: granules of four floats or of eight halves
+  const uint64_t wide = tops_groups(cols, 4), narrow = tops_groups(cols, 8);
+  *bytes = tops_bytes(rows, wide > narrow ? wide : narrow) + (rows < kBatch ? rows : kBatch) * (kParts * kSums * sizeof(unsigned long long));
   return ADMM_OK;
 }
 
