@@ -234,25 +234,25 @@ struct Sorted {
 
 // Up to kSortSmall entries, in one launch: every workgroup looks at all keys and sorts those of its own range of them in its
 // LDS; how many are below its range says where they go.  (All passes over all keys in one workgroup: 17.5 us for 4001 keys of
-// 15 bits; this: 10, and 17 for 16384 keys of 17 bits.)
-template <class Id>
+// 15 bits; this: 8, and 12.5 for 16384 keys of 17 bits.  Keys loaded one after the other instead of all at once: 10 and 17.)
+template <class Id, int kItems>
 __global__ void __launch_bounds__(1024) k_sort_small(const Id *__restrict__ ids, uint32_t n, uint32_t trows, Sorted to) {
-  constexpr int kItems = kSortSmall / 1024;
   extern __shared__ uint32_t sort_sh[];  // counters [16][256], totals [256], 16 + 16 counts of the waves, keys [n], entries [n]
   uint32_t *counters = sort_sh, *totals = counters + 16 * 256, *mine = totals + 256, *less = mine + 16, *keys = less + 16, *entries = keys + n;
   const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t width = (uint32_t)(((uint64_t)trows + gridDim.x) / gridDim.x);  // of the trows + 1 keys
   const uint64_t from = (uint64_t)width * blockIdx.x, to_key = from + width;
   uint32_t key[kItems], entry[kItems];
-  int items = (int)((n + 1023) / 1024);
   // a wave's items are consecutive, so what it keeps of them follows the order
-  const uint32_t base = wave * (uint32_t)(items * 64) + lane;
+  const uint32_t base = wave * (uint32_t)(kItems * 64) + lane;
   uint32_t kept = 0, below = 0;
+  Id id[kItems];  // all on the way before the first is looked at
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) id[i] = ids[base + i * 64 < n ? base + i * 64 : n - 1];
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
-    if (i >= items) break;
     const uint32_t at = base + i * 64;
-    key[i] = at < n ? key_of(ids[at], trows) : 0xFFFFFFFFu;
+    key[i] = at < n ? key_of(id[i], trows) : 0xFFFFFFFFu;
     const bool in = at < n && key[i] >= from && key[i] < to_key;
     const unsigned long long on = __ballot(in);
     below += (uint32_t)__popcll(__ballot(key[i] < from));
@@ -272,7 +272,6 @@ __global__ void __launch_bounds__(1024) k_sort_small(const Id *__restrict__ ids,
   }
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
-    if (i >= items) break;
     if (entry[i] == 0xFFFFFFFFu) continue;
     keys[place + entry[i]] = key[i] - (uint32_t)from;
     entries[place + entry[i]] = base + i * 64;
@@ -281,7 +280,7 @@ __global__ void __launch_bounds__(1024) k_sort_small(const Id *__restrict__ ids,
   int bits = 0;
   while (bits < 32 && (width - 1) >> bits) ++bits;
   const int passes = (bits + 7) / 8, digits = passes ? (bits + passes - 1) / passes : 0;
-  items = (int)((count + 1023) / 1024);
+  const int items = (int)((count + 1023) / 1024);
   const uint32_t b2 = wave * (uint32_t)(items * 64) + lane;
   for (int p = 0; p < passes; ++p) {
     uint32_t digit[kItems], rank[kItems];
@@ -899,10 +898,18 @@ static int sort_entries(admm_ctx *ctx, const admm_bags *b, uint32_t trows, char 
     if (b->rowptr)
       hipLaunchKernelGGL(k_entry_rows, dim3(blocks_for(b->nrows, 16)), dim3(256), 0, ctx->stream, b->rowptr, b->nrows, b->nnz, u32(at.row_of));
     const size_t lds = 4 * (17 * 256 + 32 + 2 * (size_t)n);
-    if (lds > 64 * 1024)
-      ADMM_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&k_sort_small<Id>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                         4 * (17 * 256 + 32 + 2 * kSortSmall)));
-    hipLaunchKernelGGL(k_sort_small<Id>, dim3((n + 511) / 512), dim3(1024), lds, ctx->stream, ids, n, trows, to);
+    auto launch = [&](auto kernel) -> int {
+      if (lds > 64 * 1024)
+        ADMM_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                           4 * (17 * 256 + 32 + 2 * kSortSmall)));
+      hipLaunchKernelGGL(kernel, dim3((n + 511) / 512), dim3(1024), lds, ctx->stream, ids, n, trows, to);
+      return ADMM_OK;
+    };
+    // keys a thread looks at: about as many as there are (8192 entries: 7.8 us with 8, 10.2 with 16)
+    ADMM_TRY(n <= 1024   ? launch(&k_sort_small<Id, 1>)
+             : n <= 4096 ? launch(&k_sort_small<Id, 4>)
+             : n <= 8192 ? launch(&k_sort_small<Id, 8>)
+                         : launch(&k_sort_small<Id, kSortSmall / 1024>));
     ADMM_HIP_CHECK(hipGetLastError());
     return ADMM_OK;
   }
