@@ -799,6 +799,19 @@ def test_nothing_to_do(ctx):
     assert torch.all(out == 0)
 
 
+def test_entries_without_any_row(ctx):
+    """row pointers of no row: the gradient is zero, or left as it was, and nothing of grad_out is read (it has no memory)"""
+    for n in (5, 100, 20000):
+        bags = ctx.bags(torch.randint(0, 50, (n,), device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda"))
+        order = ctx.embed_order(bags, 50)
+        grad = torch.full((50, 8), 3.0, device="cuda")
+        ctx.embed_grad(bags, order, torch.empty(0, 8, device="cuda"), grad, accumulate=True)
+        assert torch.all(grad == 3.0)
+        ctx.embed_grad(bags, order, torch.empty(0, 8, device="cuda"), grad)
+        assert torch.all(grad == 0.0)
+        ctx.embed(bags, torch.ones(50, 8, device="cuda"), torch.empty(0, 8, device="cuda"))
+
+
 def test_more_elements_than_32_bits_count(ctx):
     """a table and logits of more than 2^32 elements: rows at both ends"""
     vocab, cols = 1 << 20, 4104
