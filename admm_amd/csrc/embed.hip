@@ -230,6 +230,28 @@ struct Sorted {
     const uint32_t r = row_of[entry];
     return r < nrows && rowptr[r] <= entry && entry < rowptr[r + 1] ? r : 0xFFFFFFFFu;
   }
+  // of several entries, whose loads are on the way together
+  template <int N>
+  __device__ void rows_of(const uint32_t (&entry)[N], uint32_t (&out)[N]) const {
+    uint64_t from[N], end[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = row_of ? row_of[entry[i]] : entry[i];
+    if (!row_of) return;
+    if (nrows == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) out[i] = 0xFFFFFFFFu;
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t r = out[i] < nrows ? out[i] : nrows - 1;
+      from[i] = rowptr[r];
+      end[i] = rowptr[(uint64_t)r + 1];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (out[i] >= nrows || entry[i] < from[i] || entry[i] >= end[i]) out[i] = 0xFFFFFFFFu;
+  }
 };
 
 // Up to kSortSmall entries, in one launch: every workgroup looks at all keys and sorts those of its own range of them in its
@@ -335,7 +357,7 @@ __global__ void __launch_bounds__(256) k_entry_rows(const uint64_t *__restrict__
 // counts itself (counts by tile, then digit), which saves a launch a pass (32000 entries: 47 us instead of 53 with the
 // gradient; 98 tiles: 59 instead of 56); from more of them the sums are made by a launch of their own (counts by digit, then
 // tile).  The first count also finds the entries' rows, with workgroups of its own.  2.6 million entries with factors over 2^20
-// ids: 3 passes, 102 us in all, of which the moves 58 and the counts 28; what they read and write would take 25.
+// ids: 3 passes, 95 us in all, of which the moves 53 and the counts 27; what they read and write would take 25.
 constexpr uint32_t kFewTiles = 48;
 
 template <class Id, bool FIRST>
@@ -355,11 +377,15 @@ __global__ void __launch_bounds__(256) k_sort_count(const Id *__restrict__ ids, 
   hist[threadIdx.x] = 0;
   __syncthreads();
   const uint32_t base = blockIdx.x * (uint32_t)TILE;
-#pragma unroll 4
+  uint32_t key[TILE / 256];
+#pragma unroll
   for (int i = 0; i < TILE / 256; ++i) {
     const uint32_t at = base + i * 256 + threadIdx.x;
-    if (at < n) atomicAdd(&hist[(sort_key<Id, FIRST>(ids, keys, at, trows) >> shift) & ((1u << width) - 1)], 1u);
+    key[i] = sort_key<Id, FIRST>(ids, keys, at < n ? at : n - 1, trows);
   }
+#pragma unroll
+  for (int i = 0; i < TILE / 256; ++i)
+    if (base + i * 256 + threadIdx.x < n) atomicAdd(&hist[(key[i] >> shift) & ((1u << width) - 1)], 1u);
   __syncthreads();
   if (threadIdx.x < (1u << width))
     counts[tiles <= kFewTiles ? (uint64_t)blockIdx.x * 256 + threadIdx.x : (uint64_t)threadIdx.x * tiles + blockIdx.x] = hist[threadIdx.x];
@@ -415,20 +441,37 @@ __global__ void __launch_bounds__(256) k_sort_move(const Id *__restrict__ ids, c
   const uint32_t base = wave * (kItems * 64) + lane, mask = (1u << width) - 1;
   uint32_t key[kItems], digit[kItems], rank[kItems];
   Load load[kItems];
+  // step by step for all items, so that each step's loads are on the way together; beyond the end the last entry is read
+  uint32_t at[kItems];
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) at[i] = tile + (base + i * 64 < count ? base + i * 64 : count - 1);
+  if (FIRST) {
+    Id id[kItems];
+    uint32_t row[kItems];
+    float val[kItems];
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) id[i] = ids[at[i]];
+    if (sizeof(Load) == 8) {
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) val[i] = to.val_of[at[i]];
+    }
+    to.rows_of(at, row);
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      key[i] = key_of(id[i], trows);
+      load[i] = row[i];
+      if (sizeof(Load) == 8) load[i] |= (Load)((unsigned long long)__float_as_uint(val[i]) << 32);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      key[i] = keys[at[i]];
+      load[i] = loads[at[i]];
+    }
+  }
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
-    const uint32_t in = base + i * 64, at = tile + in;
-    key[i] = 0xFFFFFFFFu;
-    load[i] = 0;
-    if (in < count) {
-      key[i] = sort_key<Id, FIRST>(ids, keys, at, trows);
-      if (FIRST) {
-        load[i] = to.row(at);
-        if (sizeof(Load) == 8) load[i] |= (Load)((unsigned long long)__float_as_uint(to.val_of[at]) << 32);
-      } else {
-        load[i] = loads[at];
-      }
-    }
+    if (base + i * 64 >= count) key[i] = 0xFFFFFFFFu;
     digit[i] = (key[i] >> shift) & mask;
   }
   for (int i = threadIdx.x; i < 4 * 256; i += 256) counters[i] = 0;
@@ -465,15 +508,15 @@ __global__ void __launch_bounds__(256) k_sort_move(const Id *__restrict__ ids, c
   __syncthreads();
 #pragma unroll 4
   for (uint32_t i = threadIdx.x; i < count; i += 256) {
-    const uint32_t k = tile_keys[i], at = start[(k >> shift) & mask] + i;
+    const uint32_t k = tile_keys[i], place = start[(k >> shift) & mask] + i;
     const Load l = tile_loads[i];
     if (LAST) {
-      to.ids[at] = k;
-      to.rows[at] = (uint32_t)l;
-      if (sizeof(Load) == 8) to.val[at] = __uint_as_float((uint32_t)((unsigned long long)l >> 32));
+      to.ids[place] = k;
+      to.rows[place] = (uint32_t)l;
+      if (sizeof(Load) == 8) to.val[place] = __uint_as_float((uint32_t)((unsigned long long)l >> 32));
     } else {
-      keys_to[at] = k;
-      loads_to[at] = l;
+      keys_to[place] = k;
+      loads_to[place] = l;
     }
   }
 }
