@@ -668,34 +668,44 @@ __global__ void __launch_bounds__(256) k_grad(GradArgs<T, TO> a) {
   } else {
     const uint32_t nsets = (uint32_t)(((uint64_t)a.trows + 63) / 64);
     for (uint32_t q = (blockIdx.x - a.chunk_blocks) * 4 + p.wave; q < nsets; q += a.zero_blocks * 4) {
-      // which of the 64 rows from v0 on have entries
+      // Which of the 64 rows from v0 on have entries: the first position whose id is at least v0, 64 probes at a time; then the ids
+      // of the next 64 entries, of 448 more if those do not reach the end of the set, and if there are still more, every lane
+      // looks for its own row.  (64 probes for every id behind 64 entries: 23 us for 9096 entries of 262 ids; this: 10.)
       const uint32_t v0 = q * 64;
-      unsigned long long there = 0;
-      uint32_t next = v0;  // rows before it are known
-      while (next - v0 < 64) {
-        // first position whose id is at least `next`, 64 probes at a time
-        uint32_t lo = 0, hi = a.n;
-        while (hi > lo) {
-          const uint32_t step = (hi - lo + 63) / 64;
-          const uint64_t at = lo + (uint64_t)p.lane * step;
-          const int small = __popcll(__ballot(at < hi && a.ids[at < hi ? at : hi - 1] < next));  // the first `small` probes are below
-          if (small == 0) {
-            hi = lo;
-          } else {
-            const uint64_t to = lo + (uint64_t)small * step;
-            lo = lo + (uint32_t)(small - 1) * step + 1;
-            hi = to < hi ? (uint32_t)to : hi;
-          }
+      uint32_t lo = 0, hi = a.n;
+      while (hi > lo) {
+        const uint32_t step = (hi - lo + 63) / 64;
+        const uint64_t at = lo + (uint64_t)p.lane * step;
+        const int small = __popcll(__ballot(at < hi && a.ids[at < hi ? at : hi - 1] < v0));  // the first `small` probes are below
+        if (small == 0) {
+          hi = lo;
+        } else {
+          const uint64_t to = lo + (uint64_t)small * step;
+          lo = lo + (uint32_t)(small - 1) * step + 1;
+          hi = to < hi ? (uint32_t)to : hi;
         }
-        const uint32_t id = lo + p.lane < a.n ? a.ids[lo + p.lane] : 0xFFFFFFFFu;
-        const bool in = id - v0 < 64 && id < a.trows;
-        unsigned long long mark = in ? 1ull << (id - v0) : 0;
-        for (int off = 1; off < 64; off <<= 1) mark |= __shfl_xor(mark, off, 64);
-        there |= mark;
-        const uint32_t last = __shfl(id, 63, 64);
-        if (last - v0 >= 64) break;  // the ids from here on are beyond the set
-        next = last + 1;
       }
+      constexpr int kMore = 7;
+      uint64_t at = (uint64_t)lo + p.lane;
+      const uint32_t id = at < a.n ? a.ids[at] : 0xFFFFFFFFu;
+      unsigned long long there = id - v0 < 64 ? 1ull << (id - v0) : 0;  // an id beyond the table's end is not asked for below
+      if ((uint32_t)__shfl(id, 63, 64) - v0 < 64) {
+        uint32_t more[kMore];
+#pragma unroll
+        for (int i = 0; i < kMore; ++i) more[i] = at + 64 * (i + 1) < a.n ? a.ids[at + 64 * (i + 1)] : 0xFFFFFFFFu;
+#pragma unroll
+        for (int i = 0; i < kMore; ++i) there |= more[i] - v0 < 64 ? 1ull << (more[i] - v0) : 0;
+        if ((uint32_t)__shfl(more[kMore - 1], 63, 64) - v0 < 64) {
+          uint32_t from = lo, end = a.n;
+          while (from < end) {
+            const uint32_t mid = from + ((end - from) >> 1);
+            if (a.ids[mid] < v0 + p.lane) from = mid + 1;
+            else end = mid;
+          }
+          there |= from < a.n && a.ids[from] == v0 + p.lane ? 1ull << p.lane : 0;
+        }
+      }
+      for (int off = 1; off < 64; off <<= 1) there |= __shfl_xor(there, off, 64);
       if (!p.here) continue;
       float zero[N];
 #pragma unroll
