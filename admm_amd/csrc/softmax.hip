@@ -192,7 +192,7 @@ struct Edges {
 
 // Rows of any length, one workgroup each: whole granules, CH a thread, kept in registers (CH > 0) or read again (CH == 0), and
 // the edges' elements one a thread.
-// Read and written once, this is bound by memory where several rows are at work on a CU: 5.9 TB/s for 8192 rows of 32000 in 16
+// Read and written once, this is bound by memory where several rows are at work on a CU: 5.6 TB/s for 8192 rows of 32000 in 16
 // bits.  Rows of 10^5 halves fill the registers of a CU alone, and what it computes between reading and writing (two
 // exponentials an element) shows: 4.1 TB/s.  Neither keeping a part in LDS so that two rows fit (3.8) nor fetching the next row
 // as this one leaves the registers (4.0) nor reading twice (3.4) is faster.
