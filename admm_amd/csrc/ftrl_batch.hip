@@ -849,7 +849,14 @@ int ftrl_pass_persistent(admm_csr *csr, float *w, float *z, float *n, const floa
 __global__ void __launch_bounds__(256) k_max_fold(float *v, int n) {
   __shared__ float sh[4];
   float m = 0.0f;
-  for (int i = threadIdx.x; i < n; i += 256) m = fmaxf(m, v[i]);
+  constexpr int kAhead = 8;  // loads of a thread that are on the way at once
+  for (int i0 = threadIdx.x; i0 < n; i0 += kAhead * 256) {
+    float x[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) x[u] = v[i0 + u * 256 < n ? i0 + u * 256 : i0];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) m = fmaxf(m, x[u]);
+  }
   for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_down(m, off, 64));
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
   __syncthreads();
