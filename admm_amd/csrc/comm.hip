@@ -107,6 +107,7 @@ extern "C" int admm_comm_init(admm_ctx *ctx, int rank, int world, const void *un
 extern "C" int admm_allreduce_sum_f32(admm_ctx *ctx, float *buf, uint64_t n) {
   ADMM_REQUIRE(ctx && buf, "admm_allreduce_sum_f32: NULL argument");
   if (ctx->world == 1) return ADMM_OK;
+  ADMM_HIP_CHECK(use_device(ctx));
   ADMM_REQUIRE(ctx->comm, "admm_allreduce_sum_f32: world %d but no communicator (admm_comm_init)", ctx->world);
   // ncclFloat32 = 7, ncclSum = 0
   const int rc = g_rccl.all_reduce(buf, buf, (size_t)n, 7, 0, ctx->comm, ctx->stream);

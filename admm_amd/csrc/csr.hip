@@ -561,6 +561,7 @@ extern "C" int admm_csr_download(const admm_csr *csr, uint64_t *rowptr, uint32_t
   ADMM_REQUIRE(csr, "admm_csr_download: csr is NULL");
   ADMM_TRY(require_rows(csr, "admm_csr_download"));
   admm_ctx *ctx = csr->ctx;
+  ADMM_HIP_CHECK(use_device(ctx));
   ADMM_HIP_CHECK(hipStreamSynchronize(ctx->stream));
   if (rowptr) ADMM_HIP_CHECK(hipMemcpy(rowptr, csr->d_rowptr, sizeof(uint64_t) * (csr->nrows + 1), hipMemcpyDeviceToHost));
   if (col && csr->nnz) {
@@ -685,6 +686,7 @@ extern "C" int admm_csr_relabel_by_frequency(admm_csr *csr) {
 extern "C" int admm_csr_set_lean(admm_csr *csr, int on) {
   ADMM_REQUIRE(csr, "admm_csr_set_lean: csr is NULL");
   ADMM_REQUIRE(!csr->rows_released || on, "admm_csr_set_lean: the rows are gone already");
+  ADMM_HIP_CHECK(use_device(csr->ctx));
   csr->lean = on != 0;
   if (csr->lean && csr->hot_dense) {
     ADMM_TRY(release_row_major(csr));

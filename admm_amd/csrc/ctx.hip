@@ -482,12 +482,14 @@ extern "C" int admm_ctx_destroy(admm_ctx *ctx) {
 
 extern "C" int admm_sync(admm_ctx *ctx) {
   ADMM_REQUIRE(ctx, "admm_sync: ctx is NULL");
+  ADMM_HIP_CHECK(use_device(ctx));
   ADMM_HIP_CHECK(hipStreamSynchronize(ctx->stream));
   return check_device_reports(ctx);
 }
 
 extern "C" int admm_timing_enable(admm_ctx *ctx, int on) {
   ADMM_REQUIRE(ctx, "admm_timing_enable: ctx is NULL");
+  ADMM_HIP_CHECK(use_device(ctx));
   if (!on) ADMM_TRY(timing_flush(ctx));
   ctx->timing = on != 0;
   return ADMM_OK;
@@ -508,6 +510,7 @@ extern "C" int admm_timing_every(admm_ctx *ctx, unsigned n) {
 
 extern "C" int admm_timing_reset(admm_ctx *ctx) {
   ADMM_REQUIRE(ctx, "admm_timing_reset: ctx is NULL");
+  ADMM_HIP_CHECK(use_device(ctx));
   ADMM_TRY(timing_flush(ctx));
   for (int k = 0; k < ADMM_K_COUNT; ++k) {
     ctx->k_ms[k] = 0;
@@ -518,6 +521,7 @@ extern "C" int admm_timing_reset(admm_ctx *ctx) {
 
 extern "C" int admm_timing_get(admm_ctx *ctx, int kernel, double *total_ms, uint64_t *launches) {
   ADMM_REQUIRE(ctx && kernel >= 0 && kernel < ADMM_K_COUNT, "admm_timing_get: bad arguments");
+  ADMM_HIP_CHECK(use_device(ctx));
   ADMM_TRY(timing_flush(ctx));
   if (total_ms) *total_ms = ctx->k_ms[kernel];
   if (launches) *launches = ctx->k_launches[kernel];
@@ -550,6 +554,7 @@ extern "C" int admm_vec_alloc(admm_ctx *ctx, uint64_t n, float **out) {
 extern "C" int admm_vec_free(admm_ctx *ctx, float *v) {
   ADMM_REQUIRE(ctx, "admm_vec_free: ctx is NULL");
   if (!v) return ADMM_OK;
+  ADMM_HIP_CHECK(use_device(ctx));
   ADMM_HIP_CHECK(hipStreamSynchronize(ctx->stream));
   ADMM_HIP_CHECK(hipFree(v));
   return ADMM_OK;
@@ -557,18 +562,21 @@ extern "C" int admm_vec_free(admm_ctx *ctx, float *v) {
 
 extern "C" int admm_vec_zero(admm_ctx *ctx, float *v, uint64_t n) {
   ADMM_REQUIRE(ctx && v, "admm_vec_zero: bad arguments");
+  ADMM_HIP_CHECK(use_device(ctx));
   ADMM_HIP_CHECK(hipMemsetAsync(v, 0, sizeof(float) * n, ctx->stream));
   return ADMM_OK;
 }
 
 extern "C" int admm_vec_copy(admm_ctx *ctx, float *dst, const float *src, uint64_t n) {
   ADMM_REQUIRE(ctx && dst && src, "admm_vec_copy: bad arguments");
+  ADMM_HIP_CHECK(use_device(ctx));
   ADMM_HIP_CHECK(hipMemcpyAsync(dst, src, sizeof(float) * n, hipMemcpyDeviceToDevice, ctx->stream));
   return ADMM_OK;
 }
 
 extern "C" int admm_vec_upload(admm_ctx *ctx, float *dst, const float *src_host, uint64_t n) {
   ADMM_REQUIRE(ctx && dst && src_host, "admm_vec_upload: bad arguments");
+  ADMM_HIP_CHECK(use_device(ctx));
   ADMM_HIP_CHECK(hipMemcpyAsync(dst, src_host, sizeof(float) * n, hipMemcpyHostToDevice, ctx->stream));
   ADMM_HIP_CHECK(hipStreamSynchronize(ctx->stream));  // the host buffer is only borrowed
   return ADMM_OK;
@@ -576,6 +584,7 @@ extern "C" int admm_vec_upload(admm_ctx *ctx, float *dst, const float *src_host,
 
 extern "C" int admm_vec_download(admm_ctx *ctx, float *dst_host, const float *src, uint64_t n) {
   ADMM_REQUIRE(ctx && dst_host && src, "admm_vec_download: bad arguments");
+  ADMM_HIP_CHECK(use_device(ctx));
   ADMM_HIP_CHECK(hipMemcpyAsync(dst_host, src, sizeof(float) * n, hipMemcpyDeviceToHost, ctx->stream));
   ADMM_HIP_CHECK(hipStreamSynchronize(ctx->stream));
   return check_device_reports(ctx);
@@ -586,6 +595,7 @@ extern "C" int admm_vec_download(admm_ctx *ctx, float *dst_host, const float *sr
 extern "C" int admm_payload(admm_ctx *ctx, const float *x, const float *ydual, float rho, float *out,
                             uint64_t dim) {
   ADMM_REQUIRE(ctx && x && ydual && out && dim > 0, "admm_payload: bad arguments");
+  ADMM_HIP_CHECK(use_device(ctx));
   KernelTimer t(ctx, ADMM_K_ELEMENTWISE);
   hipLaunchKernelGGL(k_payload, dim3(ew_grid(ctx, dim)), dim3(256), 0, ctx->stream, x, ydual, rho, out,
                      dim);
@@ -596,6 +606,7 @@ extern "C" int admm_payload(admm_ctx *ctx, const float *x, const float *ydual, f
 extern "C" int admm_global_update(admm_ctx *ctx, const float *sum, int num_worker, float rho,
                                   float global_var, float l1, float *z, uint64_t dim) {
   ADMM_REQUIRE(ctx && sum && z && dim > 0 && num_worker > 0, "admm_global_update: bad arguments");
+  ADMM_HIP_CHECK(use_device(ctx));
   const float denom = num_worker * rho + global_var;  // src/master.cc:17, float arithmetic
   KernelTimer t(ctx, ADMM_K_ELEMENTWISE);
   hipLaunchKernelGGL(k_global_update, dim3(ew_grid(ctx, dim)), dim3(256), 0, ctx->stream, sum, denom,
@@ -607,6 +618,7 @@ extern "C" int admm_global_update(admm_ctx *ctx, const float *sum, int num_worke
 extern "C" int admm_dual_update(admm_ctx *ctx, float *ydual, const float *x, const float *z, float rho,
                                 uint64_t dim) {
   ADMM_REQUIRE(ctx && ydual && x && z && dim > 0, "admm_dual_update: bad arguments");
+  ADMM_HIP_CHECK(use_device(ctx));
   KernelTimer t(ctx, ADMM_K_ELEMENTWISE);
   hipLaunchKernelGGL(k_dual_update, dim3(ew_grid(ctx, dim)), dim3(256), 0, ctx->stream, ydual, x, z,
                      rho, dim);
@@ -619,6 +631,7 @@ extern "C" int admm_consensus(admm_ctx *ctx, const float *sum, int num_worker, f
                               uint64_t dim, double *r2, double *s2) {
   ADMM_REQUIRE(ctx && sum && x && ydual && z && dim > 0 && num_worker > 0,
                "admm_consensus: bad arguments");
+  ADMM_HIP_CHECK(use_device(ctx));
   const float denom = num_worker * rho + global_var;
   const int grid = grid_for(dim, 256, ctx->cu_count * 8);
   {

@@ -1065,6 +1065,7 @@ extern "C" int admm_ftrl_pass_multi(admm_csr *const *sets, float *const *w, floa
       ADMM_REQUIRE(w[j] != w[k] && z[j] != z[k] && n[j] != n[k],
                    "admm_ftrl_pass_multi: passes %d and %d share a state vector", j, k);
   }
+  if (count) ADMM_HIP_CHECK(use_device(sets[0]->ctx));
   return ftrl_pass_multi(sets, w, z, n, offset, reg_offset, count, alpha, beta, l1, l2);
 }
 
@@ -1072,6 +1073,7 @@ extern "C" int admm_ftrl_pass(admm_csr *csr, float *w, float *z, float *n, const
                               const float *reg_offset, float alpha, float beta, float l1, float l2,
                               uint64_t batch) {
   ADMM_REQUIRE(csr && w && z && n && offset && reg_offset, "admm_ftrl_pass: NULL argument");
+  ADMM_HIP_CHECK(use_device(csr->ctx));
   ADMM_REQUIRE(alpha > 0, "admm_ftrl_pass: alpha must be > 0");
   ADMM_TRY(require_rows(csr, "admm_ftrl_pass"));
   if (batch <= 1) return ftrl_pass_sequential(csr, w, z, n, offset, reg_offset, alpha, beta, l1, l2);

@@ -276,6 +276,10 @@ int vec_lincomb(admm_ctx *ctx, float *out, const float *a, float s, const float 
 int vec_sub(admm_ctx *ctx, float *out, const float *a, const float *b, uint64_t n);
 void comm_release(admm_ctx *ctx);  // comm.hip
 
+// The default stream (ADMM_STREAM_DEFAULT) is the current device's: a call on a context that queues there makes the context's
+// device the current one first.  Streams of their own say where they are.
+inline hipError_t use_device(const admm_ctx *ctx) { return ctx->stream ? hipSuccess : hipSetDevice(ctx->device); }
+
 inline int grid_for(uint64_t work_items, int block, int max_blocks) {
   uint64_t g = (work_items + block - 1) / block;
   if (g < 1) g = 1;

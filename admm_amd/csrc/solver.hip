@@ -388,6 +388,7 @@ static int logistic_fg(admm_csr *csr, const float *x, const float *offset, const
 
 extern "C" int admm_predict(admm_csr *csr, const float *const *groups, int ngroups, float *p_out) {
   ADMM_REQUIRE(csr && groups && p_out, "admm_predict: NULL argument");
+  ADMM_HIP_CHECK(use_device(csr->ctx));
   int nblk = 0;
   ADMM_TRY(launch_forward(csr, FWD_EVAL, 0, csr->nrows, groups, ngroups, p_out, &nblk));
   return ADMM_OK;
@@ -401,6 +402,7 @@ extern "C" int admm_metrics(admm_csr *csr, const float *const *groups, int ngrou
                             double *auc, uint64_t *nrows) {
   ADMM_REQUIRE(csr && groups, "admm_metrics: NULL argument");
   admm_ctx *ctx = csr->ctx;
+  ADMM_HIP_CHECK(use_device(ctx));
   if (nrows) *nrows = csr->nrows;
   if (csr->nrows == 0) {
     if (logloss_mean) *logloss_mean = NAN;
@@ -422,6 +424,7 @@ extern "C" int admm_metrics(admm_csr *csr, const float *const *groups, int ngrou
 extern "C" int admm_logistic_fg(admm_csr *csr, const float *x, const float *offset, const float *z,
                                 const float *ydual, float rho, double *f_out, float *g_out) {
   ADMM_REQUIRE(csr && x && g_out, "admm_logistic_fg: NULL argument");
+  ADMM_HIP_CHECK(use_device(csr->ctx));
   return logistic_fg(csr, x, offset, z, ydual, rho, f_out, g_out);
 }
 
@@ -429,6 +432,7 @@ extern "C" int admm_lbfgs_solve(admm_csr *csr, float *x, const float *offset, co
                                 float rho, const admm_lbfgs_params *params, admm_lbfgs_result *result) {
   ADMM_REQUIRE(csr && x, "admm_lbfgs_solve: NULL argument");
   admm_ctx *ctx = csr->ctx;
+  ADMM_HIP_CHECK(use_device(ctx));
   admm_lbfgs_params P = {6, 10, 20, 1e-5f, 1e-4f, 0.9f, 0};
   if (params) P = *params;
   ADMM_REQUIRE(P.m >= 1 && P.m <= 32 && P.max_iter >= 0 && P.max_linesearch >= 1, "admm_lbfgs_solve: bad params");

@@ -44,7 +44,8 @@ int admm_abi_version(void);
  * library create its own. */
 int admm_device_count(int *count);
 int admm_ctx_create(int device, void *stream, admm_ctx **out);
-/* the value of `stream` that names the device's default (legacy) stream */
+/* the value of `stream` that names the device's default (legacy) stream.  That stream is the current device's to HIP, so calls
+ * on such a context make its device the calling thread's current one, where they do not say that they leave it. */
 #define ADMM_STREAM_DEFAULT ((void *)1)
 int admm_ctx_destroy(admm_ctx *ctx);
 int admm_sync(admm_ctx *ctx);
