@@ -17,7 +17,7 @@ LIB_PATH = os.path.join(_PKG, "libadmm_hip.so")
 SYMBOLS = [
     "admm_last_error", "admm_abi_version", "admm_device_count", "admm_ctx_create", "admm_ctx_destroy", "admm_sync",
     "admm_timing_enable", "admm_timing_classes", "admm_timing_every", "admm_timing_reset", "admm_timing_get",
-    "admm_vec_alloc", "admm_vec_free", "admm_vec_zero", "admm_vec_copy", "admm_vec_upload",
+    "admm_vec_alloc", "admm_scratch_alloc", "admm_vec_free", "admm_vec_zero", "admm_vec_copy", "admm_vec_upload",
     "admm_vec_download",
     "admm_csr_upload", "admm_csr_synth", "admm_csr_shape", "admm_csr_download",
     "admm_csr_build_transposed", "admm_csr_relabel_by_frequency", "admm_csr_set_lean", "admm_synth_row_draws", "admm_csr_bytes", "admm_csr_layout_bytes", "admm_csr_layout_counts",
@@ -99,6 +99,7 @@ def load():
         "admm_timing_reset": [vp],
         "admm_timing_get": [vp, i32, C.POINTER(C.c_double), C.POINTER(u64)],
         "admm_vec_alloc": [vp, u64, C.POINTER(vp)],
+        "admm_scratch_alloc": [vp, u64, C.POINTER(vp)],
         "admm_vec_free": [vp, vp],
         "admm_vec_zero": [vp, vp, u64],
         "admm_vec_copy": [vp, vp, vp, u64],
@@ -217,6 +218,17 @@ class DeviceBuf:
         self.vec = DeviceVec(ctx, max(1, (int(nbytes) + 3) // 4))
         self.nbytes = int(nbytes)
         self.ptr = self.vec.ptr
+
+    @classmethod
+    def scratch(cls, ctx, nbytes):
+        """of any contents; the calling thread's current device stays what it is (admm_scratch_alloc)"""
+        b, v = cls.__new__(cls), DeviceVec.__new__(DeviceVec)
+        b.nbytes = max(4, int(nbytes))
+        p = C.c_void_p()
+        _check(ctx.L.admm_scratch_alloc(ctx.h, b.nbytes, C.byref(p)))
+        v.ctx, v.n, v.ptr = ctx, b.nbytes // 4, p
+        b.vec, b.ptr = v, p
+        return b
 
     def free(self):
         self.vec.free()
@@ -464,7 +476,7 @@ class Context:
             if self._scratch is not None:
                 self._retired.append(self._scratch)
             self._scratch = None
-            self._scratch = DeviceBuf(self, (need + (need >> 2) + 4095) // 4096 * 4096)
+            self._scratch = DeviceBuf.scratch(self, (need + (need >> 2) + 4095) // 4096 * 4096)
         return self._scratch.ptr, self._scratch.nbytes
 
     def buf(self, nbytes):
@@ -497,7 +509,7 @@ class Context:
     def embed_order(self, bags, table_rows, order=None):
         """admm_embed_order: the entries sorted by id, into `order` (a DeviceBuf or a torch tensor of bytes; made if None)"""
         if order is None:
-            order = DeviceBuf(self, self.embed_order_bytes(bags, table_rows))
+            order = DeviceBuf.scratch(self, self.embed_order_bytes(bags, table_rows))
         p, n = self._bytes(order, "order")
         _check(self.L.admm_embed_order(self.h, bags.packed, int(table_rows), p, n))
         return order

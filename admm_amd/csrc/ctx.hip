@@ -551,6 +551,20 @@ extern "C" int admm_vec_alloc(admm_ctx *ctx, uint64_t n, float **out) {
   return ADMM_OK;
 }
 
+extern "C" int admm_scratch_alloc(admm_ctx *ctx, uint64_t bytes, void **out) {
+  ADMM_REQUIRE(ctx && out && bytes > 0, "admm_scratch_alloc: bad arguments");
+  OnDevice on(ctx->device);
+  ADMM_HIP_CHECK(on.error);
+  hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(ctx->stream, &capturing) != hipSuccess || capturing != hipStreamCaptureStatusNone) {
+    (void)hipGetLastError();
+    set_error("admm_scratch_alloc: the context's stream is being captured: allocate before the capture");
+    return ADMM_ERR_STATE;
+  }
+  ADMM_HIP_CHECK(hipMalloc(out, bytes));
+  return ADMM_OK;
+}
+
 extern "C" int admm_vec_free(admm_ctx *ctx, float *v) {
   ADMM_REQUIRE(ctx, "admm_vec_free: ctx is NULL");
   if (!v) return ADMM_OK;

@@ -280,6 +280,23 @@ void comm_release(admm_ctx *ctx);  // comm.hip
 // device the current one first.  Streams of their own say where they are.
 inline hipError_t use_device(const admm_ctx *ctx) { return ctx->stream ? hipSuccess : hipSetDevice(ctx->device); }
 
+// the calling thread's current device is `device` while this lives
+struct OnDevice {
+  int before = -1;
+  bool changed = false;
+  hipError_t error;
+  explicit OnDevice(int device) {
+    error = hipGetDevice(&before);
+    if (error == hipSuccess && before != device) {
+      error = hipSetDevice(device);
+      changed = error == hipSuccess;
+    }
+  }
+  ~OnDevice() {
+    if (changed) hipSetDevice(before);
+  }
+};
+
 inline int grid_for(uint64_t work_items, int block, int max_blocks) {
   uint64_t g = (work_items + block - 1) / block;
   if (g < 1) g = 1;

@@ -89,23 +89,6 @@ constexpr uint64_t kMaxClasses = 0x7FFFFF00;  // chunks and columns of a row of 
 
 // ---- host side ----------------------------------------------------------------------------------
 
-// the calling thread's current device is `device` while this lives
-struct OnDevice {
-  int before = -1;
-  bool changed = false;
-  hipError_t error;
-  explicit OnDevice(int device) {
-    error = hipGetDevice(&before);
-    if (error == hipSuccess && before != device) {
-      error = hipSetDevice(device);
-      changed = error == hipSuccess;
-    }
-  }
-  ~OnDevice() {
-    if (changed) hipSetDevice(before);
-  }
-};
-
 // type, stride, alignment to the element and size of a matrix argument
 inline int check_mat(const admm_mat *m, const char *who, const char *name) {
   ADMM_REQUIRE(m, "%s: %s is NULL", who, name);

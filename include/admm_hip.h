@@ -74,6 +74,10 @@ int admm_timing_get(admm_ctx *ctx, int kernel, double *total_ms, uint64_t *launc
 /* ---- dim-sized vectors (Worker::InitWorker, src/workers.cc:32-46) ------------------------- */
 
 int admm_vec_alloc(admm_ctx *ctx, uint64_t n, float **out); /* zero-filled */
+/* DEVICE memory of any contents, on 256 bytes, for the workspaces and orders below; admm_vec_free frees it.  The calling
+ * thread's current device is left as it was.  Refused (ADMM_ERR_STATE) while the context's stream is being captured: what a
+ * graph uses is allocated before its capture. */
+int admm_scratch_alloc(admm_ctx *ctx, uint64_t bytes, void **out);
 int admm_vec_free(admm_ctx *ctx, float *v);
 int admm_vec_zero(admm_ctx *ctx, float *v, uint64_t n);
 int admm_vec_copy(admm_ctx *ctx, float *dst, const float *src, uint64_t n);

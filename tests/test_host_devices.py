@@ -106,3 +106,71 @@ def test_contexts_with_a_stream_of_their_own_do_not_touch_the_current_device(rec
     assert current() == 0
     assert all(c[2] == 0x6000 for c in calls() if c[0] not in ("hipMalloc", "hipMemcpy"))
     """)
+
+
+MANY = """
+def vec(n):
+    return ctx.vec(n)
+
+def mat(rows, cols):
+    return capi.DeviceMat(vec(rows * cols).ptr.value, rows, cols)
+
+def ids(n):
+    return capi.Bags(vec(2 * n).ptr.value, None, None, n, n, capi.I64)
+"""
+
+
+MANY_ALLOC = """
+ctx = capi.Context(1, stream=stream)
+""" + MANY + """
+x, u, tok, b = mat(3, 5000), vec(3), capi.DeviceBuf(ctx, 12), ids(100)
+src, to, loss, lab = mat(100, 8), mat(50, 8), vec(3), vec(3)
+wide = mat(3, 200000)
+rec.hipSetDevice(0)
+rec.rec_clear()
+ctx.sample(x, u, tok)
+assert current() == 0, "sample"
+order = ctx.embed_order(b, 50)
+assert current() == 0, "embed_order"
+ctx.embed_grad(b, order, src, to)
+assert current() == 0, "embed_grad"
+ctx.softmax_loss(wide, lab, loss)
+assert current() == 0, "softmax_loss"
+seen = calls()
+assert sum(c[0] == "hipMalloc" for c in seen) >= 2 and all(c[1] == 1 for c in seen), seen
+"""
+
+
+def test_calls_without_a_workspace_leave_the_current_device(recorder):
+    """the context's own workspace, and an order that embed_order makes, are allocated on the context's device; the calling
+    thread's stays what it was"""
+    run(recorder, "stream = 0x6000" + MANY_ALLOC)
+    run(recorder, "stream = capi.DEFAULT_STREAM" + MANY_ALLOC)
+
+
+def test_the_workspace_does_not_grow_under_capture(recorder):
+    """what a graph uses is allocated before its capture: growing is refused, and nothing is allocated or queued; a call whose
+    workspace is there is not"""
+    run(recorder, """
+    ctx = capi.Context(1, stream=0x6000)
+    """ + textwrap.indent(MANY, "    ") + """
+    x, u, tok, b = mat(3, 5000), vec(3), capi.DeviceBuf(ctx, 12), ids(100)
+    for status in (1, 2, 4):   # captured, capture invalidated, not to be asked for
+        rec.rec_capture(status)
+        rec.rec_clear()
+        for call in (lambda: ctx.sample(x, u, tok), lambda: ctx.embed_order(b, 50)):
+            try:
+                call()
+            except capi.AdmmError as e:
+                assert "captured" in str(e), e
+            else:
+                raise AssertionError("not refused")
+        assert not calls(), calls()
+        assert rec.hipSetDevice(1) == 0
+    rec.rec_capture(0)
+    ctx.sample(x, u, tok)
+    rec.rec_capture(1)
+    ctx.sample(x, u, tok)
+    rec.rec_capture(0)
+    ctx.close()
+    """)
