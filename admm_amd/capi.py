@@ -473,10 +473,10 @@ class Context:
         if need == 0:
             return None, 0
         if self._scratch is None or self._scratch.nbytes < need:
+            larger = DeviceBuf.scratch(self, (need + (need >> 2) + 4095) // 4096 * 4096)
             if self._scratch is not None:
                 self._retired.append(self._scratch)
-            self._scratch = None
-            self._scratch = DeviceBuf.scratch(self, (need + (need >> 2) + 4095) // 4096 * 4096)
+            self._scratch = larger
         return self._scratch.ptr, self._scratch.nbytes
 
     def buf(self, nbytes):

@@ -174,3 +174,28 @@ def test_the_workspace_does_not_grow_under_capture(recorder):
     rec.rec_capture(0)
     ctx.close()
     """)
+
+
+def test_a_refused_growth_keeps_the_workspace(recorder):
+    """a call that needs more than there is, under capture: refused, and the calls that have enough go on"""
+    run(recorder, """
+    ctx = capi.Context(1, stream=0x6000)
+    """ + textwrap.indent(MANY, "    ") + """
+    x, u, tok = mat(3, 5000), vec(3), capi.DeviceBuf(ctx, 12)
+    big, bu, btok = mat(400, 5000), vec(400), capi.DeviceBuf(ctx, 1600)
+    ctx.sample(x, u, tok)
+    had = ctx._scratch.ptr.value
+    rec.rec_capture(1)
+    try:
+        ctx.sample(big, bu, btok)
+    except capi.AdmmError as e:
+        assert "captured" in str(e), e
+    else:
+        raise AssertionError("not refused")
+    ctx.sample(x, u, tok)
+    rec.rec_capture(0)
+    assert ctx._scratch.ptr.value == had
+    ctx.sample(big, bu, btok)
+    assert ctx._scratch.ptr.value != had and [b.ptr.value for b in ctx._retired] == [had]
+    ctx.close()
+    """)
