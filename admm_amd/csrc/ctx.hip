@@ -530,21 +530,45 @@ extern "C" int admm_timing_get(admm_ctx *ctx, int kernel, double *total_ms, uint
 
 // ---- vectors --------------------------------------------------------------------------------
 
+namespace {
+__global__ void __launch_bounds__(256) k_vec_zero(float *v, uint64_t n) {
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256) v[i] = 0.0f;
+}
+
+// allocations are allowed to this thread, whatever captures go on, while this lives
+struct RelaxedCapture {
+  hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+  RelaxedCapture() { hipThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { hipThreadExchangeStreamCaptureMode(&mode); }
+};
+}  // namespace
+
 extern "C" int admm_vec_alloc(admm_ctx *ctx, uint64_t n, float **out) {
   ADMM_REQUIRE(ctx && out && n > 0, "admm_vec_alloc: bad arguments");
   ADMM_HIP_CHECK(hipSetDevice(ctx->device));
   hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(ctx->stream, &capturing) != hipSuccess || capturing != hipStreamCaptureStatusNone) {
+  if (hipStreamIsCapturing(ctx->stream, &capturing) != hipSuccess || capturing == hipStreamCaptureStatusInvalidated) {
     (void)hipGetLastError();
-    set_error("admm_vec_alloc: the context's stream is being captured: allocate before the capture");
+    set_error("admm_vec_alloc: nothing can be queued on the context's stream while a stream is being captured");
     return ADMM_ERR_STATE;
   }
   float *p = nullptr;
-  ADMM_HIP_CHECK(hipMalloc(&p, sizeof(float) * n));
-  hipError_t e = hipMemsetAsync(p, 0, sizeof(float) * n, ctx->stream);
+  hipError_t e;
+  if (capturing == hipStreamCaptureStatusNone) {
+    ADMM_HIP_CHECK(hipMalloc(&p, sizeof(float) * n));
+    e = hipMemsetAsync(p, 0, sizeof(float) * n, ctx->stream);
+  } else {
+    // the graph zeroes the vector at every replay, by a kernel: replayed memsets have left wrong values
+    {
+      RelaxedCapture relaxed;
+      ADMM_HIP_CHECK(hipMalloc(&p, sizeof(float) * n));
+    }
+    hipLaunchKernelGGL(k_vec_zero, dim3(ew_grid(ctx, n)), dim3(256), 0, ctx->stream, p, n);
+    e = hipGetLastError();
+  }
   if (e != hipSuccess) {
     hipFree(p);
-    set_error("admm_vec_alloc: memset failed: %s", hipGetErrorString(e));
+    set_error("admm_vec_alloc: zeroing failed: %s", hipGetErrorString(e));
     return ADMM_ERR_HIP;
   }
   *out = p;

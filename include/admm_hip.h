@@ -73,7 +73,8 @@ int admm_timing_get(admm_ctx *ctx, int kernel, double *total_ms, uint64_t *launc
 
 /* ---- dim-sized vectors (Worker::InitWorker, src/workers.cc:32-46) ------------------------- */
 
-int admm_vec_alloc(admm_ctx *ctx, uint64_t n, float **out); /* zero-filled */
+/* zero-filled; while the context's stream is being captured, by the graph at every replay */
+int admm_vec_alloc(admm_ctx *ctx, uint64_t n, float **out);
 /* DEVICE memory of any contents, on 256 bytes, for the workspaces and orders below; admm_vec_free frees it.  The calling
  * thread's current device is left as it was.  Refused (ADMM_ERR_STATE) while the context's stream is being captured: what a
  * graph uses is allocated before its capture. */

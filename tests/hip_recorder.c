@@ -14,6 +14,7 @@ static struct {
   void *stream;
 } calls[MAX_CALLS];
 static int ncalls, current, capture_status;
+static hipStreamCaptureMode thread_mode = hipStreamCaptureModeGlobal;
 
 static void record(const char *name, void *stream) {
   if (ncalls < MAX_CALLS) {
@@ -29,6 +30,7 @@ EXPORT const char *rec_name(int i) { return calls[i].name; }
 EXPORT int rec_device(int i) { return calls[i].device; }
 EXPORT void *rec_stream(int i) { return calls[i].stream; }
 EXPORT void rec_clear(void) { ncalls = 0; }
+EXPORT int rec_thread_mode(void) { return (int)thread_mode; }
 EXPORT void rec_capture(int status) { capture_status = status; }
 
 EXPORT hipError_t hipGetDeviceCount(int *n) { *n = 2; return hipSuccess; }
@@ -42,7 +44,7 @@ EXPORT hipError_t hipGetDevicePropertiesR0600(hipDeviceProp_tR0600 *p, int d) {
 }
 EXPORT hipError_t hipDeviceGetAttribute(int *v, hipDeviceAttribute_t a, int d) { *v = 64; return hipSuccess; }
 EXPORT hipError_t hipMalloc(void **p, size_t n) {
-  record("hipMalloc", NULL);
+  record(thread_mode == hipStreamCaptureModeRelaxed ? "hipMalloc, relaxed" : "hipMalloc", NULL);
   *p = aligned_alloc(256, (n + 255) / 256 * 256 + 256);
   if (!*p) return hipErrorOutOfMemory;
   memset(*p, 0, (n + 255) / 256 * 256 + 256);
@@ -82,9 +84,8 @@ EXPORT hipError_t hipStreamIsCapturing(hipStream_t s, hipStreamCaptureStatus *st
   return capture_status & 4 ? hipErrorStreamCaptureImplicit : hipSuccess;
 }
 EXPORT hipError_t hipThreadExchangeStreamCaptureMode(hipStreamCaptureMode *mode) {
-  static hipStreamCaptureMode now = hipStreamCaptureModeGlobal;
-  const hipStreamCaptureMode before = now;
-  now = *mode;
+  const hipStreamCaptureMode before = thread_mode;
+  thread_mode = *mode;
   *mode = before;
   return hipSuccess;
 }

@@ -199,3 +199,31 @@ def test_a_refused_growth_keeps_the_workspace(recorder):
     assert ctx._scratch.ptr.value != had and [b.ptr.value for b in ctx._retired] == [had]
     ctx.close()
     """)
+
+
+def test_vectors_may_be_allocated_under_capture(recorder):
+    """admm_vec_alloc while the stream is captured: the thread's capture mode allows the allocation and is what it was
+    afterwards, and what zeroes the vector is a kernel, not a memset, in the graph"""
+    run(recorder, """
+    ctx = capi.Context(1, stream=0x6000)
+    rec.rec_capture(1)
+    rec.rec_clear()
+    v = ctx.vec(64)
+    assert [c[0] for c in calls()] == ["hipMalloc, relaxed", "hipLaunchKernel"], calls()
+    assert calls()[1][2] == 0x6000 and rec.rec_thread_mode() == 0
+    for status in (2, 4):   # a capture that has failed, another stream's that keeps this one from being used
+        rec.rec_capture(status)
+        rec.rec_clear()
+        try:
+            ctx.vec(64)
+        except capi.AdmmError as e:
+            assert "captured" in str(e), e
+        else:
+            raise AssertionError("not refused")
+        assert not calls(), calls()
+    rec.rec_capture(0)
+    rec.rec_clear()
+    ctx.vec(64)
+    assert [c[0] for c in calls()] == ["hipMalloc", "hipMemsetAsync"], calls()
+    ctx.close()
+    """)
