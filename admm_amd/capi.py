@@ -212,11 +212,16 @@ class DeviceVec:
 
 
 class DeviceBuf:
-    """bytes in HBM (workspaces, orders, integer arrays)"""
+    """bytes in HBM (workspaces, orders, integer arrays); `type`: what elements they are (I32, I64, F32), where a call could take
+    several for them"""
 
-    def __init__(self, ctx, nbytes):
+    type = None
+
+    def __init__(self, ctx, nbytes, type=None):
+        if type is not None and type not in range(len(_BYTES)):
+            raise AdmmError("a buffer of elements of type %s" % (type,))
         self.vec = DeviceVec(ctx, max(1, (int(nbytes) + 3) // 4))
-        self.nbytes = int(nbytes)
+        self.nbytes, self.type = int(nbytes), type
         self.ptr = self.vec.ptr
 
     @classmethod
@@ -417,8 +422,8 @@ class Context:
                                        n.ptr, alpha))
 
     # models with many classes or tokens -----------------------------------------------------
-    # Matrices are torch tensors or DeviceMats, arrays are torch tensors, DeviceVecs or DeviceBufs; what they point to
-    # belongs to this context's GPU, and the work is queued on this context's stream (make the context on the stream that
+    # Matrices are torch tensors or DeviceMats, arrays are torch tensors, DeviceVecs (floats) or DeviceBufs (labels in one
+    # need its type: buf(bytes, type=I64)); what they point to belongs to this context's GPU, and the work is queued on this context's stream (make the context on the stream that
     # the tensors are used on: Context(device, stream=torch.cuda.current_stream().cuda_stream or DEFAULT_STREAM)).
     def _elsewhere(self, t, name):
         return AdmmError("%s is on %s, the context on GPU %d" % (name, t.device, self.device))
@@ -447,9 +452,13 @@ class Context:
                 raise AdmmError("%s: %d floats do not do for %d elements" % (name, a.n, count))
             return a.ptr, F32
         if isinstance(a, DeviceBuf):
-            if a.nbytes < count * _BYTES[kinds[0]]:
+            kind = kinds[0] if a.type is None and len(kinds) == 1 else a.type
+            if kind not in kinds:
+                raise AdmmError("%s: %s" % (name, "a buffer that does not say its elements' type (buf(bytes, type=...))" if kind is None
+                                            else "elements of type %d" % kind))
+            if a.nbytes < count * _BYTES[kind]:
                 raise AdmmError("%s: %d bytes do not do for %d elements" % (name, a.nbytes, count))
-            return a.ptr, kinds[0]
+            return a.ptr, kind
         raise AdmmError("%s: a torch tensor, a DeviceVec or a DeviceBuf is needed, not %s" % (name, a.__class__.__name__))
 
     def _bytes(self, buf, name):
@@ -479,8 +488,8 @@ class Context:
             self._scratch = larger
         return self._scratch.ptr, self._scratch.nbytes
 
-    def buf(self, nbytes):
-        return DeviceBuf(self, nbytes)
+    def buf(self, nbytes, type=None):
+        return DeviceBuf(self, nbytes, type)
 
     def bags(self, ids, rowptr=None, val=None):
         """Rows of ids for embed / embed_grad: one per row, or with row pointers (nrows + 1 int64) and factors"""

@@ -1,0 +1,47 @@
+"""Arguments of the many-class calls of the Python binding that are refused, or taken for what they are, before anything is
+queued: on the recording runtime, without a GPU."""
+import textwrap
+
+from test_host_devices import MANY, recorder, run  # noqa: F401
+
+REFUSED = """
+def refused(call, text):
+    rec.rec_clear()
+    try:
+        call()
+    except capi.AdmmError as e:
+        assert text in str(e), (text, str(e))
+    else:
+        raise AssertionError("not refused: " + text)
+    assert not [c for c in calls() if c[0] == "hipLaunchKernel"], calls()
+"""
+
+
+def check(recorder, body):  # noqa: F811
+    run(recorder, "ctx = capi.Context(0, stream=0x6000)" + MANY + REFUSED + textwrap.dedent(body))
+
+
+def test_labels_in_a_buffer_say_their_type(recorder):  # noqa: F811
+    """a buffer of bytes could hold labels of three types: it has to say which, and the library is told that one"""
+    check(recorder, """
+    x, loss = mat(4, 8), vec(4)
+    refused(lambda: ctx.softmax_loss(x, ctx.buf(32), loss), "type")
+    refused(lambda: ctx.softmax_loss(x, ctx.buf(16), loss), "type")
+    refused(lambda: ctx.softmax_loss(x, ctx.buf(32, type=capi.BF16), loss), "type")
+    refused(lambda: ctx.softmax_loss(x, ctx.buf(31, type=capi.I64), loss), "31 bytes")
+    refused(lambda: ctx.sample(x, ctx.buf(16, type=capi.I32), ctx.buf(16)), "uniform")
+    refused(lambda: ctx.buf(16, type=9), "type 9")
+    seen, library = [], ctx.L.admm_softmax_loss
+
+    class Spy:
+        def __getattr__(self, name):
+            if name != "admm_softmax_loss":
+                return getattr(L, name)
+            return lambda *a: seen.append(a[3]) or library(*a)
+    ctx.L = Spy()
+    for kind, size in ((capi.I32, 16), (capi.I64, 32), (capi.F32, 16)):
+        ctx.softmax_loss(x, ctx.buf(size, type=kind), loss)
+    assert seen == [capi.I32, capi.I64, capi.F32], seen
+    ctx.L = L
+    ctx.sample(x, ctx.buf(16), ctx.buf(16, type=capi.I32))   # one type only: it need not be said
+    """)
