@@ -302,12 +302,13 @@ def _not_a_matrix(m, name):
 
 
 class Bags:
-    """Rows of ids (admm_bags); keeps the arrays alive"""
+    """Rows of ids (admm_bags); keeps the arrays alive, but for those of a sample set (`source`), which are asked for again at
+    every call that reads them"""
 
-    __slots__ = ("nrows", "nnz", "keep", "packed")
+    __slots__ = ("nrows", "nnz", "keep", "packed", "source")
 
-    def __init__(self, ids, rowptr, val, nrows, nnz, id_type, keep=()):
-        self.nrows, self.nnz, self.keep = nrows, nnz, keep
+    def __init__(self, ids, rowptr, val, nrows, nnz, id_type, keep=(), source=None):
+        self.nrows, self.nnz, self.keep, self.source = nrows, nnz, keep, source
         self.packed = _BAGS(ids or 0, rowptr or 0, val or 0, nrows, nnz, id_type)
 
 
@@ -507,28 +508,36 @@ class Context:
             f, _ = self._array(val, "val", nnz, (F32,))
         return Bags(p, q, f, nrows, nnz, kind, (ids, rowptr, val))
 
+    def _bags(self, bags, read=True):
+        """what the library is told of the bags; `read`: it reads their arrays, not the counts alone"""
+        if bags.__class__ is not Bags:
+            raise AdmmError("bags: Context.bags() or SampleSet.bags() makes them, not %s" % bags.__class__.__name__)
+        return C.byref(bags.source._rows()) if read and bags.source is not None else bags.packed
+
     def embed(self, bags, table, out, scale=1.0):
         """admm_embed: out[r] = scale * sum of val_e * table[id_e] over the entries of row r"""
-        _check(self.L.admm_embed(self.h, bags.packed, DeviceMat.of(self, table, "table").packed, scale, DeviceMat.of(self, out, "out").packed))
+        _check(self.L.admm_embed(self.h, self._bags(bags), DeviceMat.of(self, table, "table").packed, scale, DeviceMat.of(self, out, "out").packed))
 
     def embed_order_bytes(self, bags, table_rows):
-        _check(self.L.admm_embed_order_bytes(bags.packed, int(table_rows), self._size_ref))
+        _check(self.L.admm_embed_order_bytes(self._bags(bags, False), int(table_rows), self._size_ref))
         return self._size.value
 
     def embed_order(self, bags, table_rows, order=None):
         """admm_embed_order: the entries sorted by id, into `order` (a DeviceBuf or a torch tensor of bytes; made if None)"""
+        rows = self._bags(bags)
         if order is None:
             order = DeviceBuf.scratch(self, self.embed_order_bytes(bags, table_rows))
         p, n = self._bytes(order, "order")
-        _check(self.L.admm_embed_order(self.h, bags.packed, int(table_rows), p, n))
+        _check(self.L.admm_embed_order(self.h, rows, int(table_rows), p, n))
         return order
 
     def embed_grad(self, bags, order, grad_out, grad_table, scale=1.0, accumulate=False, workspace=None):
         """admm_embed_grad: the gradient with respect to the table, written whole or added to"""
         src, to = DeviceMat.of(self, grad_out, "grad_out"), DeviceMat.of(self, grad_table, "grad_table")
+        counts = self._bags(bags, False)
         p, n = self._bytes(order, "order")
-        w, wn = self._workspace(workspace, self.L.admm_embed_grad_workspace, bags.packed, src.cols)
-        _check(self.L.admm_embed_grad(self.h, bags.packed, p, n, src.packed, scale, 1 if accumulate else 0, to.packed, w, wn))
+        w, wn = self._workspace(workspace, self.L.admm_embed_grad_workspace, counts, src.cols)
+        _check(self.L.admm_embed_grad(self.h, counts, p, n, src.packed, scale, 1 if accumulate else 0, to.packed, w, wn))
 
     def softmax_loss(self, logits, labels, loss, grad=None, lse=None, weight=None, grad_scale=1.0, workspace=None):
         """admm_softmax_loss: loss per row, and with `grad` (may be the logits) grad_scale times its gradient"""
@@ -642,11 +651,18 @@ class SampleSet:
                                             _ptr(label)))
         return rowptr, col[:self.nnz], val[:self.nnz], label[:self.nrows]
 
-    def bags(self):
-        """the set's rows as bags for Context.embed / embed_grad (admm_csr_bags)"""
+    def _rows(self):
+        if not self.h:
+            raise AdmmError("bags: the sample set was destroyed")
         b = BagsStruct()
         _check(self.ctx.L.admm_csr_bags(self.h, C.byref(b)))
-        return Bags(b.ids, b.rowptr, b.val, b.nrows, b.nnz, b.id_type, (self,))
+        return b
+
+    def bags(self):
+        """the set's rows as bags for Context.embed / embed_grad (admm_csr_bags).  They are the set's arrays: once it is destroyed,
+        relabelled, or lean and without its rows, calls that read them are refused (embed_grad takes only counts from them)"""
+        b = self._rows()
+        return Bags(b.ids, b.rowptr, b.val, b.nrows, b.nnz, b.id_type, source=self)
 
     def build_transposed(self, panel_rows=0, col_block=0):
         _check(self.ctx.L.admm_csr_build_transposed(self.h, int(panel_rows), int(col_block)))

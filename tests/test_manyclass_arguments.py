@@ -45,3 +45,25 @@ def test_labels_in_a_buffer_say_their_type(recorder):  # noqa: F811
     ctx.L = L
     ctx.sample(x, ctx.buf(16), ctx.buf(16, type=capi.I32))   # one type only: it need not be said
     """)
+
+
+def test_bags_of_a_set_that_is_gone(recorder):  # noqa: F811
+    """the arrays of a sample set's bags are the set's: after destroy nothing reads them; the gradient, which takes only
+    counts from its bags, goes on with an order that was made before"""
+    check(recorder, """
+    csr = ctx.csr_upload(np.array([0, 2, 3], np.uint64), np.array([0, 5, 7]), None, np.array([0, 1.]), 64)
+    bags = csr.bags()
+    table, out, grad = mat(64, 8), mat(2, 8), mat(64, 8)
+    rec.rec_clear()
+    ctx.embed(bags, table, out)
+    order = ctx.embed_order(bags, 64)
+    assert len([c for c in calls() if c[0] == "hipLaunchKernel"]) >= 2
+    csr.destroy()
+    refused(lambda: ctx.embed(bags, table, out), "destroyed")
+    refused(lambda: ctx.embed_order(bags, 64, order), "destroyed")
+    refused(lambda: ctx.embed_order(bags, 64), "destroyed")
+    refused(lambda: csr.bags(), "destroyed")
+    ctx.embed_grad(bags, order, out, grad)
+    refused(lambda: ctx.embed(None, table, out), "bags")
+    refused(lambda: ctx.embed(vec(4), table, out), "bags")
+    """)
