@@ -266,17 +266,20 @@ _BAGS = struct.Struct("PPPQQi4x").pack
 
 
 class DeviceMat:
-    """A row-major matrix in HBM (admm_mat): from a pointer, or `of` a torch tensor on the context's GPU"""
+    """A row-major matrix in HBM (admm_mat): from a pointer (`device`: the GPU it lies on, if calls are to check that), or `of` a
+    torch tensor on the context's GPU"""
 
-    __slots__ = ("rows", "cols", "packed")
+    __slots__ = ("rows", "cols", "packed", "device")
 
-    def __init__(self, ptr, rows, cols, type=F32, stride=None):
-        self.rows, self.cols = rows, cols
+    def __init__(self, ptr, rows, cols, type=F32, stride=None, device=None):
+        self.rows, self.cols, self.device = rows, cols, device
         self.packed = _MAT(ptr, rows, cols, cols if stride is None else stride, type)
 
     @classmethod
     def of(cls, ctx, m, name):
         if isinstance(m, DeviceMat):
+            if m.device is not None and m.device != ctx.device:
+                raise ctx._not_here(name, m.device)
             return m
         try:
             (rows, cols), (step, inner), kind = m.shape, m.stride(), _FLOATS[m.dtype]
@@ -290,7 +293,7 @@ class DeviceMat:
             if rows > 1:
                 raise AdmmError("%s: rows of %d elements lie %d apart" % (name, cols, step))
             step = cols
-        return cls(m.data_ptr(), rows, cols, kind, step)
+        return cls(m.data_ptr(), rows, cols, kind, step, ctx.device)
 
 
 def _not_a_matrix(m, name):
@@ -303,12 +306,12 @@ def _not_a_matrix(m, name):
 
 class Bags:
     """Rows of ids (admm_bags); keeps the arrays alive, but for those of a sample set (`source`), which are asked for again at
-    every call that reads them"""
+    every call that reads them.  `device`: the GPU they lie on, where that is known"""
 
-    __slots__ = ("nrows", "nnz", "keep", "packed", "source")
+    __slots__ = ("nrows", "nnz", "keep", "packed", "source", "device")
 
-    def __init__(self, ids, rowptr, val, nrows, nnz, id_type, keep=(), source=None):
-        self.nrows, self.nnz, self.keep, self.source = nrows, nnz, keep, source
+    def __init__(self, ids, rowptr, val, nrows, nnz, id_type, keep=(), source=None, device=None):
+        self.nrows, self.nnz, self.keep, self.source, self.device = nrows, nnz, keep, source, device
         self.packed = _BAGS(ids or 0, rowptr or 0, val or 0, nrows, nnz, id_type)
 
 
@@ -429,6 +432,9 @@ class Context:
     def _elsewhere(self, t, name):
         return AdmmError("%s is on %s, the context on GPU %d" % (name, t.device, self.device))
 
+    def _not_here(self, name, device):
+        return AdmmError("%s is on GPU %d, the context on GPU %d" % (name, device, self.device))
+
     def _array(self, a, name, count, kinds):
         """(pointer, type) of `count` adjacent elements of one of the types"""
         if a is None:
@@ -451,8 +457,12 @@ class Context:
         if isinstance(a, DeviceVec):
             if F32 not in kinds or a.n < count:
                 raise AdmmError("%s: %d floats do not do for %d elements" % (name, a.n, count))
+            if a.ctx.device != self.device:
+                raise self._not_here(name, a.ctx.device)
             return a.ptr, F32
         if isinstance(a, DeviceBuf):
+            if a.vec.ctx.device != self.device:
+                raise self._not_here(name, a.vec.ctx.device)
             kind = kinds[0] if a.type is None and len(kinds) == 1 else a.type
             if kind not in kinds:
                 raise AdmmError("%s: %s" % (name, "a buffer that does not say its elements' type (buf(bytes, type=...))" if kind is None
@@ -464,6 +474,8 @@ class Context:
 
     def _bytes(self, buf, name):
         if isinstance(buf, DeviceBuf):
+            if buf.vec.ctx.device != self.device:
+                raise self._not_here(name, buf.vec.ctx.device)
             return buf.ptr, buf.nbytes
         if not hasattr(buf, "data_ptr"):
             raise AdmmError("%s: a DeviceBuf or a torch tensor is needed, not %s" % (name, buf.__class__.__name__))
@@ -506,12 +518,14 @@ class Context:
             q, _ = self._array(rowptr, "rowptr", nrows + 1, (I64,))
         if val is not None:
             f, _ = self._array(val, "val", nnz, (F32,))
-        return Bags(p, q, f, nrows, nnz, kind, (ids, rowptr, val))
+        return Bags(p, q, f, nrows, nnz, kind, (ids, rowptr, val), device=self.device)
 
     def _bags(self, bags, read=True):
         """what the library is told of the bags; `read`: it reads their arrays, not the counts alone"""
         if bags.__class__ is not Bags:
             raise AdmmError("bags: Context.bags() or SampleSet.bags() makes them, not %s" % bags.__class__.__name__)
+        if bags.device is not None and bags.device != self.device:
+            raise self._not_here("bags", bags.device)
         return C.byref(bags.source._rows()) if read and bags.source is not None else bags.packed
 
     def embed(self, bags, table, out, scale=1.0):
@@ -662,7 +676,7 @@ class SampleSet:
         """the set's rows as bags for Context.embed / embed_grad (admm_csr_bags).  They are the set's arrays: once it is destroyed,
         relabelled, or lean and without its rows, calls that read them are refused (embed_grad takes only counts from them)"""
         b = self._rows()
-        return Bags(b.ids, b.rowptr, b.val, b.nrows, b.nnz, b.id_type, source=self)
+        return Bags(b.ids, b.rowptr, b.val, b.nrows, b.nnz, b.id_type, source=self, device=self.ctx.device)
 
     def build_transposed(self, panel_rows=0, col_block=0):
         _check(self.ctx.L.admm_csr_build_transposed(self.h, int(panel_rows), int(col_block)))

@@ -67,3 +67,30 @@ def test_bags_of_a_set_that_is_gone(recorder):  # noqa: F811
     refused(lambda: ctx.embed(None, table, out), "bags")
     refused(lambda: ctx.embed(vec(4), table, out), "bags")
     """)
+
+
+def test_memory_of_another_contexts_gpu(recorder):  # noqa: F811
+    """vectors, buffers, bags and matrices that are known to lie on another GPU are refused, as tensors are"""
+    check(recorder, """
+    other = capi.Context(1, stream=0x7000)
+    csr = other.csr_upload(np.array([0, 2, 3], np.uint64), np.array([0, 5, 7]), None, np.array([0, 1.]), 64)
+    x, loss, lab, u, tok, far = mat(4, 8), vec(4), vec(4), vec(4), ctx.buf(16), other.vec(4096)
+    table, out, grad, mine = mat(64, 8), mat(2, 8), mat(64, 8), ids(2)
+    refused(lambda: ctx.embed(csr.bags(), table, out), "bags")
+    refused(lambda: ctx.embed_order(csr.bags(), 64), "bags")
+    order = other.embed_order(csr.bags(), 64)
+    refused(lambda: ctx.embed_grad(csr.bags(), order, out, grad), "bags")
+    refused(lambda: ctx.embed_grad(mine, order, out, grad), "order")
+    refused(lambda: ctx.embed_order(mine, 64, other.buf(1 << 16)), "order")
+    refused(lambda: ctx.softmax_loss(x, far, loss), "labels")
+    refused(lambda: ctx.softmax_loss(x, lab, far), "loss")
+    refused(lambda: ctx.softmax_loss(x, lab, loss, weight=far), "weight")
+    refused(lambda: ctx.sample(x, u, other.buf(16)), "token")
+    refused(lambda: ctx.sample(x, u, tok, workspace=other.buf(1 << 16)), "workspace")
+    there = capi.DeviceMat(far.ptr.value, 4, 8, device=1)
+    refused(lambda: ctx.sample(there, u, tok), "logits")
+    refused(lambda: ctx.embed(mine, there, mat(2, 8)), "table")
+    ctx.sample(x, u, tok)
+    other.sample(there, far, other.buf(16))
+    ctx.embed(mine, mat(4, 8), mat(2, 8))      # bags and matrices from pointers may be anywhere: the caller knows
+    """)
