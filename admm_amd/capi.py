@@ -459,10 +459,14 @@ class Context:
                 raise AdmmError("%s: %d floats do not do for %d elements" % (name, a.n, count))
             if a.ctx.device != self.device:
                 raise self._not_here(name, a.ctx.device)
+            if not a.ptr and count:
+                raise AdmmError("%s was freed" % name)
             return a.ptr, F32
         if isinstance(a, DeviceBuf):
             if a.vec.ctx.device != self.device:
                 raise self._not_here(name, a.vec.ctx.device)
+            if not a.ptr:
+                raise AdmmError("%s was freed" % name)
             kind = kinds[0] if a.type is None and len(kinds) == 1 else a.type
             if kind not in kinds:
                 raise AdmmError("%s: %s" % (name, "a buffer that does not say its elements' type (buf(bytes, type=...))" if kind is None
@@ -476,6 +480,8 @@ class Context:
         if isinstance(buf, DeviceBuf):
             if buf.vec.ctx.device != self.device:
                 raise self._not_here(name, buf.vec.ctx.device)
+            if not buf.ptr:
+                raise AdmmError("%s was freed" % name)
             return buf.ptr, buf.nbytes
         if not hasattr(buf, "data_ptr"):
             raise AdmmError("%s: a DeviceBuf or a torch tensor is needed, not %s" % (name, buf.__class__.__name__))

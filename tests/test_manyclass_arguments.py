@@ -94,3 +94,21 @@ def test_memory_of_another_contexts_gpu(recorder):  # noqa: F811
     other.sample(there, far, other.buf(16))
     ctx.embed(mine, mat(4, 8), mat(2, 8))      # bags and matrices from pointers may be anywhere: the caller knows
     """)
+
+
+def test_freed_vectors_are_not_absent_ones(recorder):  # noqa: F811
+    """a weight, temperature or filter whose memory was freed is not taken for one that was not given"""
+    check(recorder, """
+    x, loss, lab, u, tok = mat(4, 8), vec(4), vec(4), vec(4), ctx.buf(16)
+    gone, k = vec(4), ctx.buf(16)
+    gone.free(), k.free()
+    refused(lambda: ctx.softmax_loss(x, lab, loss, weight=gone), "weight")
+    refused(lambda: ctx.softmax_loss(x, lab, loss, lse=gone), "lse")
+    for name in ("logprob", "temperature", "top_p", "min_p"):
+        refused(lambda: ctx.sample(x, u, tok, **{name: gone}), name)
+    refused(lambda: ctx.sample(x, u, tok, top_k=k), "top_k")
+    refused(lambda: ctx.embed_order(ids(4), 8, k), "order")
+    refused(lambda: ctx.sample(x, u, tok, workspace=k), "workspace")
+    none = capi.DeviceVec.from_ptr(ctx, 0, 0)
+    ctx.softmax_loss(capi.DeviceMat(0, 0, 8), none, none, weight=none)   # nothing of nothing
+    """)
