@@ -114,7 +114,17 @@ inline uint64_t mat_span(const admm_mat *m) {
   return m->rows && m->cols ? ((m->rows - 1) * m->stride + m->cols) * type_bytes(m->type) : 0;
 }
 
-inline bool mats_overlap(const admm_mat *a, const admm_mat *b) { return overlap(a->data, mat_span(a), b->data, mat_span(b)); }
+// Do they share an element?  Rows of one stride may lie side by side: then their places within the stride tell.
+inline bool mats_overlap(const admm_mat *a, const admm_mat *b) {
+  if (!overlap(a->data, mat_span(a), b->data, mat_span(b))) return false;
+  const uint64_t na = a->cols * type_bytes(a->type), nb = b->cols * type_bytes(b->type);
+  const uint64_t sa = a->stride * type_bytes(a->type), sb = b->stride * type_bytes(b->type);
+  if ((a->rows <= 1 && b->rows <= 1) || (a->rows > 1 && b->rows > 1 && sa != sb)) return true;
+  const uint64_t stride = a->rows > 1 ? sa : sb;
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a->data), y = reinterpret_cast<uintptr_t>(b->data);
+  const uint64_t from = y >= x ? (y - x) % stride : (stride - (x - y) % stride) % stride;  // where b's rows begin, from a's on
+  return from < na || from + nb > stride;
+}
 
 // can rows of this matrix be read and written n elements at a time from column 0 on?
 inline bool rows_aligned(const admm_mat *m, uint64_t n) {
