@@ -314,8 +314,8 @@ int admm_consensus_static(void *stream, const float *sum, int num_worker, float 
  *     the contents before and after a call mean nothing).  So every call may be captured into a HIP graph (with
  *     admm_timing_enable off); calls, and replays of graphs, that can run at the same time need workspaces of their
  *     own.  The calling thread's current device is left as it was.
- *   - Floating sums are held in 32 bits or more and in an order that depends on the shapes and the ids alone: the same
- *     call gives the same bits.  A result is rounded once to the type of its matrix.
+ *   - Floating sums are held in 32 bits or more and in an order that depends on the shapes, the ids and the rows' alignment
+ *     to 16 bytes alone: the same call gives the same bits.  A result is rounded once to the type of its matrix.
  *   - Where a shape has no elements, nothing is launched and the call succeeds. */
 
 #define ADMM_F32 0
