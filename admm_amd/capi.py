@@ -524,15 +524,15 @@ class Context:
             q, _ = self._array(rowptr, "rowptr", nrows + 1, (I64,))
         if val is not None:
             f, _ = self._array(val, "val", nnz, (F32,))
-        return Bags(p, q, f, nrows, nnz, kind, (ids, rowptr, val), device=self.device)
+        return Bags(p, q, f, nrows, nnz, kind, (ids, rowptr, val), None, self.device)
 
     def _bags(self, bags, read=True):
         """what the library is told of the bags; `read`: it reads their arrays, not the counts alone"""
         if bags.__class__ is not Bags:
             raise AdmmError("bags: Context.bags() or SampleSet.bags() makes them, not %s" % bags.__class__.__name__)
-        if bags.device is not None and bags.device != self.device:
+        if bags.device != self.device and bags.device is not None:
             raise self._not_here("bags", bags.device)
-        return C.byref(bags.source._rows()) if read and bags.source is not None else bags.packed
+        return bags.source._rows() if read and bags.source is not None else bags.packed
 
     def embed(self, bags, table, out, scale=1.0):
         """admm_embed: out[r] = scale * sum of val_e * table[id_e] over the entries of row r"""
@@ -656,6 +656,8 @@ class SampleSet:
         a, b, c = C.c_uint64(), C.c_uint64(), C.c_uint64()
         _check(ctx.L.admm_csr_shape(self.h, C.byref(a), C.byref(b), C.byref(c)))
         self.nrows, self.nnz, self.dim = a.value, b.value, c.value
+        self._bags = BagsStruct()
+        self._bags_ref = C.byref(self._bags)
 
     def destroy(self):
         if self.h:
@@ -672,16 +674,17 @@ class SampleSet:
         return rowptr, col[:self.nnz], val[:self.nnz], label[:self.nrows]
 
     def _rows(self):
+        """what admm_csr_bags says now, as a pointer to it"""
         if not self.h:
             raise AdmmError("bags: the sample set was destroyed")
-        b = BagsStruct()
-        _check(self.ctx.L.admm_csr_bags(self.h, C.byref(b)))
-        return b
+        _check(self.ctx.L.admm_csr_bags(self.h, self._bags_ref))
+        return self._bags_ref
 
     def bags(self):
         """the set's rows as bags for Context.embed / embed_grad (admm_csr_bags).  They are the set's arrays: once it is destroyed,
         relabelled, or lean and without its rows, calls that read them are refused (embed_grad takes only counts from them)"""
-        b = self._rows()
+        self._rows()
+        b = self._bags
         return Bags(b.ids, b.rowptr, b.val, b.nrows, b.nnz, b.id_type, source=self, device=self.ctx.device)
 
     def build_transposed(self, panel_rows=0, col_block=0):
