@@ -1137,7 +1137,10 @@ extern "C" int admm_embed_grad_workspace(const admm_bags *bags, uint64_t cols, u
   ADMM_REQUIRE(bytes, "admm_embed_grad_workspace: bytes is NULL");
   ADMM_TRY(check_bags(bags, "admm_embed_grad_workspace"));
   ADMM_REQUIRE(cols < (1ull << 40), "admm_embed_grad_workspace: %llu columns", (unsigned long long)cols);
-  *bytes = bags->nnz > grad_chunk(bags->nnz, cols) ? grad_parts_bytes(bags->nnz, cols) : 0;
+  *bytes = 0;
+  if (bags->nnz <= grad_chunk(bags->nnz, cols)) return ADMM_OK;
+  ADMM_TRY(check_tiles((cols + 511) / 512, "admm_embed_grad_workspace", cols));  // more columns are refused, whatever their alignment
+  *bytes = grad_parts_bytes(bags->nnz, cols);
   return ADMM_OK;
 }
 

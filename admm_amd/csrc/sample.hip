@@ -1108,8 +1108,8 @@ using namespace admm_impl;
 
 extern "C" int admm_sample_workspace(uint64_t rows, uint64_t cols, uint64_t *bytes) {
   ADMM_REQUIRE(bytes, "admm_sample_workspace: bytes is NULL");
-  ADMM_REQUIRE(rows < (1ull << 40) && cols <= kMaxClasses, "admm_sample_workspace: %llu x %llu logits", (unsigned long long)rows,
-               (unsigned long long)cols);
+  ADMM_REQUIRE(rows < (1ull << 40) && cols <= kMaxClasses && (unsigned __int128)rows * cols < ((unsigned __int128)1 << 46),
+               "admm_sample_workspace: %llu x %llu logits", (unsigned long long)rows, (unsigned long long)cols);
   *bytes = 0;
   if (cols <= kLaneCols || (cols <= kSmallCols && rows >= kSmallRows)) return ADMM_OK;
   // enough for logits of any type: granules of four floats or of eight halves
