@@ -518,6 +518,8 @@ class Context:
         p, kind = self._array(ids, "ids", nnz, (I32, I64))
         nrows, q, f = nnz, None, None
         if rowptr is not None:
+            if not hasattr(rowptr, "data_ptr"):
+                raise AdmmError("rowptr: a torch tensor is needed")
             nrows = rowptr.numel() - 1
             if nrows < 0:
                 raise AdmmError("rowptr: no element")

@@ -112,3 +112,27 @@ def test_freed_vectors_are_not_absent_ones(recorder):  # noqa: F811
     none = capi.DeviceVec.from_ptr(ctx, 0, 0)
     ctx.softmax_loss(capi.DeviceMat(0, 0, 8), none, none, weight=none)   # nothing of nothing
     """)
+
+
+def test_bags_of_something_else(recorder):  # noqa: F811
+    """row pointers and factors that are no tensors are refused as ids are"""
+    check(recorder, """
+    class Tensor:
+        def __init__(self, n, dtype):
+            self.n, self.dtype, self.mem, self.shape = n, dtype, vec(2 * n + 2), (n,)
+        data_ptr = lambda self: self.mem.ptr.value
+        numel = lambda self: self.n
+        get_device = lambda self: 0
+        is_contiguous = lambda self: True
+        stride = lambda self: (1,)
+    capi._ARRAYS.update({"i64": capi.I64, "f32": capi.F32})
+    t = Tensor(4, "i64")
+    ctx.embed(ctx.bags(t), mat(8, 2), mat(4, 2))
+    ctx.embed(ctx.bags(t, Tensor(3, "i64"), Tensor(4, "f32")), mat(8, 2), mat(2, 2))
+    for other in (np.zeros(3, np.int64), [0, 2, 4], vec(4)):
+        refused(lambda: ctx.bags(t, other), "rowptr")
+    refused(lambda: ctx.bags(t, Tensor(3, "f32")), "rowptr")
+    refused(lambda: ctx.bags(t, Tensor(0, "i64")), "rowptr")
+    refused(lambda: ctx.bags(np.zeros(3, np.int64)), "ids")
+    refused(lambda: ctx.bags(t, Tensor(3, "i64"), np.ones(4, np.float32)), "val")
+    """)
