@@ -335,7 +335,8 @@ typedef struct admm_mat {
 /* Rows of ids in DEVICE memory.  rowptr == NULL: one id per row (tokens), nnz == nrows.  Else row r holds the entries
  * [rowptr[r], rowptr[r+1]) (a sample set's rows; a row may be empty; what lies beyond nnz is not read).  An id outside
  * the table (-1 in a padded batch) stands for nothing: it adds zero and receives no gradient.  So does an entry whose
- * factor is 0, whatever its row holds.
+ * factor is 0, whatever its row holds.  Row pointers do not decrease: rows that share entries are looked up as they stand, but
+ * the gradient takes an entry for one of its rows only, any of them.
  * Limits: nrows, nnz and the table's rows at most 2^32 - 256. */
 typedef struct admm_bags {
   const void *ids;
@@ -364,7 +365,8 @@ int admm_embed_order(admm_ctx *ctx, const admm_bags *bags, uint64_t table_rows, 
 /* The gradient of admm_embed with respect to its table: for every table row v the sum over the entries with id v of
  * scale * val_e * grad_out[row_e, :].  accumulate == 0 writes every row of grad_table (zeros where no entry is),
  * accumulate != 0 adds to it and touches no row without an entry.  grad_table has grad_out's type or ADMM_F32.  `bags` and
- * `order` are those of admm_embed_order with table_rows == grad_table->rows (only the counts in `bags` are used). */
+ * `order` are those of admm_embed_order with table_rows == grad_table->rows (of `bags`, only the counts and whether there are row
+ * pointers and factors are used: the arrays themselves may be gone). */
 int admm_embed_grad_workspace(const admm_bags *bags, uint64_t cols, uint64_t *bytes);
 int admm_embed_grad(admm_ctx *ctx, const admm_bags *bags, const void *order, uint64_t order_bytes,
                     const admm_mat *grad_out, float scale, int accumulate, const admm_mat *grad_table, void *workspace,
@@ -374,8 +376,8 @@ int admm_embed_grad(admm_ctx *ctx, const admm_bags *bags, const void *order, uin
  *   lse[r] = log sum_j exp(x_j),  loss[r] = w (lse[r] - x_t),  grad[r, j] = grad_scale * w * (exp(x_j - lse[r]) - [j == t]).
  * labels: DEVICE array of label_type ADMM_I32, ADMM_I64 or ADMM_F32 (a sample set's labels, truncated).  A row whose label
  * is outside [0, cols) or whose weight is 0 is not trained on: loss 0, gradient 0.  Logits of -inf are classes that are
- * masked out: probability 0, gradient 0.  A row whose label is masked has loss +inf; one with no class left has loss +inf
- * and gradient 0 (lse -inf).  A NaN, or a logit of +inf, makes its row NaN.
+ * masked out: probability 0, gradient 0.  A row whose label is masked has loss +inf, times its weight (and, by the formula,
+ * -grad_scale * w in the label's gradient); one with no class left has loss +inf and gradient 0 (lse -inf).  A NaN, or a logit of +inf, makes its row NaN.
  * lse and grad may be NULL (not wanted); grad has the logits' shape and type and may be the logits' own memory (same data
  * and stride), else it may not overlap them.  cols <= 2^31 - 256. */
 int admm_softmax_loss_workspace(uint64_t rows, uint64_t cols, uint64_t *bytes);
@@ -396,7 +398,9 @@ int admm_softmax_loss(admm_ctx *ctx, const admm_mat *logits, const void *labels,
  * nearest end, NaN as 0.  NaN logits count as -inf; a row without any logit above -inf gives token -1 and logprob -inf;
  * logits of +inf share all the mass.
  * Weights are rounded to multiples of 2^-51 of the row's largest (for more than 2^11 classes of 2^-(62 - ceil(log2 cols)))
- * and summed as integers, so a draw does not depend on the batch it is in.  cols <= 2^31 - 256. */
+ * and summed as integers, so a draw does not depend on the batch it is in; before that they are off by up to 2.2e-12 of
+ * themselves (the exponential's polynomial).  So a class below half of such a unit is never drawn, but for uniform[r] = 0, which
+ * takes the first kept class above 2^-1075 of the largest weight.  cols <= 2^31 - 256. */
 typedef struct admm_sample_params {
   const float *temperature;
   const int32_t *top_k;
