@@ -75,9 +75,10 @@ __device__ inline void add_groups(int lanes_log2, float (&acc)[N]) {
 }
 
 // Rows of several ids.  WAVES waves share a row (1, or 16 for few long ones), each of them as 64 /
-// 2^lanes_log2 groups of lanes that take entries in turn.  65536 rows of 40 entries over 16 floats: 36 us, bound by requests
-// (2.6 million rows of 64 bytes in four 16-byte lanes each; the units that form the addresses are busy for half of the time, and an
-// entry is two reads one behind the other), not by the 75 MB that come.  65536 x 40 x 256: 441 us, 6.1 TB/s.
+// 2^lanes_log2 groups of lanes that take entries in turn.  65536 rows of 40 entries over 16 floats: 36 us, bound by scattered
+// requests to memory: 1.17 million of them (half of the 2.34 million that reach L2 hit there), 32 a ns, where a lookup of 2^24
+// distinct rows of 64 bytes in random order reaches 40 (2.5 TB/s; rows of 128 bytes 33 a ns, 4.2 TB/s).  Waves wait for 69 % of
+// their cycles, the units that form the addresses are busy for 45 %.  65536 x 40 x 256: 441 us, 6.1 TB/s.
 template <class T, class TO, int N, class Id, int WAVES>
 __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
     k_embed_bags(const Id *__restrict__ ids, const uint64_t *__restrict__ rowptr, const float *__restrict__ val, uint64_t nrows,

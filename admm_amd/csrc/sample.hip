@@ -890,7 +890,9 @@ __global__ void __launch_bounds__(kThreads) k_sample_rest(SampleArgs a, uint64_t
 // is kept, those over the classes where they are give the token.  No row is left to anyone else.  With more than kLaneCols
 // classes the sort is long for one wave (33 us where the kernels above take 23), so that fewer than kSmallRows rows that need
 // it go there: 64 rows of 1000 with top-k 33 and 24 us, 512 35 and 32, with top-p 37 and 41, 8192 137 and 417; without either
-// filter there is no sort and this is faster, 64 rows 8 and 13.
+// filter there is no sort and this is faster, 64 rows 8 and 13.  That holds for shorter rows, whose few groups leave a larger k to
+// draw_row: 64 rows in 16 bits by the kernels above, and 512 by the sort, with k = 90 of 520 classes 23 and 34 us, of 640 23 and
+// 35, of 800 27 and 35; with top-p beside it 30, 30, 34 and 36, 36, 36.
 constexpr uint64_t kSmallCols = 1024, kLaneCols = 512, kSmallRows = 512;
 
 template <class T, int LANES, int EACH>
