@@ -588,7 +588,7 @@ __device__ inline void put_part(const GradArgs<T, TO> &a, uint32_t chunk, int sl
 //    fixed order and without atomics, whatever the ids.
 //  * zeros (only where every row has to be written): rows of the table that no entry names.
 // 16384 entries of 2048 columns, bf16 added to f32: 43 us at 128 MB (reads and writes of touched rows, in no order).  2.6 million
-// entries of 16 floats: 47 us, half of it address work as in the lookup; 71 MB are written, 78 read.
+// entries of 16 floats: 47 us; 71 MB are written, 78 read in 1.2 million requests, 26 a ns (scattered as the lookup's).
 template <class T, class TO, int N>
 __global__ void __launch_bounds__(256) k_grad(GradArgs<T, TO> a) {
   const Place<N> p(a.lanes_log2, a.cols);
