@@ -530,7 +530,7 @@ class Context:
 
     def _bags(self, bags, read=True):
         """what the library is told of the bags; `read`: it reads their arrays, not the counts alone"""
-        if bags.__class__ is not Bags:
+        if not isinstance(bags, Bags):
             raise AdmmError("bags: Context.bags() or SampleSet.bags() makes them, not %s" % bags.__class__.__name__)
         if bags.device != self.device and bags.device is not None:
             raise self._not_here("bags", bags.device)
