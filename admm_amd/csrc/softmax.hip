@@ -1,8 +1,10 @@
 // Softmax loss with its gradient: the many-class form of the logistic loss and its residuals.
 //
 // With L = log2(e) and m the row's largest logit, the exponentials are 2^(x L - m L) (one fused multiply-add and one
-// hardware exp2 each), s their sum, and
-//   loss = ln 2 (log2 s - (x_t L - m L)),  grad = 2^(x L - m L) w / s - [j = t] w.
+// hardware exp2 each), o the sum of all but the label's, s = o + 2^(x_t L - m L), and
+//   loss = ln 2 (log2 s - (x_t L - m L)),  grad = 2^(x L - m L) w / s, at the label -w o / s.
+// The label is left out of o, not taken off s: a row that is nearly sure of its label has a loss and a gradient far below 1, of
+// which p - 1 and log s would keep 2^-24 of 1 only (its loss is log1p of o over the label's power).
 // Both read x L - m L through the same rounded m L, so its rounding cancels (log2 s in the exponent instead of the division
 // would add half a step of m L to it, 2e-6 of a probability where m is 30).  Where m L would overflow (a mask of the type's
 // lowest value over a whole row), 1 takes the place of L: logits of that size are equal or more than 2^100 apart.
@@ -82,16 +84,39 @@ __device__ inline void stay_packed(V &x) {
   x = __builtin_bit_cast(V, u);
 }
 
-// the gradient of a chunk; `at`: which of its elements the label is, or anything else
+// Takes the label out of a chunk before its sum; `at`: which of its elements it is, or anything else.  On the packed words, three
+// instructions each: element by element it is three times as many, and registers with them.
 template <class T>
-__device__ inline vec_t<T, 16 / sizeof(T)> chunk_grad(const vec_t<T, 16 / sizeof(T)> &x, Shift b, float share, float g, int at) {
+__device__ inline void take_out(vec_t<T, 16 / sizeof(T)> &x, int at) {
+  u32x4 u = __builtin_bit_cast(u32x4, x);
+  if (sizeof(T) == 4) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) u[k] = at == k ? 0xFF800000u : u[k];
+  } else {
+    constexpr uint32_t none = std::is_same<T, bf16_t>::value ? 0xFF80u : 0xFC00u;  // -inf
+    const uint32_t mask = at & 1 ? 0xFFFF0000u : 0xFFFFu, put = none << 16 | none;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t here = at >> 1 == k ? mask : 0u;
+      u[k] = (u[k] & ~here) | (put & here);
+    }
+  }
+  x = __builtin_bit_cast(vec_t<T, 16 / sizeof(T)>, u);
+}
+
+// the label's power; 0 where there is no label
+__device__ inline float label_power(int64_t t, float xt, Shift b) { return t >= 0 ? exp2_fast(__fmaf_rn(xt, b.l, -b.m2)) : 0.0f; }
+
+// the gradient of a chunk; `at`: which of its elements the label is, or anything else; gl: the label's, negated
+template <class T>
+__device__ inline vec_t<T, 16 / sizeof(T)> chunk_grad(const vec_t<T, 16 / sizeof(T)> &x, Shift b, float share, float gl = 0.0f, int at = -1) {
   constexpr int K = 16 / sizeof(T);
   float v[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) v[k] = share * exp2_fast(__fmaf_rn((float)x[k], b.l, -b.m2));
-  if (at >= 0 && at < K) {
+  if ((unsigned)at < (unsigned)K) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] -= at == k ? g : 0.0f;
+    for (int k = 0; k < K; ++k) v[k] = at == k ? -gl : v[k];
   }
   vec_t<T, K> y;
 #pragma unroll
@@ -99,49 +124,73 @@ __device__ inline vec_t<T, 16 / sizeof(T)> chunk_grad(const vec_t<T, 16 / sizeof
   return y;
 }
 
-// loss and lse of a row with the label t
-__device__ inline void finish_row(const SoftmaxArgs &a, uint64_t r, Shift b, float s, int64_t t, float w, float xt) {
+// log(1 + x) of 0 <= x < 1, right relative to itself: what 1 + x loses of x, log(1 + x) loses too
+__device__ inline float log1p_fast(float x) {
+  const float y = 1.0f + x, got = y - 1.0f;
+  return got == 0.0f ? x : kLn2 * __log2f(y) * (x * __builtin_amdgcn_rcpf(got));
+}
+
+// loss and lse of a row with the label t, whose power is e; the others' sum is `others`
+__device__ inline void finish_row(const SoftmaxArgs &a, uint64_t r, Shift b, float others, float e, int64_t t, float w, float xt) {
+  const float s = others + e;
   const float log2s = __log2f(s);  // -inf where no class is left
   const float nats = b.l == 1.0f ? 1.0f : kLn2;
   if (a.lse) a.lse[r] = s == 0.0f ? -INFINITY : b.m2 * nats + log2s * kLn2;
   // (a label masked by the type's lowest value: x_t L would overflow)
   const float off = fabsf(xt) < 0x1p100f ? nats * __fmaf_rn(xt, b.l, -b.m2) : xt - nats * b.m2;
-  a.loss[r] = t < 0 ? 0.0f : s == 0.0f ? INFINITY * w : w * (kLn2 * log2s - off);
+  a.loss[r] = t < 0 ? 0.0f : s == 0.0f ? INFINITY * w : others < e ? w * log1p_fast(others * __builtin_amdgcn_rcpf(e)) : w * (kLn2 * log2s - off);
 }
 
-// Rows of up to 64 CH chunks: 2^lanes_log2 lanes hold a row, CH chunks each, and reduce it among themselves.
+// Rows of up to 64 CH chunks: 2^lanes_log2 lanes hold a row, CH chunks each, and reduce it among themselves.  With more than one
+// chunk a lane the label's is left out of the sum whole, and its other elements are added by one lane each.
 template <class T, int CH>
 __global__ void __launch_bounds__(256) k_softmax_lanes(SoftmaxArgs a) {
   constexpr int K = 16 / sizeof(T);
+  constexpr bool kAside = CH > 1;  // 64 lanes a row, more than a chunk has elements
   const unsigned lanes = 1u << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
   const uint64_t per = 256u >> a.lanes_log2;
   const T none = (T)-INFINITY;
   for (uint64_t r = (uint64_t)blockIdx.x * per + (threadIdx.x >> a.lanes_log2); r < a.rows; r += (uint64_t)gridDim.x * per) {
     float w;
     const int64_t t = label_of(a, r, w);
-    const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int)a.cols);
+    const T *const from = static_cast<const T *>(a.logits) + r * a.stride;
+    const Chunks<T> row(from, (int)a.cols);
     T *to = a.grad ? static_cast<T *>(a.grad) + r * a.gstride : nullptr;
     vec_t<T, K> x[CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c)
       if ((int)(c * lanes + lane) < row.count) x[c] = row.load(c * lanes + lane, none);
       else x[c] = none;
-    const float xt = t >= 0 ? (float)row.base[row.lead + t] : 0.0f;
+    const float xt = (float)from[t >= 0 ? t : 0];
+    const int tc = t < 0 ? -1 : (int)t + row.lead;
+    int label_chunk = t < 0 ? -1 : tc / K;
+    asm volatile("" : "+v"(label_chunk));  // or the compiler traces it back to the logits' address and no longer sees that they are global memory
+    const int aside = kAside && t >= 0 && lane < K ? row.column(label_chunk, (int)lane) : -1;
+    const bool is_loose = (aside >= 0) & (aside < row.cols) & (aside != (int)t);
+    const float at_loose = kAside ? (float)from[is_loose ? aside : 0] : 0.0f;
     float m = -INFINITY;
 #pragma unroll
     for (int c = 0; c < CH; ++c) m = chunk_max<T>(x[c], m);
     for (unsigned off = 1; off < lanes; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
     const Shift b(m);
-    float s = 0.0f;
+    float others = 0.0f;
+    const float loose = is_loose ? at_loose : -INFINITY;
+    if (kAside) others = exp2_fast(__fmaf_rn(loose, b.l, -b.m2));
 #pragma unroll
-    for (int c = 0; c < CH; ++c) stay_packed(x[c]);
+    for (int c = 0; c < CH; ++c) {
+      if (!kAside) take_out<T>(x[c], tc - (c * (int)lanes + (int)lane) * K);
+      stay_packed(x[c]);
+    }
 #pragma unroll
-    for (int c = 0; c < CH; ++c) s += chunk_sum<T>(x[c], b);
-    for (unsigned off = 1; off < lanes; off <<= 1) s += __shfl_xor(s, off, 64);
-    if (lane == 0) finish_row(a, r, b, s, t, w, xt);
+    for (int c = 0; c < CH; ++c) {
+      const float part = chunk_sum<T>(x[c], b);
+      others += kAside && c * (int)lanes + (int)lane == label_chunk ? 0.0f : part;
+    }
+    for (unsigned off = 1; off < lanes; off <<= 1) others += __shfl_xor(others, off, 64);
+    const float e = label_power(t, xt, b), s = others + e;
+    if (lane == 0) finish_row(a, r, b, others, e, t, w, xt);
     if (!to) continue;
-    const float g = t < 0 ? 0.0f : w * a.grad_scale, share = g / s;
-    const int tc = t < 0 ? -1 : (int)t + row.lead;
+    const float share = (t < 0 ? 0.0f : w * a.grad_scale) / s, gl = share * others;
 #pragma unroll
     for (int c = 0; c < CH; ++c) stay_packed(x[c]);
 #pragma unroll
@@ -149,8 +198,10 @@ __global__ void __launch_bounds__(256) k_softmax_lanes(SoftmaxArgs a) {
       const int at = c * (int)lanes + (int)lane;
       if (at >= row.count) continue;
       const vec_t<T, K> zero = (T)0.0f;
-      row.store(to, a.apart, at, t < 0 || s == 0.0f ? zero : chunk_grad<T>(x[c], b, share, g, tc - at * K));
+      row.store(to, a.apart, at, t < 0 || s == 0.0f ? zero : chunk_grad<T>(x[c], b, share, gl, kAside ? -1 : tc - at * K));
     }
+    // over what this lane has just written there
+    if (kAside & (t >= 0) & ((label_chunk & ((int)lanes - 1)) == (int)lane)) to[t] = s == 0.0f ? (T)0.0f : (T)-gl;
   }
 }
 
@@ -192,7 +243,7 @@ struct Edges {
 
 // Rows of any length, one workgroup each: whole granules, CH a thread, kept in registers (CH > 0) or read again (CH == 0), and
 // the edges' elements one a thread.
-// Read and written once, this is bound by memory where several rows are at work on a CU: 5.6 TB/s for 8192 rows of 32000 in 16
+// Read and written once, this is bound by memory where several rows are at work on a CU: 5.7 TB/s for 8192 rows of 32000 in 16
 // bits.  Rows of 10^5 halves fill the registers of a CU alone, and what it computes between reading and writing (two
 // exponentials an element) shows: 4.1 TB/s.  Neither keeping a part in LDS so that two rows fit (3.8) nor fetching the next row
 // as this one leaves the registers (4.0) nor reading twice (3.4) is faster.
@@ -229,14 +280,23 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 4 : 1) k_softmax_block(Softmax
       if (tid == 0) a.loss[r] = 0.0f;
       continue;
     }
-    const float xt = t >= 0 ? (float)from[t] : 0.0f;  // before anyone writes over it
-    const float edge = tid < edges.count ? (float)from[edges.column(tid)] : -INFINITY;
+    const float xt = (float)from[t >= 0 ? t : 0];  // before anyone writes over it
+    // The label's chunk is not held or walked through with the others, which so need not ask for the label: its elements are loose
+    // ones like the edges', one a thread.  (Every chunk asked: 100 us for 1001 rows of 100003, this: 95.)
+    const int tc = t < 0 ? -1 : (int)t + row.lead - row.whole_from * K;
+    const int label_chunk = tc >= 0 && tc < count * K ? tc / K : -1;  // or the label is at an edge
+    int loose = -1;  // this thread's column
+    if (tid < edges.count) loose = edges.column(tid);
+    else if (label_chunk >= 0 && tid < edges.count + K) loose = row.column(row.whole_from + label_chunk, tid - edges.count);
+    const float at_loose = (float)from[loose >= 0 ? loose : 0];  // without a branch, which would wait for it before the row is asked for
+    float edge = loose >= 0 ? at_loose : -INFINITY;
+    float m = edge;  // the label is in the maximum, not in the sum
+    if (loose >= 0 && loose == (int)t) edge = -INFINITY;
     chunk x[CH ? CH : 1];
-    // One pass: the sum is kept relative to the running maximum, so that the exponentials are computed while the row arrives: 179
+    // One pass: the sum is kept relative to the running maximum, so that the exponentials are computed while the row arrives: 177
     // us for 8192 rows of 32000 where a maximum first and the sum after it takes 185.  With 16 granules a thread it needs more
-    // registers than there are: 97 us the other way for 1001 rows of 100003, 100 this way.
+    // registers than there are: 95 us the other way for 1001 rows of 100003, 100 this way.
     constexpr bool kOnePass = CH < 16;
-    float m = edge;
     Shift b(m);
     float s = exp2_fast(__fmaf_rn(edge, b.l, -b.m2));
     auto take = [&](const chunk &y) {
@@ -252,8 +312,9 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 4 : 1) k_softmax_block(Softmax
     if (CH) {
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
+        const int at = c * NT + tid;
         x[c] = none;
-        if (c * NT + tid < count) x[c] = in[c * NT + tid];
+        if (at < count && at != label_chunk) x[c] = in[at];
       }
       if (kOnePass) {
 #pragma unroll
@@ -263,7 +324,8 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 4 : 1) k_softmax_block(Softmax
         for (int c = 0; c < CH; ++c) m = chunk_max<T>(x[c], m);
       }
     } else {
-      for (int c = tid; c < count; c += NT) take(in[c]);
+      for (int c = tid; c < count; c += NT)
+        if (c != label_chunk) take(in[c]);
     }
     const float mine = m;
     const Shift was = b;
@@ -279,25 +341,23 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 4 : 1) k_softmax_block(Softmax
         s += chunk_sum<T>(x[c], b);
       }
     }
-    s = block_sum<NT>(s, sh[1]);
-    if (tid == 0) finish_row(a, r, b, s, t, w, xt);
+    const float others = block_sum<NT>(s, sh[1]), e = label_power(t, xt, b);
+    s = others + e;
+    if (tid == 0) finish_row(a, r, b, others, e, t, w, xt);
     if (to) {
-      const float g = t < 0 ? 0.0f : w * a.grad_scale, share = g / s;
-      const int tc = t < 0 ? -1 : (int)t + row.lead - row.whole_from * K;
+      const float share = (t < 0 ? 0.0f : w * a.grad_scale) / s, gl = share * others;
       const bool no = t < 0 || s == 0.0f;
-      if (tid < edges.count) {
-        const int j = edges.column(tid);
-        to[j] = no ? (T)0.0f : (T)(share * exp2_fast(__fmaf_rn(edge, b.l, -b.m2)) - (j == (int)t ? g : 0.0f));
-      }
+      if (loose >= 0) to[loose] = no ? (T)0.0f : (T)(loose == (int)t ? -gl : share * exp2_fast(__fmaf_rn(edge, b.l, -b.m2)));
       if (CH) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
           const int at = c * NT + tid;
           stay_packed(x[c]);
-          if (at < count) put(at, no ? zero : chunk_grad<T>(x[c], b, share, g, tc - at * K));
+          if (at < count && at != label_chunk) put(at, no ? zero : chunk_grad<T>(x[c], b, share));
         }
       } else {
-        for (int c = tid; c < count; c += NT) put(c, no ? zero : chunk_grad<T>(in[c], b, share, g, tc - c * K));
+        for (int c = tid; c < count; c += NT)
+          if (c != label_chunk) put(c, no ? zero : chunk_grad<T>(in[c], b, share));
       }
     }
     __syncthreads();  // sh is free again
@@ -340,8 +400,12 @@ __global__ void __launch_bounds__(256) k_softmax_pieces(SoftmaxArgs a, Piece *pi
   }
   m = block_max<256>(m, sh[0]);
   const Shift b(m);
+  // the label is in the maximum, not in the sum
+  const int tc = t < 0 ? -1 : (int)t + row.lead, label_chunk = t < 0 ? -1 : tc / K;
 #pragma unroll
   for (int i = 0; i < kPiece / 256; ++i) {
+    const bool labels = c0 + i * 256 == label_chunk;
+    if (__ballot(labels)) take_out<T>(x[i], labels ? tc - label_chunk * K : -1);
     stay_packed(x[i]);
     s += chunk_sum<T>(x[i], b);
   }
@@ -359,7 +423,8 @@ __global__ void __launch_bounds__(256) k_softmax_pieces_grad(SoftmaxArgs a, cons
   const int64_t t = label_of(a, r, w);
   const Chunks<T> row(static_cast<const T *>(a.logits) + r * a.stride, (int)a.cols);
   const vec_t<T, K> zero = (T)0.0f;
-  float s = 0.0f;
+  const float xt = label_logits[r];  // of a row that is not trained on it may be anything
+  float others = 0.0f, e = 0.0f;
   Shift b(0.0f);
   if (t >= 0 || a.lse) {
     // every wave for itself: its lanes take pieces in turn
@@ -369,22 +434,23 @@ __global__ void __launch_bounds__(256) k_softmax_pieces_grad(SoftmaxArgs a, cons
     b = Shift(m);
     for (unsigned i = threadIdx.x & 63; i < count; i += 64) {
       const Piece p = pieces[r * count + i];
-      s += p.m == -INFINITY ? p.s : p.s * moved(Shift(p.m), b);  // s of a piece without classes: 0, or NaN
+      others += p.m == -INFINITY ? p.s : p.s * moved(Shift(p.m), b);  // s of a piece without classes: 0, or NaN
     }
-    for (int off = 1; off < 64; off <<= 1) s += __shfl_xor(s, off, 64);
-    if (blockIdx.x == 0 && threadIdx.x == 0) finish_row(a, r, b, s, t, w, label_logits[r]);
+    for (int off = 1; off < 64; off <<= 1) others += __shfl_xor(others, off, 64);
+    e = label_power(t, xt, b);
+    if (blockIdx.x == 0 && threadIdx.x == 0) finish_row(a, r, b, others, e, t, w, xt);
   } else if (blockIdx.x == 0 && threadIdx.x == 0) {
     a.loss[r] = 0.0f;
   }
   if (!a.grad) return;
   T *const to = static_cast<T *>(a.grad) + r * a.gstride;
-  const float g = t < 0 ? 0.0f : w * a.grad_scale, share = g / s;
+  const float s = others + e, share = (t < 0 ? 0.0f : w * a.grad_scale) / s, gl = share * others;
   const int tc = t < 0 ? -1 : (int)t + row.lead;
 #pragma unroll
   for (int i = 0; i < kPiece / 256; ++i) {
     const int at = (int)blockIdx.x * kPiece + (int)threadIdx.x + i * 256;
     if (at >= row.count) break;
-    row.store(to, a.apart, at, t < 0 || s == 0.0f ? zero : chunk_grad<T>(row.load(at, (T)-INFINITY), b, share, g, tc - at * K));
+    row.store(to, a.apart, at, t < 0 || s == 0.0f ? zero : chunk_grad<T>(row.load(at, (T)-INFINITY), b, share, gl, tc - at * K));
   }
 }
 

@@ -373,7 +373,8 @@ int admm_embed_grad(admm_ctx *ctx, const admm_bags *bags, const void *order, uin
                     uint64_t workspace_bytes);
 
 /* Per row r with label t and weight w (weight == NULL: 1):
- *   lse[r] = log sum_j exp(x_j),  loss[r] = w (lse[r] - x_t),  grad[r, j] = grad_scale * w * (exp(x_j - lse[r]) - [j == t]).
+ *   lse[r] = log sum_j exp(x_j),  loss[r] = w (lse[r] - x_t),  grad[r, j] = grad_scale * w * (exp(x_j - lse[r]) - [j == t]),
+ * loss and gradient right relative to themselves, also where the row is nearly sure of its label.
  * labels: DEVICE array of label_type ADMM_I32, ADMM_I64 or ADMM_F32 (a sample set's labels, truncated).  A row whose label
  * is outside [0, cols) or whose weight is 0 is not trained on: loss 0, gradient 0.  Logits of -inf are classes that are
  * masked out: probability 0, gradient 0.  A row whose label is masked has loss +inf, times its weight (and, by the formula,
