@@ -427,8 +427,9 @@ class Context:
 
     # models with many classes or tokens -----------------------------------------------------
     # Matrices are torch tensors or DeviceMats, arrays are torch tensors, DeviceVecs (floats) or DeviceBufs (labels in one
-    # need its type: buf(bytes, type=I64)); what they point to belongs to this context's GPU, and the work is queued on this context's stream (make the context on the stream that
-    # the tensors are used on: Context(device, stream=torch.cuda.current_stream().cuda_stream or DEFAULT_STREAM)).
+    # need its type: buf(bytes, type=I64)); what they point to belongs to this context's GPU, and the work is queued on this
+    # context's stream (make the context on the stream that the tensors are used on:
+    # Context(device, stream=torch.cuda.current_stream().cuda_stream or DEFAULT_STREAM)).
     def _elsewhere(self, t, name):
         return AdmmError("%s is on %s, the context on GPU %d" % (name, t.device, self.device))
 
@@ -545,7 +546,8 @@ class Context:
         return self._size.value
 
     def embed_order(self, bags, table_rows, order=None):
-        """admm_embed_order: the entries sorted by id, into `order` (a DeviceBuf or a torch tensor of bytes; made if None)"""
+        """admm_embed_order: the entries sorted by id, into `order` (a DeviceBuf or a torch tensor of bytes; made if None, and then
+        the caller's to free())"""
         rows = self._bags(bags)
         if order is None:
             order = DeviceBuf.scratch(self, self.embed_order_bytes(bags, table_rows))
